@@ -13,7 +13,7 @@ import torch
 
 own = False
 
-GRAMMAR_ROW = 40          # bytes of a beam's grammar position
+GRAMMAR_ROW = 36          # bytes of a dlk_grammar_row: a beam's grammar position
 
 
 def _quantise(name, rows, n, dtype, pad=0):
