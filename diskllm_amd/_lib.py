@@ -22,6 +22,9 @@ DLK_ERR_FORMAT = -4
 DLK_STATUS_HISTORY_TOO_LONG = 1
 DLK_STATUS_SYNC_TIMEOUT = 2
 DLK_STATUS_UNSUPPORTED_ROW = 4
+DLK_STATUS_NOT_FINITE = 8
+F32, BF16, F16 = 0, 1, 2
+MAX_BEAMS = 64
 PATH_AUTO, PATH_ROW, PATH_FULL_EXACT, PATH_FULL_NO_WAIT = 0, 1, 2, 3
 
 OP_REPETITION, OP_FREQUENCY, OP_PRESENCE = 1, 2, 3
@@ -41,6 +44,35 @@ class Batch(C.Structure):
                 ("mask", C.c_void_p), ("mask_ld", C.c_int64), ("mask_row", C.c_void_p), ("rng", C.c_void_p),
                 ("out_ids", C.c_void_p), ("out_cand_ids", C.c_void_p), ("out_cand_probs", C.c_void_p),
                 ("out_cand_logprobs", C.c_void_p), ("status", C.c_void_p)]
+
+
+class BeamBatch(C.Structure):
+    """dlk_beam_batch (include/diskllm_amd.h)."""
+    _fields_ = [("logits", C.c_void_p), ("ld", C.c_int64), ("hist_off", C.c_void_p), ("hist_ids", C.c_void_p),
+                ("mask", C.c_void_p), ("mask_ld", C.c_int64), ("mask_row", C.c_void_p), ("scores", C.c_void_p),
+                ("lengths", C.c_void_p), ("finished", C.c_void_p), ("out_tokens", C.c_void_p),
+                ("out_parents", C.c_void_p), ("out_scores", C.c_void_p), ("out_lengths", C.c_void_p),
+                ("out_finished", C.c_void_p), ("status", C.c_void_p)]
+
+
+class BeamParams(C.Structure):
+    """dlk_beam_params (include/diskllm_amd.h)."""
+    _fields_ = [("beams", C.c_int), ("n_out", C.c_int), ("eos_id", C.c_int), ("length_penalty", C.c_float),
+                ("repeat_penalty", C.c_float), ("frequency_penalty", C.c_float), ("presence_penalty", C.c_float),
+                ("penalty_order", C.c_uint32), ("max_history", C.c_int)]
+
+
+class BeamState(C.Structure):
+    """dlk_beam_state (include/diskllm_amd.h)."""
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("bytes", C.c_int64), ("src_row", C.c_int64),
+                ("src_outer", C.c_int64), ("src_inner", C.c_int64), ("dst_row", C.c_int64), ("dst_outer", C.c_int64),
+                ("dst_inner", C.c_int64), ("n_outer", C.c_int), ("n_inner", C.c_int)]
+
+
+class BeamHistory(C.Structure):
+    """dlk_beam_history (include/diskllm_amd.h)."""
+    _fields_ = [("off", C.c_void_p), ("ids", C.c_void_p), ("tokens", C.c_void_p), ("max_history", C.c_int),
+                ("out_off", C.c_void_p), ("out_ids", C.c_void_p)]
 
 
 class SamplerConfig(C.Structure):
@@ -78,7 +110,8 @@ EXPORTS = [
     # include/diskllm_amd.h
     "dlk_seed_state", "dlk_sample", "dlk_sample_noalloc", "dlk_release_stream", "dlk_dfa_mask", "dlk_expf", "dlk_apply_penalties", "dlk_grammar_mode_of",
     "dlk_grammar_row_init", "dlk_grammar_row_feed", "dlk_grammar_mask", "dlk_grammar_advance", "dlk_sample_grammar",
-    "dlk_vocab_csr_from_gguf", "dlk_csr_token_str", "dlk_softcap",
+    "dlk_vocab_csr_from_gguf", "dlk_csr_token_str", "dlk_softcap", "dlk_quantize_rows", "dlk_logits_i8",
+    "dlk_beam_select", "dlk_beam_reorder",
     # include/sampler.h
     "sampler_create", "sampler_free", "sampler_apply_repetition_penalty", "sampler_apply_presence_penalty",
     "sampler_sample", "greedy_sample",
@@ -161,6 +194,17 @@ def lib() -> C.CDLL:
                                          C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]
         L.dlk_softcap.restype = C.c_int
         L.dlk_softcap.argtypes = [C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_float, C.c_void_p]
+        L.dlk_quantize_rows.restype = C.c_int
+        L.dlk_quantize_rows.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.c_int64,
+                                        C.c_void_p, C.c_void_p]
+        L.dlk_logits_i8.restype = C.c_int
+        L.dlk_logits_i8.argtypes = [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int,
+                                    C.c_int, C.c_int, C.c_float, C.c_void_p, C.c_int64, C.c_void_p]
+        L.dlk_beam_select.restype = C.c_int
+        L.dlk_beam_select.argtypes = [C.POINTER(BeamBatch), C.c_int, C.c_int, C.POINTER(BeamParams), C.c_void_p]
+        L.dlk_beam_reorder.restype = C.c_int
+        L.dlk_beam_reorder.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.POINTER(BeamState), C.c_int,
+                                       C.POINTER(BeamHistory), C.c_void_p]
         L.dlk_vocab_csr_from_gguf.restype = C.c_int
         L.dlk_vocab_csr_from_gguf.argtypes = [C.c_char_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int64,
                                               C.POINTER(C.c_int32), C.POINTER(C.c_int64)]

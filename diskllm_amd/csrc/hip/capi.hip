@@ -15,6 +15,7 @@
 #include "sampler_params.h"
 #include "sampler_topk.h"
 #include "sampler_full.h"
+#include "beam_select.h"
 #include "tanhf_glibc.h"
 
 extern "C" int dlk_launch_row_kernel(const dlk::RowParams *p, int rows, size_t lds_bytes, hipStream_t stream);
@@ -28,6 +29,7 @@ extern "C" int dlk_launch_long_history_penalties(float *logits, int64_t ld, int 
                                                  const uint64_t *rng, uint64_t *rng_saved, hipStream_t stream);
 extern "C" int dlk_launch_long_history_fixup(int rows, const int32_t *too_long, const uint64_t *rng_saved,
                                              uint64_t *rng, int32_t *out_ids, uint32_t *status, hipStream_t stream);
+extern "C" int dlk_launch_beam_select(const dlk::BeamParams *p, int groups, hipStream_t stream);
 extern "C" int dlk_launch_prepare_rows(const float *src, int64_t ld, float *dst, int64_t dld, int rows, int vocab,
                                        const uint32_t *mask, int64_t mask_ld, const int32_t *mask_row, float cap,
                                        hipStream_t stream);
@@ -39,6 +41,7 @@ constexpr int kMaxTopKLds = 4096;          /* larger top-k: candidates in global
 constexpr int kHcapDirect = 1024;          /* longer histories: penalties applied to a scratch copy first */
 constexpr size_t kFullWorkspace = (size_t)512 << 20;      /* workspace per launch of the fused kernel */
 constexpr size_t kGlobalTopkBudget = (size_t)256 << 20;   /* workspace per launch of the large-k row kernel */
+constexpr size_t kBeamWorkspace = (size_t)64 << 20;       /* workspace per launch of the beam selection */
 constexpr int kLsdWords = 256 + 16 * 256 + 16;            /* select_top_k_global's LDS words */
 
 size_t r16(size_t b) { return (b + 15) & ~(size_t)15; }
@@ -670,4 +673,56 @@ extern "C" int dlk_sample_noalloc(const dlk_batch *b, int rows, int vocab, const
     const int rc = sample_impl(b, rows, vocab, prm, stream);
     g_noalloc = false;
     return rc;
+}
+
+/* One step of a beam search (beam_select.hip), the groups in as many launches as the
+ * workspace's bound asks for. */
+extern "C" int dlk_beam_select(const dlk_beam_batch *b, int groups, int vocab, const dlk_beam_params *prm,
+                               hipStream_t stream) {
+    using namespace dlk;
+    if (!b || !prm || groups < 0 || vocab <= 0 || !b->logits || b->ld < vocab) return DLK_ERR_INVALID;
+    if (!b->out_tokens || !b->out_parents || !b->out_scores) return DLK_ERR_INVALID;
+    if (prm->beams <= 0 || prm->n_out <= 0 || prm->max_history < 0) return DLK_ERR_INVALID;
+    if ((b->hist_off == nullptr) != (b->hist_ids == nullptr)) return DLK_ERR_INVALID;
+    if (b->mask && b->mask_ld < (vocab + 31) / 32) return DLK_ERR_INVALID;
+    if (prm->eos_id < -1 || prm->eos_id >= vocab || (b->finished && prm->eos_id < 0)) return DLK_ERR_INVALID;
+    if (!(fabsf(prm->length_penalty) <= 16.0f)) return DLK_ERR_INVALID;
+    if (((uintptr_t)b->logits & 3) != 0) return DLK_ERR_INVALID;
+    if (prm->beams > DLK_MAX_BEAMS || prm->n_out > DLK_MAX_BEAMS) return DLK_ERR_UNSUPPORTED;
+    if (prm->max_history > 65535 || vocab > 0x7fffffff - kBeamSlice) return DLK_ERR_UNSUPPORTED;
+    if ((int64_t)groups * prm->beams > 0x7fffffff || (int64_t)groups * prm->n_out > 0x7fffffff) return DLK_ERR_UNSUPPORTED;
+    if (groups == 0) return DLK_OK;
+    BeamParams p;
+    memset(&p, 0, sizeof(p));
+    p.logits = b->logits; p.ld = b->ld; p.V = vocab;
+    p.hist_off = b->hist_off; p.hist_ids = b->hist_ids;
+    p.mask = b->mask; p.mask_ld = b->mask_ld; p.mask_row = b->mask_row;
+    p.scores = b->scores; p.lengths = b->lengths; p.finished = b->finished;
+    p.out_tokens = b->out_tokens; p.out_parents = b->out_parents; p.out_scores = b->out_scores;
+    p.out_lengths = b->out_lengths; p.out_finished = b->out_finished;
+    p.status = b->status;
+    p.beams = prm->beams; p.n = prm->n_out; p.eos = prm->eos_id;
+    p.max_hist = prm->max_history > 0 ? prm->max_history : 1024;
+    p.alpha = prm->length_penalty;
+    p.order = prm->penalty_order;
+    p.rep = prm->repeat_penalty; p.freq = prm->frequency_penalty; p.pres = prm->presence_penalty;
+    p.slices = (vocab + kBeamSlice - 1) / kBeamSlice;
+    /* per group: its rows' slots, then their lists */
+    const size_t lists = (size_t)p.beams * p.slices, per = lists * (sizeof(BeamSlot) + (size_t)p.n * 8);
+    int64_t most = (int64_t)(kBeamWorkspace / per);
+    if (most > (int64_t)(0x3fffffff / lists)) most = (int64_t)(0x3fffffff / lists);
+    if (most < 1) most = 1;
+    const int step = most < groups ? (int)most : groups;
+    std::lock_guard<std::mutex> lock(g_mu);
+    WsView ws;
+    if (!workspace(stream, 0, (size_t)step, (size_t)step * per, ws)) return ws_status();
+    p.counters = ws.counters;
+    p.slots = (BeamSlot *)ws.data;
+    p.cands = (uint64_t *)(ws.data + (size_t)step * lists * sizeof(BeamSlot));
+    for (p.g0 = 0; p.g0 < groups; p.g0 += step) {
+        const int n = groups - p.g0 < step ? groups - p.g0 : step;
+        if (dlk_launch_beam_select(&p, n, stream) != 0) return DLK_ERR_HIP;
+        if (groups - p.g0 <= step) break;
+    }
+    return DLK_OK;
 }

@@ -248,6 +248,124 @@ int dlk_sample_grammar(const dlk_batch *batch, int rows, int vocab, const dlk_sa
  * bit-identical to the host libm's.  No-op unless cap > 0, as in the reference. */
 int dlk_softcap(float *logits, int64_t ld, int rows, int vocab, float cap, hipStream_t stream);
 
+/* ---- logits from 8-bit weights -------------------------------------------------
+ * What stands before the calls above in a decode step: the LM head of a model whose
+ * weights are kept in 8 bits, with the soft-cap as its epilogue (the reference's LM
+ * head and cap, src/core/context.c:854-876, on block-quantised weights there).  No
+ * counterpart of the 8-bit form in the reference. */
+
+/* Element types of dlk_quantize_rows' input. */
+#define DLK_F32 0
+#define DLK_BF16 1
+#define DLK_F16 2
+
+/* Row-wise symmetric quantisation: scale[r] = max_i |x[r * ldx + i]| / 127 (one
+ * float rounding), q[r * ldq + i] = x / scale[r] to the nearest integer, halves to
+ * even, decided exactly; within +-127.  A row of zeros: scale 0 and zeros.  A row
+ * that holds NaN or infinity: scale NaN and zeros, so its logits are NaN.  Hidden
+ * states take it per token, weights [vocab, n] once per channel.  x, q and scale
+ * need the alignment of their elements only; strides are in elements. */
+int dlk_quantize_rows(const void *x, int dtype, int64_t ldx, int rows, int n, int8_t *q, int64_t ldq, float *scale,
+                      hipStream_t stream);
+
+/* logits[r * ld + v] = (sum_i x[r * ldx + i] * w[v * ldw + i]) * x_scale[r] * w_scale[v],
+ * the sum exact in 32-bit integers (n <= 131,071, else DLK_ERR_UNSUPPORTED), then
+ * three float roundings (the sum's, and one per scale); softcap > 0: then the cap,
+ * with the bits dlk_softcap gives.  Any strides and byte alignment of x and w.
+ * Entries past vocab in a row of logits are left as they are. */
+int dlk_logits_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw,
+                  const float *w_scale, int rows, int vocab, int n, float softcap, float *logits, int64_t ld,
+                  hipStream_t stream);
+
+/* ---- beam search ----------------------------------------------------------------
+ * The deterministic counterpart of dlk_sample: the best continuations of each group
+ * (request) of `beams` rows over the vocabulary, and the beams' states following
+ * their parents.  No counterpart in the reference. */
+
+#define DLK_STATUS_NOT_FINITE 8u        /* dlk_beam_select: a row's allowed logits held NaN or +inf, or its score
+                                           was NaN or +inf: it has no continuations */
+#define DLK_MAX_BEAMS 64                /* beams and n_out */
+
+typedef struct {
+    const float *logits;      /* [groups * beams, ld] fp32, read only; row g * beams + b is beam b of group g */
+    int64_t ld;
+    const int32_t *hist_off;  /* histories and masks as in dlk_batch, per row; or NULL */
+    const int32_t *hist_ids;
+    const uint32_t *mask;
+    int64_t mask_ld;
+    const int32_t *mask_row;
+    const float *scores;      /* [groups * beams] sums of log-probabilities, -inf: no such beam; NULL = all 0 */
+    const int32_t *lengths;   /* [groups * beams] tokens so far, for the length penalty; NULL = all 0 */
+    const uint8_t *finished;  /* [groups * beams] not 0: the beam has ended; NULL = none */
+    int32_t *out_tokens;      /* [groups * n_out] the continuations, best first; -1 where a group has no more */
+    int32_t *out_parents;     /* [groups * n_out] the row each continues; -1 likewise */
+    float *out_scores;        /* [groups * n_out] their scores; -inf likewise */
+    int32_t *out_lengths;     /* [groups * n_out] or NULL; 0 likewise */
+    uint8_t *out_finished;    /* [groups * n_out] 1 where the token is eos_id, or NULL; 0 likewise */
+    uint32_t *status;         /* one word of DLK_STATUS_* bits, OR-ed, or NULL */
+} dlk_beam_batch;
+
+typedef struct {
+    int beams;                /* rows per group (1 before the first step of a request), at most DLK_MAX_BEAMS */
+    int n_out;                /* continuations per group, at most DLK_MAX_BEAMS */
+    int eos_id;               /* a continuation by this id has ended; -1 = none (finished is NULL then) */
+    float length_penalty;     /* candidates are ordered by score / length^length_penalty; 0 = by score */
+    float repeat_penalty;     /* as in dlk_sample_params */
+    float frequency_penalty;
+    float presence_penalty;
+    uint32_t penalty_order;
+    int max_history;          /* upper bound on any row's history (0 = 1024; at most 65,535); a row past it has no
+                                 continuations and sets DLK_STATUS_HISTORY_TOO_LONG */
+} dlk_beam_params;
+
+/* One step of a beam search.  Row r's logits l are masked, then penalised, as
+ * dlk_sample does; its continuation by id v has
+ *   score = scores[r] + (l_v - max l) - log(sum_u exp(l_u - max l)),  length = lengths[r] + 1,
+ * computed in 64 bits and rounded once.  A finished row has one continuation: eos_id,
+ * with its score and length as they are (its logits are not read).  Ids with logit
+ * -inf are no continuations, nor are those of rows with score -inf.
+ * Of each group's continuations the n_out with the largest score / max(length,
+ * 1)^length_penalty (before rounding) are written, largest first; of equal ones the
+ * lower row first, then the larger logit, then the lower id.  Outputs may not overlap
+ * inputs.  Takes workspace as dlk_sample does (dlk_release_stream; one call on the
+ * stream before capturing it, else DLK_ERR_HIP). */
+int dlk_beam_select(const dlk_beam_batch *batch, int groups, int vocab, const dlk_beam_params *params,
+                    hipStream_t stream);
+
+/* One buffer whose rows follow the beams: bytes at
+ *   base + o * outer + r * row + i * inner,  o < n_outer, i < n_inner,
+ * for row r; a cache [layers, rows, heads, room, width] filled up to `length` has outer =
+ * layer, inner = head and bytes = length * width * element size.  Strides in bytes,
+ * not negative.  src == dst: in place, with equal strides. */
+typedef struct {
+    const void *src;
+    void *dst;
+    int64_t bytes;
+    int64_t src_row, src_outer, src_inner;
+    int64_t dst_row, dst_outer, dst_inner;
+    int n_outer, n_inner;
+} dlk_beam_state;
+
+/* The rows' histories (CSR, as in dlk_batch) and the tokens to append. */
+typedef struct {
+    const int32_t *off;       /* [groups * beams + 1] */
+    const int32_t *ids;
+    const int32_t *tokens;    /* [groups * n_out] appended; a negative one appends nothing; NULL = none */
+    int max_history;          /* each new history keeps its last max_history ids */
+    int32_t *out_off;         /* [groups * n_out + 1]; no overlap with the inputs */
+    int32_t *out_ids;         /* room for groups * n_out * max_history ids; those past out_off's last are left */
+} dlk_beam_history;
+
+/* The states of groups * n_out rows from those of groups * beams: row r takes row
+ * parents[r] (as dlk_beam_select writes it).  A parent outside its own group's rows
+ * (-1 among them) moves nothing: the row's states are left, its history is empty.
+ * In-place states need n_out == beams; they move as if all rows were read before
+ * any is written, and rows that are their own parents cost nothing.  Destinations of
+ * one call may not overlap one another, nor any source but their own in place.
+ * n_states of any number; history may be NULL. */
+int dlk_beam_reorder(const int32_t *parents, int groups, int beams, int n_out, const dlk_beam_state *states,
+                     int n_states, const dlk_beam_history *history, hipStream_t stream);
+
 /* The vocabulary table of the calls above (token t = bytes[off[t] .. off[t+1]),
  * read up to its first NUL) from a GGUF file's `tokenizer.ggml.tokens` string
  * array: the strings tokenizer_init loads (src/tokenizer.c:247-300) and
