@@ -48,95 +48,119 @@ DLK_DEV i4 load16_to(const int8_t *p, int k, int n) {
     return i4{(int)(uint32_t)l1, (int)(uint32_t)(l1 >> 32), (int)(uint32_t)h1, (int)(uint32_t)(h1 >> 32)};
 }
 
-template <int MT, int NT, int WAVES, int BK, bool CAP>
-__global__ __launch_bounds__(WAVES * 64) void logits_i8_kernel(I8Params p) {
-    constexpr int T = WAVES * 64, KS = BK / 64, NF = NT / 16, MF = MT / 16;
-    constexpr int CPR = BK / 16;                   /* 16-byte chunks in a staged row */
-    constexpr int XC = MT * CPR / T;               /* chunks a thread stages */
-    static_assert(MT * CPR % T == 0 && CPR % 8 == 0, "staging");
-    __shared__ __align__(16) int8_t xs[2][MT * BK];
-    const int t = threadIdx.x, lane = lane_id(), wave = wave_id();
-    const int mtiles = (p.rows + MT - 1) / MT;
-    const int vt = blockIdx.x / mtiles, m0 = (blockIdx.x % mtiles) * MT;
-    const int v0 = vt * (NT * WAVES) + wave * NT;
-    const int lr = lane & 15, lk = lane >> 4;
-    const int8_t *wrow[NF];
+/* Waits until at most N of the wave's loads are in flight and its LDS work is done. */
+template <int N>
+DLK_DEV void wait_loads() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (N >> 4) << 14);
+    asm volatile("" ::: "memory");
+}
+
+/* 16-byte chunk c of row r of a staged tile lies at chunk place(r, c): the lanes of a
+ * fragment read (16 rows at one or two neighbouring chunks) then meet every bank once. */
+template <int BK>
+DLK_DEV int place(int r, int c) {
+    return BK == 64 ? c ^ ((0x78 >> (2 * ((r >> 2) & 3))) & 3) : BK == 128 ? c ^ (r & 7) : c ^ (r & 15);
+}
+
+/* BM rows of x and BN rows of w per workgroup, WGM x WGN waves, steps of BK bytes of n,
+ * ST stages in LDS.  DMA: the rows of both are whole 16-byte chunks, loaded straight into
+ * LDS; else through registers, any alignment. */
+template <int BM, int BN, int WGM, int WGN, int BK, int ST, int OCC, bool DMA, bool CAP>
+__global__ __launch_bounds__(WGM * WGN * 64, OCC) void logits_i8_kernel(I8Params p) {
+    constexpr int W = WGM * WGN, WM = BM / WGM, WN = BN / WGN, MF = WM / 16, NF = WN / 16;
+    constexpr int CPR = BK / 16, RPI = 64 / CPR;   /* chunks of a row; rows that a wave loads at once */
+    constexpr int NI = (BM + BN) / RPI / W;        /* loads of a wave per stage */
+    constexpr int STAGE = (BM + BN) * BK;
+    static_assert((BM + BN) % (RPI * W) == 0 && BM % RPI == 0 && (BK == 64 || BK == 128 || BK == 256), "tiles");
+    __shared__ __align__(1024) int8_t lds[ST * STAGE];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
+    /* workgroups go to the XCDs in turn: each XCD gets a run of tiles, the rows' tiles of one
+     * tile of w side by side, so that w comes from memory once */
+    const int mtiles = (p.rows + BM - 1) / BM, vtiles = (p.vocab + BN - 1) / BN;
+    const int tile = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+    if (tile >= mtiles * vtiles) return;
+    const int m0 = tile % mtiles * BM, v0 = tile / mtiles * BN;
+    const int8_t *src[NI];                         /* the row of this lane's chunk */
+    int at[NI];                                    /* and its place in the row */
 #pragma unroll
-    for (int f = 0; f < NF; f++) wrow[f] = p.w + (int64_t)min(v0 + f * 16 + lr, p.vocab - 1) * p.ldw + lk * 16;
+    for (int j = 0; j < NI; j++) {
+        const int r = (j * W + wave) * RPI + lane / CPR;
+        at[j] = place<BK>(r, lane % CPR) * 16;
+        src[j] = r < BM ? p.x + (int64_t)min(m0 + r, p.rows - 1) * p.ldx
+                        : p.w + (int64_t)min(v0 + r - BM, p.vocab - 1) * p.ldw;
+    }
+    i4 reg[DMA ? 1 : NI];
+    auto fetch = [&](int k0, int slot) {
+#pragma unroll
+        for (int j = 0; j < NI; j++) {
+            if (DMA && k0 + BK <= p.n) {
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src[j] + k0 + at[j]),
+                                                 (__attribute__((address_space(3))) void *)&lds[slot * STAGE + (j * W + wave) * 1024],
+                                                 16, 0, 0);
+            } else {
+                const i4 v = k0 + BK <= p.n ? (i4)*(const i4_any *)(src[j] + k0 + at[j]) : load16_to(src[j], k0 + at[j], p.n);
+                if (DMA) *(i4 *)&lds[slot * STAGE + (j * W + wave) * 1024 + lane * 16] = v;
+                else reg[j] = v;
+            }
+        }
+    };
+    auto put = [&](int slot) {
+        if (!DMA) {
+#pragma unroll
+            for (int j = 0; j < NI; j++) *(i4 *)&lds[slot * STAGE + (j * W + wave) * 1024 + lane * 16] = reg[j];
+        }
+    };
+    const int lr = lane & 15, lk = lane >> 4, wm = wave % WGM * WM, wn = wave / WGM * WN;
     i4 acc[MF][NF];
 #pragma unroll
     for (int m = 0; m < MF; m++)
 #pragma unroll
         for (int f = 0; f < NF; f++) acc[m][f] = i4{0, 0, 0, 0};
-    i4 xr[XC];
-    auto load_x = [&](int k0) {
+    const int steps = (p.n + BK - 1) / BK;
 #pragma unroll
-        for (int c = 0; c < XC; c++) {
-            const int ch = t + c * T, r = ch / CPR, k = k0 + (ch % CPR) * 16;
-            const int8_t *row = p.x + (int64_t)min(m0 + r, p.rows - 1) * p.ldx;
-            xr[c] = k0 + BK <= p.n ? (i4)*(const i4_any *)(row + k) : load16_to(row, k, p.n);
-        }
-    };
-    auto store_x = [&](int buf) {
+    for (int s = 0; s < ST - 1; s++)
+        if (s < steps) { fetch(s * BK, s); put(s); }
+    int slot = 0;
+    for (int it = 0; it < steps; it++) {
+        if (it + ST - 2 < steps) wait_loads<NI *(ST - 2)>();
+        else wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const int next = slot == 0 ? ST - 1 : slot - 1;        /* the slot that step it - 1 has left */
+        if (it + ST - 1 < steps) fetch((it + ST - 1) * BK, next);
+        const int8_t *xs = &lds[slot * STAGE], *ws = xs + BM * BK;
 #pragma unroll
-        for (int c = 0; c < XC; c++) {
-            const int ch = t + c * T, r = ch / CPR, cc = ch % CPR;
-            *(i4 *)&xs[buf][r * BK + (cc ^ (r & 7)) * 16] = xr[c];
-        }
-    };
-    auto load_w = [&](i4 (&w)[NF][KS], int k0) {
-        if (k0 + BK <= p.n) {
+        for (int s = 0; s < BK / 64; s++) {
+            i4 a[NF], b[MF];
 #pragma unroll
-            for (int f = 0; f < NF; f++)
-#pragma unroll
-                for (int s = 0; s < KS; s++) w[f][s] = *(const i4_any *)(wrow[f] + k0 + s * 64);
-        } else {
-#pragma unroll
-            for (int f = 0; f < NF; f++)
-#pragma unroll
-                for (int s = 0; s < KS; s++) w[f][s] = load16_to(wrow[f] - lk * 16, k0 + s * 64 + lk * 16, p.n);
-        }
-    };
-    auto compute = [&](const i4 (&w)[NF][KS], int buf) {
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
+            for (int f = 0; f < NF; f++) {
+                const int r = wn + f * 16 + lr;
+                a[f] = *(const i4 *)&ws[r * BK + place<BK>(BM + r, s * 4 + lk) * 16];
+            }
 #pragma unroll
             for (int m = 0; m < MF; m++) {
-                const int r = m * 16 + lr;
-                const i4 b = *(const i4 *)&xs[buf][r * BK + ((s * 4 + lk) ^ (r & 7)) * 16];
+                const int r = wm + m * 16 + lr;
+                b[m] = *(const i4 *)&xs[r * BK + place<BK>(r, s * 4 + lk) * 16];
+            }
+#pragma unroll
+            for (int m = 0; m < MF; m++)
 #pragma unroll
                 for (int f = 0; f < NF; f++)
-                    acc[m][f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[f][s], b, acc[m][f], 0, 0, 0);
-            }
+                    acc[m][f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[f], b[m], acc[m][f], 0, 0, 0);
         }
-    };
-    i4 w0[NF][KS], w1[NF][KS];
-    load_x(0);
-    load_w(w0, 0);
-    store_x(0);
-    __syncthreads();
-    for (int k = 0; k < p.n; k += 2 * BK) {
-        const bool more1 = k + BK < p.n, more2 = k + 2 * BK < p.n;
-        if (more1) { load_x(k + BK); load_w(w1, k + BK); }
-        compute(w0, 0);
-        if (!more1) break;
-        store_x(1);
-        __syncthreads();
-        if (more2) { load_x(k + 2 * BK); load_w(w0, k + 2 * BK); }
-        compute(w1, 1);
-        if (!more2) break;
-        store_x(0);
-        __syncthreads();
+        if (it + ST - 1 < steps) put(next);
+        slot = slot == ST - 1 ? 0 : slot + 1;
     }
 #pragma unroll
     for (int f = 0; f < NF; f++) {
-        const int v = v0 + f * 16 + lk * 4;
+        const int v = v0 + wn + f * 16 + lk * 4;
         float ws[4];
 #pragma unroll
         for (int c = 0; c < 4; c++) ws[c] = p.w_scale[min(v + c, p.vocab - 1)];
 #pragma unroll
         for (int m = 0; m < MF; m++) {
-            const int r = m0 + m * 16 + lr;
+            const int r = m0 + wm + m * 16 + lr;
             const float sx = p.x_scale[min(r, p.rows - 1)];
             float y[4];
 #pragma unroll
@@ -156,17 +180,25 @@ __global__ __launch_bounds__(WAVES * 64) void logits_i8_kernel(I8Params p) {
     }
 }
 
-template <int MT, int NT, int WAVES, int BK>
+template <int BM, int BN, int WGM, int WGN, int BK, int ST, int OCC, bool DMA>
 int launch_i8(const I8Params &p, hipStream_t stream) {
-    const int64_t blocks = (((int64_t)p.vocab + NT * WAVES - 1) / (NT * WAVES)) * (((int64_t)p.rows + MT - 1) / MT);
-    if (blocks > 0x7fffffff) return DLK_ERR_UNSUPPORTED;
+    const int64_t tiles = (((int64_t)p.vocab + BN - 1) / BN) * (((int64_t)p.rows + BM - 1) / BM);
+    if (tiles > 0x3fffffff) return DLK_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)((tiles + 7) / 8 * 8)), block(WGM * WGN * 64);
     if (p.cap > 0.0f)
-        hipLaunchKernelGGL((logits_i8_kernel<MT, NT, WAVES, BK, true>), dim3((unsigned)blocks), dim3(WAVES * 64), 0,
-                           stream, p);
+        hipLaunchKernelGGL((logits_i8_kernel<BM, BN, WGM, WGN, BK, ST, OCC, DMA, true>), grid, block, 0, stream, p);
     else
-        hipLaunchKernelGGL((logits_i8_kernel<MT, NT, WAVES, BK, false>), dim3((unsigned)blocks), dim3(WAVES * 64), 0,
-                           stream, p);
+        hipLaunchKernelGGL((logits_i8_kernel<BM, BN, WGM, WGN, BK, ST, OCC, DMA, false>), grid, block, 0, stream, p);
     return hipGetLastError() == hipSuccess ? DLK_OK : DLK_ERR_HIP;
+}
+
+template <bool DMA>
+int launch_i8_rows(const I8Params &p, hipStream_t stream) {
+    if (p.rows <= 16) return launch_i8<16, 64, 1, 4, 256, 3, 2, DMA>(p, stream);
+    if (p.rows <= 32) return launch_i8<32, 64, 1, 4, 128, 4, 2, DMA>(p, stream);
+    if (p.rows <= 64) return launch_i8<64, 64, 1, 4, 128, 4, 2, DMA>(p, stream);
+    if (p.rows <= 128) return launch_i8<128, 128, 2, 2, 64, 3, 2, DMA>(p, stream);
+    return launch_i8<256, 128, 2, 2, 64, 3, 2, DMA>(p, stream);
 }
 
 }  // namespace dlk
@@ -187,8 +219,6 @@ extern "C" int dlk_logits_i8(const int8_t *x, int64_t ldx, const float *x_scale,
     p.rows = rows; p.vocab = vocab; p.n = n;
     p.cap = softcap > 0.0f ? softcap : 0.0f;
     p.recip = p.cap > 0.0f ? dlk_softcap_recip(p.cap) : 0.0f;
-    if (rows <= 16) return launch_i8<16, 16, 4, 512>(p, stream);
-    if (rows <= 32) return launch_i8<32, 16, 4, 512>(p, stream);
-    if (rows <= 64) return launch_i8<64, 32, 4, 256>(p, stream);
-    return launch_i8<128, 32, 4, 128>(p, stream);
+    const bool chunks = (((uintptr_t)x | (uintptr_t)w | (uintptr_t)ldx | (uintptr_t)ldw) & 15) == 0;
+    return chunks ? launch_i8_rows<true>(p, stream) : launch_i8_rows<false>(p, stream);
 }
