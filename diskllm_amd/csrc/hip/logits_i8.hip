@@ -2,9 +2,12 @@
  * logits_i8.hip -- an LM head in 8-bit integers: logits[r, v] = (x_r . w_v) * x_scale[r] *
  * w_scale[v], the soft-cap as epilogue (dlk_logits_i8).
  */
+#include <float.h>
+#include <math.h>
+
 #include <hip/hip_runtime.h>
 
-#include "softcap4.h"
+#include "dlk_device.h"
 #include "../../../include/diskllm_amd.h"
 
 namespace dlk {
@@ -63,6 +66,80 @@ DLK_DEV int place(int r, int c) {
     return BK == 64 ? c ^ ((0x78 >> (2 * ((r >> 2) & 3))) & 3) : BK == 128 ? c ^ (r & 7) : c ^ (r & 15);
 }
 
+/* cap * tanh(y / cap) in some 16 instructions (libm's bits, which dlk_softcap gives, take
+ * 65: 240 us of the 512 x 262,144 product against 60).  t = |y| / cap: below 0.35 the
+ * series of tanh(t) / t to t^10 (what is left out: 2e-9 of it), above (1 - e) / (1 + e)
+ * with e = exp(-2t).  At 0.35, the worst place, e is off by 3.4 half-steps, which 2 e / (1
+ * + e)^2 / tanh makes 4.5; with t's own two and those of 1 + e, its reciprocal and the
+ * products some 10 half-steps of the result at most.  recip: 1 / cap. */
+DLK_DEV float capped(float y, float cap, float recip) {
+    const float q = y * recip, t = fabsf(q), t2 = t * t;
+    float s = fmaf(t2, -1382.0f / 155925.0f, 62.0f / 2835.0f);
+    s = fmaf(t2, s, -17.0f / 315.0f);
+    s = fmaf(t2, s, 2.0f / 15.0f);
+    s = fmaf(t2, s, -1.0f / 3.0f);
+    s = fmaf(t * t2, s, t);
+    const float e = __builtin_amdgcn_exp2f(-2.88539008177792681f * t);
+    const float b = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
+    return copysignf(t < 0.35f ? s : b, q) * cap;
+}
+
+/* A wave's MF x NF fragments of sums as logits: rows m0 .., ids v0 ...  A fragment's lane
+ * holds four ids of one row; where WIDE, 16 rows at a time go through the wave's own 16 *
+ * (NF * 16 + 4) floats of LDS, so that a store writes whole rows of NF * 64 bytes (512 x
+ * 262,144 out of n = 512: 252 -> 181 us), else each lane stores its own 16 bytes. */
+template <bool CAP, bool WIDE, int MF, int NF>
+DLK_DEV void write_logits(const I8Params &p, const i4 (&acc)[MF][NF], int m0, int v0, float *mine) {
+    const int lane = lane_id(), lr = lane & 15, lk = lane >> 4;
+    constexpr int LD = NF * 16 + 4, LPR = NF * 4, RPS = 64 / LPR;        /* lanes of a row, rows of a store */
+    auto store = [&](int r, int v, const float (&y)[4]) {
+        if (r >= p.rows) return;
+        float *out = p.logits + (int64_t)r * p.ld + v;
+        if (v + 3 < p.vocab) {
+            store4(out, make_float4(y[0], y[1], y[2], y[3]));
+        } else {
+#pragma unroll
+            for (int c = 0; c < 3; c++)
+                if (v + c < p.vocab) out[c] = y[c];
+        }
+    };
+    float ws[NF][4];
+#pragma unroll
+    for (int f = 0; f < NF; f++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) ws[f][c] = p.w_scale[min(v0 + f * 16 + lk * 4 + c, p.vocab - 1)];
+#pragma unroll
+    for (int m = 0; m < MF; m++) {
+        const float sx = p.x_scale[min(m0 + m * 16 + lr, p.rows - 1)];
+#pragma unroll
+        for (int f = 0; f < NF; f++) {
+            float y[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                y[c] = (float)acc[m][f][c] * sx * ws[f][c];
+                if (CAP) y[c] = capped(y[c], p.cap, p.recip);
+            }
+            if (WIDE) *(float4 *)&mine[lr * LD + f * 16 + lk * 4] = make_float4(y[0], y[1], y[2], y[3]);
+            else store(m0 + m * 16 + lr, v0 + f * 16 + lk * 4, y);
+        }
+        if (WIDE) {
+#pragma unroll
+            for (int i = 0; i < 16 / RPS; i++) {
+                const int r = i * RPS + lane / LPR, c = lane % LPR * 4;
+                const float4 q = *(const float4 *)&mine[r * LD + c];
+                const float y[4] = {q.x, q.y, q.z, q.w};
+                store(m0 + m * 16 + r, v0 + c, y);
+            }
+        }
+    }
+}
+
+/* Loads 16 bytes a lane straight into LDS: lane i's to dst + 16 i (dst the same in all lanes). */
+DLK_DEV void load_to_lds(const int8_t *src, int8_t *dst) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
+                                     (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+}
+
 /* BM rows of x and BN rows of w per workgroup, WGM x WGN waves, steps of BK bytes of n,
  * ST stages in LDS.  DMA: the rows of both are whole 16-byte chunks, loaded straight into
  * LDS; else through registers, any alignment. */
@@ -95,9 +172,7 @@ __global__ __launch_bounds__(WGM * WGN * 64, OCC) void logits_i8_kernel(I8Params
 #pragma unroll
         for (int j = 0; j < NI; j++) {
             if (DMA && k0 + BK <= p.n) {
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src[j] + k0 + at[j]),
-                                                 (__attribute__((address_space(3))) void *)&lds[slot * STAGE + (j * W + wave) * 1024],
-                                                 16, 0, 0);
+                load_to_lds(src[j] + k0 + at[j], &lds[slot * STAGE + (j * W + wave) * 1024]);
             } else {
                 const i4 v = k0 + BK <= p.n ? (i4)*(const i4_any *)(src[j] + k0 + at[j]) : load16_to(src[j], k0 + at[j], p.n);
                 if (DMA) *(i4 *)&lds[slot * STAGE + (j * W + wave) * 1024 + lane * 16] = v;
@@ -152,32 +227,127 @@ __global__ __launch_bounds__(WGM * WGN * 64, OCC) void logits_i8_kernel(I8Params
         if (it + ST - 1 < steps) put(next);
         slot = slot == ST - 1 ? 0 : slot + 1;
     }
+    constexpr bool WIDE = NF >= 4;
+    static_assert(!WIDE || W * 16 * (WN + 4) * 4 <= ST * STAGE, "room for the output");
+    if (WIDE) __syncthreads();
+    write_logits<CAP, WIDE>(p, acc, m0 + wm, v0 + wn, (float *)lds + (WIDE ? wave * 16 * (WN + 4) : 0));
+}
+
+/* The product of many rows: 256 x 256 tiles, eight waves of 128 x 64, steps of 128 bytes (whole
+ * cache lines: 64 cost 8% more) in two stages of 64 KB.  Each half-step's fragments are read
+ * into registers while the matrix cores work on the half-step before, the reads spread
+ * between the products (sched_group_barrier; the compiler alone puts them last), and a stage
+ * is loaded again as soon as its second half is in registers. */
+template <bool CAP>
+__global__ __launch_bounds__(512, 2) void logits_i8_wide_kernel(I8Params p) {
+    constexpr int BM = 256, BN = 256, BK = 128, WGM = 2, WM = 128, WN = 64, MF = 8, NF = 4;
+    constexpr int W = 8, RPI = 8, NX = BM / RPI / W, NW = BN / RPI / W, XST = BM * BK, WST = BN * BK;
+    __shared__ __align__(1024) int8_t lds[2 * (XST + WST)];
+    int8_t *const ldw = lds + 2 * XST;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
+    const int mtiles = (p.rows + BM - 1) / BM, vtiles = (p.vocab + BN - 1) / BN;
+    const int tile = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+    if (tile >= mtiles * vtiles) return;
+    const int m0 = tile % mtiles * BM, v0 = tile / mtiles * BN;
+    const int8_t *sx[NX], *sw[NW];
 #pragma unroll
-    for (int f = 0; f < NF; f++) {
-        const int v = v0 + wn + f * 16 + lk * 4;
-        float ws[4];
+    for (int j = 0; j < NX; j++) {
+        const int r = (j * W + wave) * RPI + lane / 8;
+        sx[j] = p.x + (int64_t)min(m0 + r, p.rows - 1) * p.ldx + place<BK>(r, lane % 8) * 16;
+    }
 #pragma unroll
-        for (int c = 0; c < 4; c++) ws[c] = p.w_scale[min(v + c, p.vocab - 1)];
+    for (int j = 0; j < NW; j++) {
+        const int r = (j * W + wave) * RPI + lane / 8;
+        sw[j] = p.w + (int64_t)min(v0 + r, p.vocab - 1) * p.ldw + place<BK>(r, lane % 8) * 16;
+    }
+    auto fetch = [&](int it, int slot) {
 #pragma unroll
-        for (int m = 0; m < MF; m++) {
-            const int r = m0 + wm + m * 16 + lr;
-            const float sx = p.x_scale[min(r, p.rows - 1)];
-            float y[4];
+        for (int j = 0; j < NX; j++) load_to_lds(sx[j] + it * BK, &lds[slot * XST + (j * W + wave) * 1024]);
 #pragma unroll
-            for (int c = 0; c < 4; c++) y[c] = (float)acc[m][f][c] * sx * ws[c];
-            if (CAP) softcap4<false>(y, p.cap, p.recip);
-            if (r < p.rows) {
-                float *out = p.logits + (int64_t)r * p.ld + v;
-                if (v + 3 < p.vocab) {
-                    store4(out, make_float4(y[0], y[1], y[2], y[3]));
-                } else {
+        for (int j = 0; j < NW; j++) load_to_lds(sw[j] + it * BK, &ldw[slot * WST + (j * W + wave) * 1024]);
+    };
+    const int lr = lane & 15, lk = lane >> 4, wm = wave % WGM * WM, wn = wave / WGM * WN;
+    const int half0 = lr * BK + place<BK>(lr, lk) * 16, half1 = lr * BK + place<BK>(lr, 4 + lk) * 16;
+    auto take = [&](i4 (&a)[NF], i4 (&b)[MF], int slot, int half) {
+        const int8_t *xs = &lds[slot * XST + wm * BK + half], *ws = &ldw[slot * WST + wn * BK + half];
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        if (v + c < p.vocab) out[c] = y[c];
-                }
+        for (int f = 0; f < NF; f++) a[f] = *(const i4 *)&ws[f * 16 * BK];
+#pragma unroll
+        for (int m = 0; m < MF; m++) b[m] = *(const i4 *)&xs[m * 16 * BK];
+    };
+    i4 acc[MF][NF];
+#pragma unroll
+    for (int m = 0; m < MF; m++)
+#pragma unroll
+        for (int f = 0; f < NF; f++) acc[m][f] = i4{0, 0, 0, 0};
+    auto multiply = [&](const i4 (&a)[NF], const i4 (&b)[MF]) {
+#pragma unroll
+        for (int m = 0; m < MF; m++)
+#pragma unroll
+            for (int f = 0; f < NF; f++)
+                acc[m][f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[f], b[m], acc[m][f], 0, 0, 0);
+        /* one LDS read (0x100), two products (0x8), over and over; then the other products */
+#pragma unroll
+        for (int i = 0; i < MF + NF; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, MF * NF - 2 * (MF + NF), 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    i4 a0[NF], b0[MF], a1[NF], b1[MF];
+    const int steps = p.n / BK;
+    if (steps > 0) {
+        fetch(0, 0);
+        if (steps > 1) {
+            fetch(1, 1);
+            wait_loads<NX + NW>();
+        } else {
+            wait_loads<0>();
+        }
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        take(a0, b0, 0, half0);
+        for (int it = 0; it < steps; it++) {
+            take(a1, b1, it & 1, half1);
+            multiply(a0, b0);
+            if (it + 1 < steps) {
+                wait_loads<0>();                   /* step it + 1 is there; this wave has read all of step it */
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if (it + 2 < steps) fetch(it + 2, it & 1);
+                take(a0, b0, (it + 1) & 1, half0);
             }
+            multiply(a1, b1);
         }
     }
+    if (p.n % BK != 0) {                           /* what is left of n, through registers, zeros past it */
+        __syncthreads();
+#pragma unroll 1
+        for (int j = 0; j < NX + NW; j++) {
+            const int r = ((j < NX ? j : j - NX) * W + wave) * RPI + lane / 8;
+            const int8_t *row = j < NX ? p.x + (int64_t)min(m0 + r, p.rows - 1) * p.ldx
+                                       : p.w + (int64_t)min(v0 + r, p.vocab - 1) * p.ldw;
+            int8_t *dst = j < NX ? &lds[(j * W + wave) * 1024] : &ldw[((j - NX) * W + wave) * 1024];
+            *(i4 *)&dst[lane * 16] = load16_to(row, steps * BK + place<BK>(r, lane % 8) * 16, p.n);
+        }
+        __syncthreads();
+        take(a0, b0, 0, half0);
+        multiply(a0, b0);
+        take(a0, b0, 0, half1);
+        multiply(a0, b0);
+    }
+    __syncthreads();
+    write_logits<CAP, true>(p, acc, m0 + wm, v0 + wn, (float *)lds + wave * 16 * (WN + 4));
+}
+
+int launch_i8_wide(const I8Params &p, hipStream_t stream) {
+    const int64_t tiles = (((int64_t)p.vocab + 255) / 256) * (((int64_t)p.rows + 255) / 256);
+    if (tiles > 0x3fffffff) return DLK_ERR_UNSUPPORTED;
+    const dim3 grid((unsigned)((tiles + 7) / 8 * 8));
+    if (p.cap > 0.0f) hipLaunchKernelGGL((logits_i8_wide_kernel<true>), grid, dim3(512), 0, stream, p);
+    else hipLaunchKernelGGL((logits_i8_wide_kernel<false>), grid, dim3(512), 0, stream, p);
+    return hipGetLastError() == hipSuccess ? DLK_OK : DLK_ERR_HIP;
 }
 
 template <int BM, int BN, int WGM, int WGN, int BK, int ST, int OCC, bool DMA>
@@ -197,8 +367,8 @@ int launch_i8_rows(const I8Params &p, hipStream_t stream) {
     if (p.rows <= 16) return launch_i8<16, 64, 1, 4, 256, 3, 2, DMA>(p, stream);
     if (p.rows <= 32) return launch_i8<32, 64, 1, 4, 128, 4, 2, DMA>(p, stream);
     if (p.rows <= 64) return launch_i8<64, 64, 1, 4, 128, 4, 2, DMA>(p, stream);
-    if (p.rows <= 128) return launch_i8<128, 128, 2, 2, 64, 3, 2, DMA>(p, stream);
-    return launch_i8<256, 128, 2, 2, 64, 3, 2, DMA>(p, stream);
+    if (DMA && p.rows > 128) return launch_i8_wide(p, stream);
+    return launch_i8<128, 128, 2, 2, 128, 2, 2, DMA>(p, stream);
 }
 
 }  // namespace dlk
@@ -208,7 +378,7 @@ extern "C" int dlk_logits_i8(const int8_t *x, int64_t ldx, const float *x_scale,
                              hipStream_t stream) {
     using namespace dlk;
     if (!x || !x_scale || !w || !w_scale || !logits || rows < 0 || vocab <= 0 || n <= 0) return DLK_ERR_INVALID;
-    if (ldx < n || ldw < n || ld < vocab) return DLK_ERR_INVALID;
+    if (ldx < n || ldw < n || ld < vocab || softcap == INFINITY) return DLK_ERR_INVALID;
     if ((((uintptr_t)x_scale | (uintptr_t)w_scale | (uintptr_t)logits) & 3) != 0) return DLK_ERR_INVALID;
     /* |sum| <= 128 * 128 * n in 32 bits; int indices */
     if (n > 131071 || vocab > 0x7fffffff - 65536 || rows > 0x7fffffff - 65536) return DLK_ERR_UNSUPPORTED;
@@ -218,7 +388,7 @@ extern "C" int dlk_logits_i8(const int8_t *x, int64_t ldx, const float *x_scale,
     p.x_scale = x_scale; p.w_scale = w_scale; p.logits = logits;
     p.rows = rows; p.vocab = vocab; p.n = n;
     p.cap = softcap > 0.0f ? softcap : 0.0f;
-    p.recip = p.cap > 0.0f ? dlk_softcap_recip(p.cap) : 0.0f;
+    p.recip = p.cap > 0.0f ? fminf(1.0f / p.cap, FLT_MAX) : 0.0f;
     const bool chunks = (((uintptr_t)x | (uintptr_t)w | (uintptr_t)ldx | (uintptr_t)ldw) & 15) == 0;
     return chunks ? launch_i8_rows<true>(p, stream) : launch_i8_rows<false>(p, stream);
 }

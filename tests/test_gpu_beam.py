@@ -518,7 +518,7 @@ def test_search(cuda, groups, beams, V, n):
         lg = s.lg.cpu().numpy()
         qx, sx = quantized(h)
         want = 8.0 * np.tanh(product(qx, sx, qw, sw) / 8.0)
-        assert np.abs(lg - want).max() <= 8.0 * 2.0 ** -20              # (a rounded quotient and tanh of it)
+        assert np.abs(lg - want).max() <= 8.0 * 2.0 ** -20              # (16 half-steps of the cap)
         got = {key: v.cpu().numpy() for key, v in s.out[(k + 1) % 2].items()}
         exp, status = select(lg, beams, beams, scores=now["scores"], lengths=now["lengths"], finished=now["finished"],
                              hists=hists, mask=s.mask.cpu().numpy().view(np.uint32), eos=V - 1, alpha=0.6, rep=1.1,
