@@ -140,24 +140,62 @@ DLK_DEV void load_to_lds(const int8_t *src, int8_t *dst) {
                                      (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
 }
 
-/* BM rows of x and BN rows of w per workgroup, WGM x WGN waves, steps of BK bytes of n,
- * ST stages in LDS.  DMA: the rows of both are whole 16-byte chunks, loaded straight into
- * LDS; else through registers, any alignment. */
-template <int BM, int BN, int WGM, int WGN, int BK, int ST, int OCC, bool DMA, bool CAP>
-__global__ __launch_bounds__(WGM * WGN * 64, OCC) void logits_i8_kernel(I8Params p) {
+/* One tile's place: workgroups go to the XCDs in turn, so each XCD gets a run of tiles, the
+ * tiles of x for one tile of w side by side: w comes from memory once. */
+template <int BM, int BN>
+DLK_DEV bool tile_of(const I8Params &p, int &m0, int &v0) {
+    const int mtiles = (p.rows + BM - 1) / BM, vtiles = (p.vocab + BN - 1) / BN;
+    const int tile = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+    m0 = tile % mtiles * BM;
+    v0 = tile / mtiles * BN;
+    return tile < mtiles * vtiles;
+}
+
+/* The products of one staged step: x in xs, w in ws, BK bytes a row, chunks at place(). */
+template <int BK, int MF, int NF>
+DLK_DEV void multiply_stage(const int8_t *xs, const int8_t *ws, i4 (&acc)[MF][NF]) {
+    const int lr = lane_id() & 15, lk = lane_id() >> 4;
+#pragma unroll
+    for (int s = 0; s < BK / 64; s++) {
+        const int at = lr * BK + place<BK>(lr, s * 4 + lk) * 16;      /* (tiles start at multiples of 16 rows) */
+        i4 a[NF], b[MF];
+#pragma unroll
+        for (int f = 0; f < NF; f++) a[f] = *(const i4 *)&ws[f * 16 * BK + at];
+#pragma unroll
+        for (int m = 0; m < MF; m++) b[m] = *(const i4 *)&xs[m * 16 * BK + at];
+#pragma unroll
+        for (int m = 0; m < MF; m++)
+#pragma unroll
+            for (int f = 0; f < NF; f++)
+                acc[m][f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[f], b[m], acc[m][f], 0, 0, 0);
+    }
+}
+
+template <int MF, int NF>
+DLK_DEV void clear(i4 (&acc)[MF][NF]) {
+#pragma unroll
+    for (int m = 0; m < MF; m++)
+#pragma unroll
+        for (int f = 0; f < NF; f++) acc[m][f] = i4{0, 0, 0, 0};
+}
+
+/* Rows of whole 16-byte chunks: BM rows of x and BN of w per workgroup, WGM x WGN waves, steps
+ * of BK bytes of n loaded straight into LDS, ST stages in a ring: step it + ST - 1 is asked
+ * for while step it is multiplied, one barrier a step.  The loop holds nothing but that: with
+ * the last, shorter step in it the compiler waited for every load before each LDS read.  Few
+ * rows are bound by w's bytes: two workgroups a CU fill its LDS with loads in flight, long
+ * pieces of w's rows at a time (16 x 151,936 x 4,096: 116 us, 5.5 TB/s). */
+template <int BM, int BN, int WGM, int WGN, int BK, int ST, bool CAP>
+__global__ __launch_bounds__(WGM * WGN * 64, 2) void logits_i8_kernel(I8Params p) {
     constexpr int W = WGM * WGN, WM = BM / WGM, WN = BN / WGN, MF = WM / 16, NF = WN / 16;
     constexpr int CPR = BK / 16, RPI = 64 / CPR;   /* chunks of a row; rows that a wave loads at once */
     constexpr int NI = (BM + BN) / RPI / W;        /* loads of a wave per stage */
     constexpr int STAGE = (BM + BN) * BK;
-    static_assert((BM + BN) % (RPI * W) == 0 && BM % RPI == 0 && (BK == 64 || BK == 128 || BK == 256), "tiles");
+    static_assert((BM + BN) % (RPI * W) == 0 && BM % RPI == 0 && BK >= 64 && BK <= 512, "tiles");
     __shared__ __align__(1024) int8_t lds[ST * STAGE];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
-    /* workgroups go to the XCDs in turn: each XCD gets a run of tiles, the rows' tiles of one
-     * tile of w side by side, so that w comes from memory once */
-    const int mtiles = (p.rows + BM - 1) / BM, vtiles = (p.vocab + BN - 1) / BN;
-    const int tile = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
-    if (tile >= mtiles * vtiles) return;
-    const int m0 = tile % mtiles * BM, v0 = tile / mtiles * BN;
+    int m0, v0;
+    if (!tile_of<BM, BN>(p, m0, v0)) return;
     const int8_t *src[NI];                         /* the row of this lane's chunk */
     int at[NI];                                    /* and its place in the row */
 #pragma unroll
@@ -167,70 +205,98 @@ __global__ __launch_bounds__(WGM * WGN * 64, OCC) void logits_i8_kernel(I8Params
         src[j] = r < BM ? p.x + (int64_t)min(m0 + r, p.rows - 1) * p.ldx
                         : p.w + (int64_t)min(v0 + r - BM, p.vocab - 1) * p.ldw;
     }
-    i4 reg[DMA ? 1 : NI];
-    auto fetch = [&](int k0, int slot) {
+    auto fetch = [&](int it, int slot) {
 #pragma unroll
-        for (int j = 0; j < NI; j++) {
-            if (DMA && k0 + BK <= p.n) {
-                load_to_lds(src[j] + k0 + at[j], &lds[slot * STAGE + (j * W + wave) * 1024]);
-            } else {
-                const i4 v = k0 + BK <= p.n ? (i4)*(const i4_any *)(src[j] + k0 + at[j]) : load16_to(src[j], k0 + at[j], p.n);
-                if (DMA) *(i4 *)&lds[slot * STAGE + (j * W + wave) * 1024 + lane * 16] = v;
-                else reg[j] = v;
-            }
-        }
+        for (int j = 0; j < NI; j++) load_to_lds(src[j] + it * BK + at[j], &lds[slot * STAGE + (j * W + wave) * 1024]);
     };
-    auto put = [&](int slot) {
-        if (!DMA) {
-#pragma unroll
-            for (int j = 0; j < NI; j++) *(i4 *)&lds[slot * STAGE + (j * W + wave) * 1024 + lane * 16] = reg[j];
-        }
-    };
-    const int lr = lane & 15, lk = lane >> 4, wm = wave % WGM * WM, wn = wave / WGM * WN;
+    const int wm = wave % WGM * WM, wn = wave / WGM * WN;
     i4 acc[MF][NF];
-#pragma unroll
-    for (int m = 0; m < MF; m++)
-#pragma unroll
-        for (int f = 0; f < NF; f++) acc[m][f] = i4{0, 0, 0, 0};
-    const int steps = (p.n + BK - 1) / BK;
+    clear(acc);
+    const int steps = p.n / BK;
 #pragma unroll
     for (int s = 0; s < ST - 1; s++)
-        if (s < steps) { fetch(s * BK, s); put(s); }
+        if (s < steps) fetch(s, s);
     int slot = 0;
     for (int it = 0; it < steps; it++) {
         if (it + ST - 2 < steps) wait_loads<NI *(ST - 2)>();
         else wait_loads<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        const int next = slot == 0 ? ST - 1 : slot - 1;        /* the slot that step it - 1 has left */
-        if (it + ST - 1 < steps) fetch((it + ST - 1) * BK, next);
-        const int8_t *xs = &lds[slot * STAGE], *ws = xs + BM * BK;
-#pragma unroll
-        for (int s = 0; s < BK / 64; s++) {
-            i4 a[NF], b[MF];
-#pragma unroll
-            for (int f = 0; f < NF; f++) {
-                const int r = wn + f * 16 + lr;
-                a[f] = *(const i4 *)&ws[r * BK + place<BK>(BM + r, s * 4 + lk) * 16];
-            }
-#pragma unroll
-            for (int m = 0; m < MF; m++) {
-                const int r = wm + m * 16 + lr;
-                b[m] = *(const i4 *)&xs[r * BK + place<BK>(r, s * 4 + lk) * 16];
-            }
-#pragma unroll
-            for (int m = 0; m < MF; m++)
-#pragma unroll
-                for (int f = 0; f < NF; f++)
-                    acc[m][f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[f], b[m], acc[m][f], 0, 0, 0);
-        }
-        if (it + ST - 1 < steps) put(next);
+        /* the slot that step it - 1 has left */
+        if (it + ST - 1 < steps) fetch(it + ST - 1, slot == 0 ? ST - 1 : slot - 1);
+        multiply_stage<BK>(&lds[slot * STAGE + wm * BK], &lds[slot * STAGE + (BM + wn) * BK], acc);
         slot = slot == ST - 1 ? 0 : slot + 1;
+    }
+    if (p.n % BK != 0) {                           /* what is left of n, through registers, zeros past it */
+        __syncthreads();
+#pragma unroll 1
+        for (int j = 0; j < NI; j++) {
+            const int r = (j * W + wave) * RPI + lane / CPR;
+            const int8_t *row = r < BM ? p.x + (int64_t)min(m0 + r, p.rows - 1) * p.ldx
+                                       : p.w + (int64_t)min(v0 + r - BM, p.vocab - 1) * p.ldw;
+            *(i4 *)&lds[(j * W + wave) * 1024 + lane * 16] = load16_to(row, steps * BK + place<BK>(r, lane % CPR) * 16, p.n);
+        }
+        __syncthreads();
+        multiply_stage<BK>(&lds[wm * BK], &lds[(BM + wn) * BK], acc);
     }
     constexpr bool WIDE = NF >= 4;
     static_assert(!WIDE || W * 16 * (WN + 4) * 4 <= ST * STAGE, "room for the output");
     if (WIDE) __syncthreads();
     write_logits<CAP, WIDE>(p, acc, m0 + wm, v0 + wn, (float *)lds + (WIDE ? wave * 16 * (WN + 4) : 0));
+}
+
+/* Rows of any alignment: as above through registers, two stages in LDS and two on their
+ * way, so that a step's loads have two steps' time. */
+template <int BM, int BN, int WGM, int WGN, int BK, bool CAP>
+__global__ __launch_bounds__(WGM * WGN * 64, BM == 32 ? 3 : 4) void logits_i8_any_kernel(I8Params p) {
+    constexpr int W = WGM * WGN, WM = BM / WGM, WN = BN / WGN, MF = WM / 16, NF = WN / 16;
+    constexpr int CPR = BK / 16, RPI = 64 / CPR, NI = (BM + BN) / RPI / W, STAGE = (BM + BN) * BK;
+    static_assert((BM + BN) % (RPI * W) == 0 && BM % RPI == 0 && BK >= 64 && BK <= 512, "tiles");
+    __shared__ __align__(1024) int8_t lds[2 * STAGE];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
+    int m0, v0;
+    if (!tile_of<BM, BN>(p, m0, v0)) return;
+    const int8_t *src[NI];
+    int at[NI];
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+        const int r = (j * W + wave) * RPI + lane / CPR;
+        at[j] = place<BK>(r, lane % CPR) * 16;
+        src[j] = r < BM ? p.x + (int64_t)min(m0 + r, p.rows - 1) * p.ldx
+                        : p.w + (int64_t)min(v0 + r - BM, p.vocab - 1) * p.ldw;
+    }
+    auto load = [&](i4 (&reg)[NI], int k0) {
+        if (k0 + BK <= p.n) {
+#pragma unroll
+            for (int j = 0; j < NI; j++) reg[j] = *(const i4_any *)(src[j] + k0 + at[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NI; j++) reg[j] = load16_to(src[j], k0 + at[j], p.n);
+        }
+    };
+    auto put = [&](const i4 (&reg)[NI], int slot) {
+#pragma unroll
+        for (int j = 0; j < NI; j++) *(i4 *)&lds[slot * STAGE + (j * W + wave) * 1024 + lane * 16] = reg[j];
+    };
+    const int wm = wave % WGM * WM, wn = wave / WGM * WN;
+    i4 acc[MF][NF], even[NI], odd[NI];
+    clear(acc);
+    const int steps = (p.n + BK - 1) / BK;
+    load(even, 0);
+    if (steps > 1) load(odd, BK);
+    put(even, 0);
+    for (int it = 0; it < steps; it += 2) {
+        __syncthreads();
+        if (it + 2 < steps) load(even, (it + 2) * BK);
+        multiply_stage<BK>(&lds[wm * BK], &lds[(BM + wn) * BK], acc);
+        if (it + 1 >= steps) break;
+        put(odd, 1);
+        __syncthreads();
+        if (it + 3 < steps) load(odd, (it + 3) * BK);
+        multiply_stage<BK>(&lds[STAGE + wm * BK], &lds[STAGE + (BM + wn) * BK], acc);
+        if (it + 2 < steps) put(even, 0);
+    }
+    write_logits<CAP, false>(p, acc, m0 + wm, v0 + wn, nullptr);
 }
 
 /* The product of many rows: 256 x 256 tiles, eight waves of 128 x 64, steps of 128 bytes (whole
@@ -245,10 +311,8 @@ __global__ __launch_bounds__(512, 2) void logits_i8_wide_kernel(I8Params p) {
     __shared__ __align__(1024) int8_t lds[2 * (XST + WST)];
     int8_t *const ldw = lds + 2 * XST;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
-    const int mtiles = (p.rows + BM - 1) / BM, vtiles = (p.vocab + BN - 1) / BN;
-    const int tile = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
-    if (tile >= mtiles * vtiles) return;
-    const int m0 = tile % mtiles * BM, v0 = tile / mtiles * BN;
+    int m0, v0;
+    if (!tile_of<BM, BN>(p, m0, v0)) return;
     const int8_t *sx[NX], *sw[NW];
 #pragma unroll
     for (int j = 0; j < NX; j++) {
@@ -276,10 +340,7 @@ __global__ __launch_bounds__(512, 2) void logits_i8_wide_kernel(I8Params p) {
         for (int m = 0; m < MF; m++) b[m] = *(const i4 *)&xs[m * 16 * BK];
     };
     i4 acc[MF][NF];
-#pragma unroll
-    for (int m = 0; m < MF; m++)
-#pragma unroll
-        for (int f = 0; f < NF; f++) acc[m][f] = i4{0, 0, 0, 0};
+    clear(acc);
     auto multiply = [&](const i4 (&a)[NF], const i4 (&b)[MF]) {
 #pragma unroll
         for (int m = 0; m < MF; m++)
@@ -341,34 +402,28 @@ __global__ __launch_bounds__(512, 2) void logits_i8_wide_kernel(I8Params p) {
     write_logits<CAP, true>(p, acc, m0 + wm, v0 + wn, (float *)lds + wave * 16 * (WN + 4));
 }
 
-int launch_i8_wide(const I8Params &p, hipStream_t stream) {
-    const int64_t tiles = (((int64_t)p.vocab + 255) / 256) * (((int64_t)p.rows + 255) / 256);
+/* One launch of `kernel`, tiles of BM x BN; the grid a multiple of the XCDs. */
+int launch_tiles(void (*kernel)(I8Params), int bm, int bn, int threads, const I8Params &p, hipStream_t stream) {
+    const int64_t tiles = (((int64_t)p.vocab + bn - 1) / bn) * (((int64_t)p.rows + bm - 1) / bm);
     if (tiles > 0x3fffffff) return DLK_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)((tiles + 7) / 8 * 8));
-    if (p.cap > 0.0f) hipLaunchKernelGGL((logits_i8_wide_kernel<true>), grid, dim3(512), 0, stream, p);
-    else hipLaunchKernelGGL((logits_i8_wide_kernel<false>), grid, dim3(512), 0, stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(threads), 0, stream, p);
     return hipGetLastError() == hipSuccess ? DLK_OK : DLK_ERR_HIP;
 }
 
-template <int BM, int BN, int WGM, int WGN, int BK, int ST, int OCC, bool DMA>
+template <int BM, int BN, int WGM, int WGN, int BK, int ST>
 int launch_i8(const I8Params &p, hipStream_t stream) {
-    const int64_t tiles = (((int64_t)p.vocab + BN - 1) / BN) * (((int64_t)p.rows + BM - 1) / BM);
-    if (tiles > 0x3fffffff) return DLK_ERR_UNSUPPORTED;
-    const dim3 grid((unsigned)((tiles + 7) / 8 * 8)), block(WGM * WGN * 64);
-    if (p.cap > 0.0f)
-        hipLaunchKernelGGL((logits_i8_kernel<BM, BN, WGM, WGN, BK, ST, OCC, DMA, true>), grid, block, 0, stream, p);
-    else
-        hipLaunchKernelGGL((logits_i8_kernel<BM, BN, WGM, WGN, BK, ST, OCC, DMA, false>), grid, block, 0, stream, p);
-    return hipGetLastError() == hipSuccess ? DLK_OK : DLK_ERR_HIP;
+    return launch_tiles(p.cap > 0.0f ? logits_i8_kernel<BM, BN, WGM, WGN, BK, ST, true>
+                                     : logits_i8_kernel<BM, BN, WGM, WGN, BK, ST, false>, BM, BN, WGM * WGN * 64, p, stream);
 }
 
-template <bool DMA>
-int launch_i8_rows(const I8Params &p, hipStream_t stream) {
-    if (p.rows <= 16) return launch_i8<16, 64, 1, 4, 256, 3, 2, DMA>(p, stream);
-    if (p.rows <= 32) return launch_i8<32, 64, 1, 4, 128, 4, 2, DMA>(p, stream);
-    if (p.rows <= 64) return launch_i8<64, 64, 1, 4, 128, 4, 2, DMA>(p, stream);
-    if (DMA && p.rows > 128) return launch_i8_wide(p, stream);
-    return launch_i8<128, 128, 2, 2, 128, 2, 2, DMA>(p, stream);
+template <int BM, int BN, int WGM, int WGN, int BK>
+int launch_i8_any(const I8Params &p, hipStream_t stream) {
+    return launch_tiles(p.cap > 0.0f ? logits_i8_any_kernel<BM, BN, WGM, WGN, BK, true>
+                                     : logits_i8_any_kernel<BM, BN, WGM, WGN, BK, false>, BM, BN, WGM * WGN * 64, p, stream);
+}
+
+int launch_i8_wide(const I8Params &p, hipStream_t stream) {
+    return launch_tiles(p.cap > 0.0f ? logits_i8_wide_kernel<true> : logits_i8_wide_kernel<false>, 256, 256, 512, p, stream);
 }
 
 }  // namespace dlk
@@ -389,6 +444,28 @@ extern "C" int dlk_logits_i8(const int8_t *x, int64_t ldx, const float *x_scale,
     p.rows = rows; p.vocab = vocab; p.n = n;
     p.cap = softcap > 0.0f ? softcap : 0.0f;
     p.recip = p.cap > 0.0f ? fminf(1.0f / p.cap, FLT_MAX) : 0.0f;
+    /* Tiles by the rows (us at 32,000 and 151,936 ids of n = 4,096; the smallest tile that holds
+     * the rows unless said otherwise):
+     *   16 rows     64 ids of 512 bytes a step 27.4, 116; of 256 bytes and 4 stages 28.4, 119
+     *   32          64 ids of 256 bytes 30.1, 128; 128 ids of 128 bytes 32.7, 130
+     *   64          64 ids of 128 bytes 34.8, 145; of 256 bytes 34.2, 163
+     *   128         128 ids of 64 bytes 41.3, 173; of 128 bytes 44.5, 190
+     *   200         128 x 256 47.9, 219; 128 x 128 58.1, 234; 256 x 256 62.2, 221
+     *   300         128 x 256 76.5, 283; 256 x 256 67.5, 306
+     *   512         256 x 256 (262,144 ids) 558; 128 x 256 657; 128 x 128 787 */
     const bool chunks = (((uintptr_t)x | (uintptr_t)w | (uintptr_t)ldx | (uintptr_t)ldw) & 15) == 0;
-    return chunks ? launch_i8_rows<true>(p, stream) : launch_i8_rows<false>(p, stream);
+    if (!chunks) {
+        /* (33 x 50,257 x 2,047: 35.6; 300 x 100,001 x 4,097: 433, in tiles of 128 rows 562) */
+        if (rows <= 16) return launch_i8_any<16, 64, 1, 4, 256>(p, stream);
+        if (rows <= 32) return launch_i8_any<32, 64, 1, 4, 256>(p, stream);
+        return launch_i8_any<64, 128, 2, 4, 128>(p, stream);
+    }
+    if (rows <= 16) return launch_i8<16, 64, 1, 4, 512, 2>(p, stream);
+    if (rows <= 32) return launch_i8<32, 64, 2, 2, 256, 3>(p, stream);
+    if (rows <= 64) return launch_i8<64, 64, 2, 2, 128, 4>(p, stream);
+    if (rows <= 128) return launch_i8<128, 128, 2, 2, 64, 3>(p, stream);
+    /* past that tiles of 256 rows where they leave little empty */
+    const int64_t by128 = ((int64_t)rows + 127) / 128 * 128, by256 = ((int64_t)rows + 255) / 256 * 256;
+    if (rows <= 384 || by128 * 6 < by256 * 5) return launch_i8<128, 256, 2, 4, 128, 3>(p, stream);
+    return launch_i8_wide(p, stream);
 }

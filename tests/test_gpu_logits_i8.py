@@ -235,3 +235,22 @@ def test_rows_far_apart(cuda):
     w2 = torch.randint(-127, 128, (2, n), device="cuda", generator=g, dtype=torch.int8)
     want = (w2.double() @ x.double().t()).float()
     assert torch.equal(api.logits_i8(w2, two, x, one, out=out), want)
+
+
+@pytest.mark.parametrize("rows", [1, 16, 17, 32, 33, 64, 65, 128, 129, 256, 257, 384, 385, 512, 520, 700])
+@pytest.mark.parametrize("n", [64, 512, 1000, 1536])
+@pytest.mark.parametrize("packed", [False, True])
+def test_logits_tiles(cuda, rows, n, packed):
+    """Every tile, full and partly filled, one stage, several, and a shorter last one; the sums are exact."""
+    import torch
+    from diskllm_amd import api
+    V = 777
+    g = torch.Generator("cuda").manual_seed(rows + n)
+    ld = n + 1 if packed else (n + 15) // 16 * 16
+    x = torch.randint(-128, 128, (rows, ld), device="cuda", generator=g, dtype=torch.int8)[:, :n]
+    w = torch.randint(-128, 128, (V, ld), device="cuda", generator=g, dtype=torch.int8)[:, :n]
+    one, each = torch.ones(rows, device="cuda"), torch.ones(V, device="cuda")
+    out = api.logits_i8(x, one, w, each)
+    want = (x.double() @ w.double().t()).float()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
