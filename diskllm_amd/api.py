@@ -162,6 +162,7 @@ def results(db: DeviceBatch) -> dict:
 # Tensors on one device, the call on that device's current stream unless `stream` says
 # otherwise; what does not fit raises ValueError before anything is launched.
 
+_F32, _I32, _I8, _U8 = torch.float32, torch.int32, torch.int8, torch.uint8
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
@@ -170,34 +171,37 @@ def _want(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _on(device, *tensors) -> None:
-    for t in tensors:
-        _want(t is None or t.device == device, "tensors on different devices")
+def _rows2d(t: torch.Tensor, dev: int, dtype, what: str):
+    """(rows, n, row stride) of a [rows, n] tensor whose rows are contiguous (dtype None: any)."""
+    if t.dim() != 2 or (dtype is not None and t.dtype is not dtype) or t.get_device() != dev:
+        raise ValueError(f"{what}: [rows, n] of {dtype} on the call's device is wanted")
+    rows, n = t.shape
+    ld, one = t.stride()
+    if rows <= 1 and ld < n:
+        ld = n
+    if (one != 1 and n > 1) or ld < n:
+        raise ValueError(f"{what}: contiguous rows that do not overlap are wanted")
+    return rows, n, ld
 
 
-def _rows2d(t: torch.Tensor, what: str) -> int:
-    """The row stride of a [rows, n] tensor whose rows are contiguous."""
-    _want(t.dim() == 2 and (t.shape[1] == 1 or t.stride(1) == 1), f"{what}: [rows, n] with contiguous rows is wanted")
-    ld = t.stride(0)
-    if t.shape[0] <= 1:
-        return max(ld, t.shape[1])
-    _want(ld >= t.shape[1], f"{what}: rows overlap")
-    return ld
+def _flat(t: torch.Tensor, n: int, dev: int, dtype, what: str) -> int:
+    """The address of at least n contiguous values."""
+    if t.dtype is not dtype or t.numel() < n or not t.is_contiguous() or t.get_device() != dev:
+        raise ValueError(f"{what}: at least {n} contiguous values of {dtype} on the call's device are wanted")
+    return t.data_ptr()
 
 
-def _flat(t: Optional[torch.Tensor], n: int, dtype, what: str) -> None:
-    _want(t is None or (t.numel() >= n and t.dtype == dtype and t.is_contiguous()),
-          f"{what}: at least {n} contiguous values of {dtype} are wanted")
-
-
-def _call(device, stream, what: str, fn, *args) -> None:
-    """fn(*args, stream) with `device` current (the kernels run there)."""
-    _want(device.type == "cuda", f"{what}: tensors on the GPU are wanted")
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, stream if stream is not None else torch.cuda.current_stream().cuda_stream)
+def _call(dev: int, stream, what: str, fn, *args) -> None:
+    """fn(*args, stream) with device `dev` current (the kernels run there)."""
+    if dev < 0:
+        raise ValueError(f"{what}: tensors on the GPU are wanted")
+    if stream is None:
+        stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, stream if stream is not None else torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(dev):
+            rc = fn(*args, stream)
     if rc != 0:
         _lib.check(rc, what)
 
@@ -206,21 +210,20 @@ def quantize_rows(x: torch.Tensor, q: Optional[torch.Tensor] = None, scale: Opti
                   stream: Optional[int] = None):
     """(q int8 [rows, n], scale float32 [rows]) of x [rows, n] in float32, bfloat16 or float16: hidden states with a
     scale per token, or weights [vocab, n] with one per channel (dlk_quantize_rows)."""
-    _want(x.dtype in _DTYPES, "x: float32, bfloat16 or float16 is wanted")
-    ldx = _rows2d(x, "x")
-    rows, n = x.shape
+    dt = _DTYPES.get(x.dtype)
+    _want(dt is not None, "x: float32, bfloat16 or float16 is wanted")
+    dev = x.get_device()
+    rows, n, ldx = _rows2d(x, dev, None, "x")
     if q is None:
-        q = torch.empty((rows, (n + 15) // 16 * 16), dtype=torch.int8, device=x.device)[:, :n]
+        q = torch.empty((rows, (n + 15) // 16 * 16), dtype=_I8, device=x.device)[:, :n]
     if scale is None:
-        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    ldq = _rows2d(q, "q")
-    _want(q.shape == x.shape and q.dtype == torch.int8, "q: int8 of x's shape is wanted")
-    _flat(scale, rows, torch.float32, "scale")
-    _on(x.device, q, scale)
-    if rows == 0:
-        return q, scale
-    _call(x.device, stream, "dlk_quantize_rows", _lib.lib().dlk_quantize_rows, x.data_ptr(), _DTYPES[x.dtype], ldx,
-          rows, n, q.data_ptr(), ldq, scale.data_ptr())
+        scale = torch.empty(rows, dtype=_F32, device=x.device)
+    q_rows, q_n, ldq = _rows2d(q, dev, _I8, "q")
+    _want(q_rows == rows and q_n == n, "q: x's shape is wanted")
+    at = _flat(scale, rows, dev, _F32, "scale")
+    if rows:
+        _call(dev, stream, "dlk_quantize_rows", _lib.lib().dlk_quantize_rows, x.data_ptr(), dt, ldx, rows, n,
+              q.data_ptr(), ldq, at)
     return q, scale
 
 
@@ -228,22 +231,18 @@ def logits_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
               out: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> torch.Tensor:
     """Logits float32 [rows, vocab] of x int8 [rows, n] (x_scale [rows]) over w int8 [vocab, n] (w_scale [vocab]),
     soft-capped where softcap > 0 (dlk_logits_i8)."""
-    _want(x.dtype == torch.int8 and w.dtype == torch.int8, "x and w: int8 is wanted")
-    ldx, ldw = _rows2d(x, "x"), _rows2d(w, "w")
-    rows, n = x.shape
-    V = w.shape[0]
-    _want(w.shape[1] == n, "x and w: rows of one length are wanted")
+    dev = x.get_device()
+    rows, n, ldx = _rows2d(x, dev, _I8, "x")
+    V, w_n, ldw = _rows2d(w, dev, _I8, "w")
+    _want(w_n == n, "x and w: rows of one length are wanted")
     if out is None:
-        out = torch.empty((rows, (V + 63) // 64 * 64), dtype=torch.float32, device=x.device)[:, :V]
-    ld = _rows2d(out, "out")
-    _want(out.shape == (rows, V) and out.dtype == torch.float32, "out: float32 [rows, vocab] is wanted")
-    _flat(x_scale, rows, torch.float32, "x_scale")
-    _flat(w_scale, V, torch.float32, "w_scale")
-    _on(x.device, x_scale, w, w_scale, out)
-    if rows == 0:
-        return out
-    _call(x.device, stream, "dlk_logits_i8", _lib.lib().dlk_logits_i8, x.data_ptr(), ldx, x_scale.data_ptr(),
-          w.data_ptr(), ldw, w_scale.data_ptr(), rows, V, n, float(softcap), out.data_ptr(), ld)
+        out = torch.empty((rows, (V + 63) // 64 * 64), dtype=_F32, device=x.device)[:, :V]
+    o_rows, o_n, ld = _rows2d(out, dev, _F32, "out")
+    _want(o_rows == rows and o_n == V, "out: [rows, vocab] is wanted")
+    xs, ws = _flat(x_scale, rows, dev, _F32, "x_scale"), _flat(w_scale, V, dev, _F32, "w_scale")
+    if rows:
+        _call(dev, stream, "dlk_logits_i8", _lib.lib().dlk_logits_i8, x.data_ptr(), ldx, xs, w.data_ptr(), ldw, ws,
+              rows, V, n, softcap, out.data_ptr(), ld)
     return out
 
 
@@ -257,53 +256,42 @@ def beam_select(logits: torch.Tensor, beams: int, n_out: int, *, scores: Optiona
                 stream: Optional[int] = None) -> dict:
     """One step of a beam search over logits float32 [groups * beams, vocab] (dlk_beam_select): tokens, parents,
     lengths (int32), scores (float32) and finished (uint8) of the n_out best continuations of each group."""
-    _want(logits.dtype == torch.float32, "logits: float32 is wanted")
-    ld = _rows2d(logits, "logits")
-    rows, V = logits.shape
+    dev = logits.get_device()
+    rows, V, ld = _rows2d(logits, dev, _F32, "logits")
     _want(beams > 0 and n_out > 0 and rows % beams == 0, "logits: whole groups of beams are wanted")
     groups = rows // beams
-    dev = logits.device
+    n = groups * n_out
     if out is None:
-        out = dict(tokens=torch.empty(groups * n_out, dtype=torch.int32, device=dev),
-                   parents=torch.empty(groups * n_out, dtype=torch.int32, device=dev),
-                   scores=torch.empty(groups * n_out, dtype=torch.float32, device=dev),
-                   lengths=torch.empty(groups * n_out, dtype=torch.int32, device=dev),
-                   finished=torch.empty(groups * n_out, dtype=torch.uint8, device=dev))
-    for k, t, n, dt in (("scores", scores, rows, torch.float32), ("lengths", lengths, rows, torch.int32),
-                        ("finished", finished, rows, torch.uint8), ("hist_off", hist_off, rows + 1, torch.int32),
-                        ("hist_ids", hist_ids, 0, torch.int32), ("mask_row", mask_row, rows, torch.int32),
-                        ("status", status, 1, torch.int32)):
-        if t is not None:
-            _flat(t, n, dt, k)
-            _want(t.device == dev, "tensors on different devices")
-    mask_ld = 0
+        i32, at = torch.empty((3, n), dtype=_I32, device=logits.device), logits.device
+        out = dict(tokens=i32[0], parents=i32[1], lengths=i32[2], scores=torch.empty(n, dtype=_F32, device=at),
+                   finished=torch.empty(n, dtype=_U8, device=at))
+    sc = 0 if scores is None else _flat(scores, rows, dev, _F32, "scores")
+    ln = 0 if lengths is None else _flat(lengths, rows, dev, _I32, "lengths")
+    fi = 0 if finished is None else _flat(finished, rows, dev, _U8, "finished")
+    ho = 0 if hist_off is None else _flat(hist_off, rows + 1, dev, _I32, "hist_off")
+    hi = 0 if hist_ids is None else _flat(hist_ids, 0, dev, _I32, "hist_ids") or ho     # (an empty tensor has no address)
+    mk = mask_ld = 0
+    mr = 0 if mask_row is None else _flat(mask_row, rows, dev, _I32, "mask_row")
     if mask is not None:
-        mask_ld = _rows2d(mask, "mask")
-        _want(mask.dtype == torch.int32 and mask.shape[1] >= (V + 31) // 32 and mask.device == dev and
-              (mask_row is not None or mask.shape[0] >= rows), "mask: int32 words of every row are wanted")
-    for k, dt in (("tokens", torch.int32), ("parents", torch.int32), ("scores", torch.float32),
-                  ("lengths", torch.int32), ("finished", torch.uint8)):
-        _flat(out[k], groups * n_out, dt, k)
-        _want(out[k].device == dev, "tensors on different devices")
-    if groups == 0:
-        return out
-    b = _lib.BeamBatch(
-        logits=logits.data_ptr(), ld=ld, hist_off=_ptr(hist_off),
-        hist_ids=_ptr(hist_ids) or _ptr(hist_off) if hist_ids is not None else None,   # (an empty tensor has no address)
-        mask=_ptr(mask), mask_ld=mask_ld, mask_row=_ptr(mask_row), scores=_ptr(scores), lengths=_ptr(lengths), finished=_ptr(finished),
-        out_tokens=out["tokens"].data_ptr(), out_parents=out["parents"].data_ptr(),
-        out_scores=out["scores"].data_ptr(), out_lengths=out["lengths"].data_ptr(),
-        out_finished=out["finished"].data_ptr(), status=_ptr(status))
-    p = _lib.BeamParams(beams, n_out, eos_id, length_penalty, repeat_penalty, frequency_penalty, presence_penalty,
-                        order, max_history)
-    _call(dev, stream, "dlk_beam_select", _lib.lib().dlk_beam_select, C.byref(b), groups, V, C.byref(p))
+        m_rows, words, mask_ld = _rows2d(mask, dev, _I32, "mask")
+        _want(words >= (V + 31) // 32 and (mr or m_rows >= rows), "mask: the words of every row are wanted")
+        mk = mask.data_ptr()
+    st = 0 if status is None else _flat(status, 1, dev, _I32, "status")
+    to = (_flat(out["tokens"], n, dev, _I32, "tokens"), _flat(out["parents"], n, dev, _I32, "parents"),
+          _flat(out["scores"], n, dev, _F32, "scores"), _flat(out["lengths"], n, dev, _I32, "lengths"),
+          _flat(out["finished"], n, dev, _U8, "finished"))
+    if groups:
+        _call(dev, stream, "dlk_beam_select", _lib.lib().dlk_beam_select,
+              _lib.BeamBatch(logits.data_ptr(), ld, ho, hi, mk, mask_ld, mr, sc, ln, fi, *to, st), groups, V,
+              _lib.BeamParams(beams, n_out, eos_id, length_penalty, repeat_penalty, frequency_penalty,
+                              presence_penalty, order, max_history))
     return out
 
 
 def _span(sizes, strides) -> Optional[tuple]:
     """(count, stride) of several dimensions walked as one, or None where they are no single stride."""
     n, stride = 1, 0
-    for size, st in reversed(list(zip(sizes, strides))):
+    for size, st in zip(reversed(sizes), reversed(strides)):
         if size == 1:
             continue
         if n == 1:
@@ -321,33 +309,36 @@ def beam_state(src: torch.Tensor, dst: Optional[torch.Tensor] = None, row_dim: i
     first `length` entries of dimension length_dim where that is given (the filled part of a cache).  The
     dimensions before the rows, those up to length_dim and those from it on have to be one stride each.  The
     caller keeps the tensors."""
-    dst = src if dst is None else dst
-    nd = src.dim()
-    _want(0 <= row_dim < nd and dst.dim() == nd and dst.dtype == src.dtype, "dst: a tensor of src's kind is wanted")
-    cut = row_dim + 1 if length_dim is None else length_dim
-    _want(row_dim < cut < nd or length_dim is None, "length_dim: a dimension after the rows is wanted")
     shape = list(src.shape)
+    nd, rows, dst_rows = len(shape), shape[row_dim] if row_dim < len(shape) else 0, 0
+    cut = row_dim + 1 if length_dim is None else length_dim
+    _want(0 <= row_dim < nd and (length_dim is None or row_dim < cut < nd), "length_dim: a dimension after the rows is wanted")
     if length_dim is not None and length is not None:
-        _want(0 <= length <= min(src.shape[length_dim], dst.shape[length_dim]), "length: more than the tensors hold")
-        shape[length_dim] = length
-    _want(all(a == b for i, (a, b) in enumerate(zip(src.shape, dst.shape)) if i not in (row_dim, length_dim)) and
-          (length_dim is None or shape[length_dim] <= dst.shape[length_dim]), "dst: another shape than src's")
+        _want(0 <= length <= shape[cut], "length: more than the tensors hold")
+        shape[cut] = length
+    dst_rows = rows
+    if dst is not None:
+        other = list(dst.shape)
+        _want(len(other) == nd and dst.dtype == src.dtype, "dst: a tensor of src's kind is wanted")
+        dst_rows = other[row_dim]
+        other[row_dim] = rows
+        if length_dim is not None and other[cut] >= shape[cut]:
+            other[cut] = shape[cut]
+        _want(other == shape, "dst: another shape than src's")
     item = src.element_size()
-    s = _lib.BeamState()
-    for t, k in ((src, "src"), (dst, "dst")):
-        outer = _span(shape[:row_dim], t.stride()[:row_dim])
-        inner = _span(shape[row_dim + 1:cut], t.stride()[row_dim + 1:cut])
-        rest = _span(shape[cut:], t.stride()[cut:])
-        _want(None not in (outer, inner, rest) and (rest[0] == 1 or rest[1] == 1),
-              f"{k}: strides that are not one per part, or rows whose entries are apart")
-        setattr(s, k, t.data_ptr())
-        setattr(s, k + "_row", t.stride(row_dim) * item)
-        setattr(s, k + "_outer", outer[1] * item)
-        setattr(s, k + "_inner", inner[1] * item)
-        s.n_outer, s.n_inner, s.bytes = outer[0], inner[0], rest[0] * item
-    if 0 in shape:
-        s.bytes = 0
-    s.rows = (src.shape[row_dim], dst.shape[row_dim], src.device, dst.device)
+
+    def layout(t):
+        st = t.stride()
+        outer, inner = _span(shape[:row_dim], st[:row_dim]), _span(shape[row_dim + 1:cut], st[row_dim + 1:cut])
+        rest = _span(shape[cut:], st[cut:])
+        _want(outer is not None and inner is not None and rest is not None and (rest[0] == 1 or rest[1] == 1),
+              "strides that are not one per part, or rows whose entries are apart")
+        return t.data_ptr(), st[row_dim] * item, outer, inner, rest[0] * item
+    at, row, outer, inner, size = layout(src)
+    d_at, d_row, d_outer, d_inner, _ = (at, row, outer, inner, size) if dst is None else layout(dst)
+    s = _lib.BeamState(at, d_at, 0 if 0 in shape else size, row, outer[1] * item, inner[1] * item, d_row,
+                       d_outer[1] * item, d_inner[1] * item, outer[0], inner[0])
+    s.rows = (rows, dst_rows, src.get_device(), src.get_device() if dst is None else dst.get_device())
     return s
 
 
@@ -355,34 +346,36 @@ def beam_history(off: torch.Tensor, ids: torch.Tensor, tokens: Optional[torch.Te
                  out_off: torch.Tensor, out_ids: torch.Tensor) -> _lib.BeamHistory:
     """The rows' histories (CSR) and the tokens to append, for beam_reorder; out_ids has room for max_history ids
     of every new row.  The caller keeps the tensors."""
-    for k, t in (("off", off), ("ids", ids), ("tokens", tokens), ("out_off", out_off), ("out_ids", out_ids)):
-        _flat(t, 0, torch.int32, k)
-        _want(t is None or t.device == off.device, "tensors on different devices")
-    h = _lib.BeamHistory(off.data_ptr(), ids.data_ptr() or off.data_ptr(), _ptr(tokens), max_history, out_off.data_ptr(),
-                         out_ids.data_ptr())
-    h.sizes = (off.numel(), None if tokens is None else tokens.numel(), out_off.numel(), out_ids.numel(), off.device)
+    dev = off.get_device()
+    at = _flat(off, 0, dev, _I32, "off")
+    h = _lib.BeamHistory(at, _flat(ids, 0, dev, _I32, "ids") or at,
+                         0 if tokens is None else _flat(tokens, 0, dev, _I32, "tokens"), max_history,
+                         _flat(out_off, 0, dev, _I32, "out_off"), _flat(out_ids, 0, dev, _I32, "out_ids"))
+    h.sizes = (off.numel(), None if tokens is None else tokens.numel(), out_off.numel(), out_ids.numel(), dev)
     return h
+
+
+_STATES = {n: _lib.BeamState * n for n in range(1, 9)}
 
 
 def beam_reorder(parents: torch.Tensor, beams: int, n_out: int, states=(), history: Optional[_lib.BeamHistory] = None,
                  stream: Optional[int] = None) -> None:
     """The states (beam_state) and histories (beam_history) of the new rows from their parents' (dlk_beam_reorder);
     parents int32 [groups * n_out] as beam_select writes them."""
-    _flat(parents, 0, torch.int32, "parents")
-    _want(beams > 0 and n_out > 0 and parents.numel() % n_out == 0, "parents: whole groups of n_out are wanted")
-    groups = parents.numel() // n_out
-    dev = parents.device
+    dev = parents.get_device()
+    at = _flat(parents, 0, dev, _I32, "parents")
+    total = parents.numel()
+    _want(beams > 0 and n_out > 0 and total % n_out == 0, "parents: whole groups of n_out are wanted")
+    groups = total // n_out
     for s in states:
-        _want(s.rows[0] >= groups * beams and s.rows[1] >= groups * n_out, "states: fewer rows than the groups have")
-        _want(s.rows[2] == dev and s.rows[3] == dev, "tensors on different devices")
+        _want(s.rows[0] >= groups * beams and s.rows[1] >= total, "states: fewer rows than the groups have")
+        _want(s.rows[2] == dev and s.rows[3] == dev, "states: tensors on the call's device are wanted")
     if history is not None:
         n_off, n_tok, n_out_off, n_out_ids, where = history.sizes
-        _want(n_off >= groups * beams + 1 and n_out_off >= groups * n_out + 1 and
-              (n_tok is None or n_tok >= groups * n_out) and
-              n_out_ids >= groups * n_out * history.max_history, "history: fewer entries than the groups need")
-        _want(where == dev, "tensors on different devices")
-    if groups == 0:
-        return
-    arr = (_lib.BeamState * max(len(states), 1))(*states)
-    _call(dev, stream, "dlk_beam_reorder", _lib.lib().dlk_beam_reorder, parents.data_ptr(), groups, beams, n_out, arr,
-          len(states), C.byref(history) if history is not None else None)
+        _want(n_off >= groups * beams + 1 and n_out_off >= total + 1 and (n_tok is None or n_tok >= total) and
+              n_out_ids >= total * history.max_history, "history: fewer entries than the groups need")
+        _want(where == dev, "history: tensors on the call's device are wanted")
+    if groups:
+        k = len(states)
+        arr = (_STATES.get(k) or _lib.BeamState * k)(*states) if k else None
+        _call(dev, stream, "dlk_beam_reorder", _lib.lib().dlk_beam_reorder, at, groups, beams, n_out, arr, k, history)

@@ -10,8 +10,7 @@
 namespace dlk {
 
 constexpr int kBeamThreads = 256;
-constexpr int kBeamGroups = 8;                                  /* groups of four logits per thread */
-constexpr int kBeamSlice = kBeamThreads * kBeamGroups * 4;      /* logits of one workgroup */
+constexpr int kBeamBatch = kBeamThreads * 16;                   /* logits of a batch: four groups of four per thread */
 
 /* What a workgroup says of its slice of a row. */
 struct BeamSlot {
@@ -40,10 +39,28 @@ struct BeamParams {
     float rep, freq, pres;
     int g0;              /* first group of the launch */
     int slices;          /* workgroups per row */
+    int batches;         /* of each */
     uint32_t *counters;  /* [groups] zero between launches */
     BeamSlot *slots;     /* [rows][slices] */
     uint64_t *cands;     /* [rows][slices][n] */
 };
+
+/* Batches of each workgroup for rows of `vocab` logits: about 1,100 workgroups (some four a CU,
+ * resident together) where that takes at most six batches each, so that a workgroup's
+ * fixed 5 us are paid few times (us by batches of each:
+ *   64 x 151,936 with histories   1: 46, 2: 33.4, 3: 32.9, 4: 35, 8: 50
+ *   128 x 50,257 in groups of 16  1: 39, 2: 32.5, 3: 31.6, 4: 38
+ *   512 x 262,144                 1: 302, 2: 185, 3: 156, 4: 145, 8: 145
+ *   4 x 32,000                    1: 11.4, 2: 13.8);
+ * more where the merge would meet over 256 lists a group, which it takes in one round trip. */
+inline int beam_batches(int64_t rows, int beams, int vocab) {
+    const int64_t per_row = ((int64_t)vocab + kBeamBatch - 1) / kBeamBatch;
+    int64_t m = (rows * per_row + 1099) / 1100;
+    if (m > 6) m = 6;
+    if (m < (per_row * beams + 255) / 256) m = (per_row * beams + 255) / 256;
+    const int64_t slices = (per_row + m - 1) / m;
+    return (int)((per_row + slices - 1) / slices);
+}
 
 }  // namespace dlk
 

@@ -2,7 +2,7 @@
  * beam_select.hip -- one step of a beam search: of the continuations (row, id) of a group
  * of rows the n with the largest score + log softmax(l)[id] (dlk_beam_select).
  *
- * One workgroup reads a slice of 8,192 logits of a row once, into registers; masks and
+ * One workgroup reads a slice of 2,048 to 8,192 logits of a row once, into registers; masks and
  * penalises them; sums exp(l - slice maximum) in 64 bits; and lists the slice's n
  * largest entries in order.  Log softmax is increasing in l, so a row's n best
  * continuations are its n largest logits and none of the others is needed again.  The
@@ -25,23 +25,46 @@ DLK_DEV uint64_t bget64(const uint64_t *a) {
     return __hip_atomic_load((uint64_t *)a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-/* exp(x) for x <= 0 to some 1e-11: 2^k times the series of e^r, |r| <= ln2 / 2. */
+/* a * b + c with c in scalar registers and its own destination (the compiler's choice adds
+ * a move of c for each). */
+DLK_DEV double fma3(double a, double b, double c) {
+    double d;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
+    return d;
+}
+
+/* exp(x) for x <= 0 to 5e-11 of it (below -700: of exp(-700)): 2^k times a polynomial of e^r on
+ * |r| <= ln2 / 2, exactly 1 at 0 (sums are rescaled by it many times), of the degree that
+ * brings its largest error to 4.7e-11 (least squares re-weighted to equal peaks).  k by
+ * the addition that leaves it in the sum's low bits. */
 DLK_DEV double exp_neg(double x) {
+    const double round = 6755399441055744.0;             /* 1.5 * 2^52 */
     x = fmax(x, -700.0);
-    const double k = rint(x * 1.4426950408889634);
-    const double r = fma(-k, 1.9082149292705877e-10, fma(-k, 0.693147180369123816490, x));
-    double y = 1.0 / 3628800.0;
-    y = fma(y, r, 1.0 / 362880.0);
-    y = fma(y, r, 1.0 / 40320.0);
-    y = fma(y, r, 1.0 / 5040.0);
-    y = fma(y, r, 1.0 / 720.0);
-    y = fma(y, r, 1.0 / 120.0);
-    y = fma(y, r, 1.0 / 24.0);
-    y = fma(y, r, 1.0 / 6.0);
-    y = fma(y, r, 0.5);
+    const double t = fma(x, 1.4426950408889634, round);
+    const double r = fma(t - round, -0.6931471805599453, x);
+    double y = 0.00019767657717010163;
+    y = fma3(y, r, 0.0013945909123789359);
+    y = fma3(y, r, 0.008333568991418506);
+    y = fma3(y, r, 0.04166627239474941);
+    y = fma3(y, r, 0.16666665162903352);
+    y = fma3(y, r, 0.5000000077192173);
+    y = fma3(y, r, 1.0000000002087612);
     y = fma(y, r, 1.0);
-    y = fma(y, r, 1.0);
-    return ldexp(y, (int)k);
+    return __hiloint2double(__double2hiint(y) + (__double2loint(t) << 20), __double2loint(y));
+}
+
+/* x where bit c of `bits` is set, else -inf (a bit field's sign, a bitwise choice). */
+DLK_DEV float allowed_or_ninf(float x, uint32_t bits, int c) {
+    const uint32_t m = (uint32_t)((int)(bits << (31 - c)) >> 31);
+    return u2f((f2u(x) & m) | (0xff800000u & ~m));
+}
+
+/* The larger of three (NaN: of the others): one instruction, where fmaxf makes one for each
+ * value to quiet it. */
+DLK_DEV float max3(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
 }
 
 /* An entry of a list: larger is better (the logit's ascending key, then the lower id). */
@@ -73,31 +96,19 @@ DLK_DEV float beam_penalised(const BeamParams &p, float x, int cnt) {
     return x;
 }
 
-/* The largest key of 20 leading bits that at least r of the lanes' keys reach (0: fewer
- * than r lanes have one). */
+/* A key that at least r of the lanes' keys reach (0: fewer than r lanes have one): the largest
+ * for r = 1, else the largest of 20 leading bits (0.5 us where few waves run). */
 DLK_DEV uint32_t wave_rth(uint32_t a, int r) {
     uint32_t K = 0;
+    if (r == 1) return wave_minmax_u32<false>(a);
 #pragma unroll 1
     for (uint32_t bit = 0x80000000u; bit >= 0x1000u; bit >>= 1)
         if ((int)__popcll(ballot(a >= (K | bit))) >= r) K |= bit;
     return K;
 }
 
-template <class T>
-DLK_DEV T block_sum(T v, T *part) {
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) v += shfl_xor(v, m);
-    if (lane_id() == 0) part[wave_id()] = v;
-    __syncthreads();
-    T s = part[0];
-#pragma unroll
-    for (int w = 1; w < kBeamThreads / 64; w++) s += part[w];
-    __syncthreads();
-    return s;
-}
-
 struct BeamShared {
-    uint64_t key[kBeamList];            /* merge: keys; slice: entries */
+    __align__(16) uint64_t key[kBeamList];      /* merge: keys; slice: entries */
     uint64_t ent[kBeamList];
     double base[DLK_MAX_BEAMS];         /* per row of the group: log-sum, norm, score, maximum */
     double norm[DLK_MAX_BEAMS];
@@ -106,11 +117,11 @@ struct BeamShared {
     float top[DLK_MAX_BEAMS];
     uint32_t wave_key[kBeamThreads / 64];
     int wave_n[kBeamThreads / 64];
-    int place[kBeamList];               /* list of each entry */
+    int place[kBeamList];               /* row of each entry */
     int kind[DLK_MAX_BEAMS];            /* 0: none, 1: by its lists, 2: finished */
     int count, last;
     uint64_t best_key[kBeamThreads / 64], best_ent[kBeamThreads / 64];
-    int best_list[kBeamThreads / 64];
+    int best_row[kBeamThreads / 64];
 };
 
 /* a before b: larger key, lower row, larger entry. */
@@ -118,6 +129,24 @@ DLK_DEV bool before(uint64_t ka, int ra, uint64_t ea, uint64_t kb, int rb, uint6
     if (ka != kb) return ka > kb;
     if (ra != rb) return ra < rb;
     return ea > eb;
+}
+
+/* How many of list[0 .. n) are above v, and how many equal to it. */
+DLK_DEV int rank_in(const uint64_t *list, int n, uint64_t v, int &equal) {
+    int above = 0;
+    equal = 0;
+    int c = 0;
+    for (; c + 4 <= n; c += 4) {
+        const ulonglong2 a = *(const ulonglong2 *)&list[c], b = *(const ulonglong2 *)&list[c + 2];
+        above += (a.x > v ? 1 : 0) + (a.y > v ? 1 : 0) + (b.x > v ? 1 : 0) + (b.y > v ? 1 : 0);
+        equal += (a.x == v ? 1 : 0) + (a.y == v ? 1 : 0) + (b.x == v ? 1 : 0) + (b.y == v ? 1 : 0);
+    }
+    for (; c < n; c++) {
+        const uint64_t a = list[c];
+        above += a > v ? 1 : 0;
+        equal += a == v ? 1 : 0;
+    }
+    return above;
 }
 
 /* The continuation (row b, entry e) in 64 bits. */
@@ -147,98 +176,134 @@ DLK_DEV void write_none(const BeamParams &p, int g, int j) {
     if (p.out_finished) p.out_finished[o] = 0;
 }
 
-/* The group's lists merged, by its last workgroup. */
+/* The group's lists merged, by its last workgroup.  Up to one list per thread (256) the
+ * slots and each list's first entries are asked for at once: a round trip to the other
+ * workgroups' words is most of what a merge takes. */
 DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
+    constexpr int T = kBeamThreads, PRE = 4;
     const int t = threadIdx.x, lane = lane_id(), wave = wave_id(), g = p.g0 + gl;
     const int L = p.beams * p.slices;
     const BeamSlot *slots = p.slots + (int64_t)gl * L;
     const uint64_t *cands = p.cands + (int64_t)gl * L * p.n;
+    /* list i, that of (row i / slices, slice i % slices), goes to thread (i % 4) * 64 + i / 4 % 64, so
+     * that the waves share few lists evenly */
+    const int mine = (t & 63) * 4 + (t >> 6);
+    const bool once = L <= T;
+    uint64_t pre[PRE] = {0, 0, 0, 0}, sum0 = 0, mk0 = 0;
+    if (once && mine < L) {
+        sum0 = bget64(&slots[mine].sum);
+        mk0 = bget64(&slots[mine].max_kept);
+#pragma unroll
+        for (int j = 0; j < PRE; j++)
+            if (j < p.n) pre[j] = bget64(&cands[(int64_t)mine * p.n + j]);
+        sh.key[mine] = sum0;
+        sh.ent[mine] = mk0;
+    }
+    if (t == 0) sh.count = 0;
+    __syncthreads();
     /* the rows' sums, a wave each */
-    for (int b = wave; b < p.beams; b += kBeamThreads / 64) {
-        const int64_t row = (int64_t)g * p.beams + b;
-        const float cum = p.scores ? p.scores[row] : 0.0f;
-        const bool over = p.finished && p.finished[row];
+    for (int b = wave; b < p.beams; b += T / 64) {
         float top = -INFINITY;
         double sum = 0.0;
         bool bad = false;
         for (int s = lane; s < p.slices; s += 64) {
-            const uint64_t sm = bget64(&slots[b * p.slices + s].sum), mk = bget64(&slots[b * p.slices + s].max_kept);
+            const int i = b * p.slices + s;
+            const uint64_t sm = once ? sh.key[i] : bget64(&slots[i].sum), mk = once ? sh.ent[i] : bget64(&slots[i].max_kept);
             const float m = u2f((uint32_t)(mk >> 32));
             bad |= (uint32_t)mk == 0xffffffffu;
             if (m > -INFINITY) {
                 const float to = fmaxf(top, m);
-                sum = sum * (top > -INFINITY ? exp_neg((double)top - (double)to) : 0.0) +
+                sum = (top > -INFINITY ? sum * exp_neg((double)top - (double)to) : 0.0) +
                       u2d(sm) * exp_neg((double)m - (double)to);
                 top = to;
             }
         }
         const float all = wave_max_dpp(top);
-        sum = all > -INFINITY && top > -INFINITY ? sum * exp_neg((double)top - (double)all) : 0.0;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) sum += shfl_xor(sum, m);
+        sum = top > -INFINITY ? sum * exp_neg((double)top - (double)all) : 0.0;
+        sum = wave_incl_scan_d(sum);
         bad = ballot(bad) != 0;
-        if (lane == 0) {
-            const int len = p.lengths ? p.lengths[row] : 0;
-            const double length = fmax((double)len + (over ? 0.0 : 1.0), 1.0);
-            const bool alive = cum > -INFINITY && cum < INFINITY;
-            sh.cum[b] = cum;
+        if (lane == 63) {
             sh.top[b] = all;
-            sh.base[b] = all > -INFINITY ? log(sum) : 0.0;
-            sh.norm[b] = p.alpha == 0.0f ? 1.0 : pow(length, (double)p.alpha);
-            sh.kind[b] = !alive ? 0 : over ? 2 : bad || !(all > -INFINITY) ? 0 : 1;
-            if (p.status && (!(cum < INFINITY) || (alive && !over && bad))) atomicOr(p.status, DLK_STATUS_NOT_FINITE);
+            sh.base[b] = sum;
+            sh.kind[b] = bad ? -1 : all > -INFINITY ? 1 : 0;
         }
     }
-    if (t == 0) sh.count = 0;
     __syncthreads();
-    /* a list per (row, slice); a finished row's first list holds its one continuation.  List i
-     * goes to thread (i % 4) * 64 + i / 4 % 64, so that the waves share few lists evenly */
-    const int mine = (t & 63) * 4 + (t >> 6);
-    auto listed = [&](int i) {
-        const int b = i / p.slices;
-        if (sh.kind[b] == 0) return 0;
-        if (sh.kind[b] == 2) return i % p.slices == 0 ? 1 : 0;
-        return (int)(uint32_t)bget64(&slots[i].max_kept);
+    /* what each row adds to its continuations, a lane each */
+    if (t < p.beams) {
+        const int64_t row = (int64_t)g * p.beams + t;
+        const float cum = p.scores ? p.scores[row] : 0.0f;
+        const bool over = p.finished && p.finished[row];
+        const int kind = sh.kind[t];
+        const bool alive = cum > -INFINITY && cum < INFINITY;
+        const double length = fmax((double)(p.lengths ? p.lengths[row] : 0) + (over ? 0.0 : 1.0), 1.0);
+        sh.cum[t] = cum;
+        sh.base[t] = kind == 1 ? log(sh.base[t]) : 0.0;
+        sh.norm[t] = p.alpha == 0.0f ? 1.0 : 1.0 / pow(length, (double)p.alpha);
+        sh.kind[t] = !alive ? 0 : over ? 2 : kind == 1 ? 1 : 0;
+        if (p.status && (!(cum < INFINITY) || (alive && !over && kind < 0))) atomicOr(p.status, DLK_STATUS_NOT_FINITE);
+    }
+    __syncthreads();
+    /* list i of row b: its entries (a finished row's first list holds its one continuation), and
+     * their keys */
+    auto listed = [&](int i, int b) {
+        const int kind = sh.kind[b];
+        if (kind != 1) return kind == 2 && i == b * p.slices ? 1 : 0;
+        return (int)(uint32_t)(once ? mk0 : bget64(&slots[i].max_kept));
     };
-    auto entry = [&](int i, int j) { return sh.kind[i / p.slices] == 2 ? ~0ull : bget64(&cands[(int64_t)i * p.n + j]); };
-    auto key = [&](int i, uint64_t e) {
-        const int b = i / p.slices;
-        return double_key(beam_score(sh, b, e) / sh.norm[b]);
+    auto entry = [&](int i, int b, int j) -> uint64_t {
+        return sh.kind[b] == 2 ? ~(uint64_t)0 : bget64(&cands[(int64_t)i * p.n + j]);
     };
+    auto key = [&](int b, uint64_t e) { return double_key(beam_score(sh, b, e) * sh.norm[b]); };
     uint64_t head = 0;
-    for (int i = mine; i < L; i += kBeamThreads)
-        if (listed(i) > 0) head = max(head, key(i, entry(i, 0)));
+    for (int i = mine; i < L; i += T) {
+        const int b = i / p.slices;
+        if (listed(i, b) > 0) head = max(head, key(b, once ? pre[0] : entry(i, b, 0)));
+    }
     /* a bound that n heads, thus n continuations, reach */
     const uint32_t kw = wave_rth((uint32_t)(head >> 32), (p.n + 3) / 4);
     if (lane == 0) sh.wave_key[wave] = kw;
     __syncthreads();
     uint32_t bound = sh.wave_key[0];
 #pragma unroll
-    for (int w = 1; w < kBeamThreads / 64; w++) bound = min(bound, sh.wave_key[w]);
-    for (int i = mine; i < L; i += kBeamThreads) {
-        const int n = listed(i);
-        for (int j = 0; j < n; j++) {
-            const uint64_t e = entry(i, j), k = key(i, e);
-            if ((uint32_t)(k >> 32) < bound) break;
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kBeamList) {
-                sh.key[at] = k;
-                sh.ent[at] = e;
-                sh.place[at] = i;
+    for (int w = 1; w < T / 64; w++) bound = min(bound, sh.wave_key[w]);
+    for (int i = mine; i < L; i += T) {
+        const int b = i / p.slices, n = listed(i, b);
+        bool more = n > 0;
+        for (int j = 0; more && j < n; j += PRE) {
+            if (!once || j > 0) {                         /* the next few entries, in one round trip */
+#pragma unroll
+                for (int q = 0; q < PRE; q++) pre[q] = j + q < n ? entry(i, b, j + q) : 0;
+            }
+#pragma unroll
+            for (int q = 0; q < PRE; q++) {
+                if (!more || j + q >= n) break;
+                const uint64_t k = key(b, pre[q]);
+                more = (uint32_t)(k >> 32) >= bound;      /* (the list is in order) */
+                if (more) {
+                    const int at = atomicAdd(&sh.count, 1);
+                    if (at < kBeamList) {
+                        sh.key[at] = k;
+                        sh.ent[at] = pre[q];
+                        sh.place[at] = b;
+                    }
+                }
             }
         }
     }
     __syncthreads();
     const int C = sh.count;
     if (DLK_HOT(C <= kBeamList)) {
-        for (int a = t; a < C; a += kBeamThreads) {
+        for (int a = t; a < C; a += T) {
             const uint64_t k = sh.key[a], e = sh.ent[a];
-            const int i = sh.place[a], b = i / p.slices;
-            int rank = 0;
-            for (int c = 0; c < C; c++) rank += before(sh.key[c], sh.place[c] / p.slices, sh.ent[c], k, b, e) ? 1 : 0;
+            const int b = sh.place[a];
+            int equal, rank = rank_in(sh.key, C, k, equal);
+            if (equal > 1)
+                for (int c = 0; c < C; c++)
+                    rank += sh.key[c] == k && before(k, sh.place[c], sh.ent[c], k, b, e) ? 1 : 0;
             if (rank < p.n) write_continuation(p, sh, g, rank, b, e);
         }
-        for (int j = C + t; j < p.n; j += kBeamThreads) write_none(p, g, j);
+        for (int j = C + t; j < p.n; j += T) write_none(p, g, j);
     } else {
         /* too many at or above the bound (few lists for n, or runs of equal keys): the best one
          * still left, n times, the written ones known by the last one's place in the order */
@@ -247,47 +312,73 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
         for (int j = 0; j < p.n; j++) {
             uint64_t bk = 0, be = 0;
             int bi = -1;
-            for (int i = mine; i < L; i += kBeamThreads) {
-                const int n = listed(i), b = i / p.slices;
+            for (int i = mine; i < L; i += T) {
+                const int b = i / p.slices, n = listed(i, b);
                 for (int q = 0; q < n; q++) {
-                    const uint64_t e = entry(i, q), k = key(i, e);
+                    const uint64_t e = entry(i, b, q), k = key(b, e);
                     if (!before(lk, lb, le, k, b, e)) continue;               /* written */
-                    if (bi < 0 || before(k, b, e, bk, bi / p.slices, be)) { bk = k; be = e; bi = i; }
+                    if (bi < 0 || before(k, b, e, bk, bi, be)) { bk = k; be = e; bi = b; }
                     break;                                                    /* (the list is in order) */
                 }
             }
             for (int m = 1; m < 64; m <<= 1) {
                 const uint64_t ok = shfl_xor(bk, m), oe = shfl_xor(be, m);
                 const int oi = shfl_xor(bi, m);
-                if (oi >= 0 && (bi < 0 || before(ok, oi / p.slices, oe, bk, bi / p.slices, be))) { bk = ok; be = oe; bi = oi; }
+                if (oi >= 0 && (bi < 0 || before(ok, oi, oe, bk, bi, be))) { bk = ok; be = oe; bi = oi; }
             }
-            if (lane == 0) { sh.best_key[wave] = bk; sh.best_ent[wave] = be; sh.best_list[wave] = bi; }
+            if (lane == 0) { sh.best_key[wave] = bk; sh.best_ent[wave] = be; sh.best_row[wave] = bi; }
             __syncthreads();
             bi = -1;
-            for (int w = 0; w < kBeamThreads / 64; w++) {
-                const int oi = sh.best_list[w];
-                if (oi >= 0 && (bi < 0 || before(sh.best_key[w], oi / p.slices, sh.best_ent[w], bk, bi / p.slices, be))) {
+            for (int w = 0; w < T / 64; w++) {
+                const int oi = sh.best_row[w];
+                if (oi >= 0 && (bi < 0 || before(sh.best_key[w], oi, sh.best_ent[w], bk, bi, be))) {
                     bk = sh.best_key[w]; be = sh.best_ent[w]; bi = oi;
                 }
             }
             __syncthreads();
             if (t == 0) {
-                if (bi >= 0) write_continuation(p, sh, g, j, bi / p.slices, be);
+                if (bi >= 0) write_continuation(p, sh, g, j, bi, be);
                 else write_none(p, g, j);
             }
-            if (bi >= 0) { lk = bk; le = be; lb = bi / p.slices; }
+            if (bi >= 0) { lk = bk; le = be; lb = bi; }
         }
     }
 }
 
+/* A slice in p.batches batches of four groups of four logits per thread. */
 template <bool HIST>
-__global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamParams p) {
+__global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams p) {
+    constexpr int T = kBeamThreads, GR = 4, B = kBeamBatch;
     __shared__ BeamShared sh;
-    __shared__ __align__(16) uint32_t times[HIST ? kBeamSlice / 2 : 4];      /* occurrences, 16 bits an id */
+    __shared__ __align__(16) uint32_t times[HIST ? B / 2 : 4];               /* occurrences, 16 bits an id */
     const int t = threadIdx.x, lane = lane_id(), wave = wave_id();
     const int slice = blockIdx.x % p.slices, rl = blockIdx.x / p.slices;      /* rl: row of the launch */
     const int64_t row = (int64_t)p.g0 * p.beams + rl;
-    const int s0 = slice * kBeamSlice;
+    const float *lg = p.logits + row * p.ld;
+    const uint32_t *mw = p.mask ? p.mask + (int64_t)(p.mask_row ? p.mask_row[row] : row) * p.mask_ld : nullptr;
+    const int s0 = slice * p.batches * B, s1 = (int)min((int64_t)p.V, (int64_t)s0 + (int64_t)p.batches * B);
+    float x[GR][4];
+    auto load = [&](int b0) {
+        int t4 = t * 4;
+        asm volatile("" : "+v"(t4));                         /* (places kept from batch to batch are 50 registers) */
+        if (b0 + B <= s1) {
+#pragma unroll
+            for (int j = 0; j < GR; j++) {
+                const float4 v = load4(lg + b0 + j * T * 4 + t4);
+                x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < GR; j++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const int i = b0 + j * T * 4 + t4 + c;
+                    const float v = lg[min(i, s1 - 1)];
+                    x[j][c] = i < s1 ? v : -INFINITY;
+                }
+        }
+    };
+    load(s0);                                                /* (asked for before it is known whether the row is used) */
     const float cum = p.scores ? p.scores[row] : 0.0f;
     int hn = 0;
     const int32_t *hist = nullptr;
@@ -296,7 +387,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamParams p)
         hn = p.hist_off[row + 1] - h0;
         hist = p.hist_ids + h0;
     }
-    /* a row without continuations, or a finished one: its logits are not read */
+    /* a row without continuations, or a finished one: what its logits hold does not matter */
     bool idle = !(cum > -INFINITY && cum < INFINITY) || (p.finished && p.finished[row]);
     const bool too_long = HIST && !idle && hn > p.max_hist;
     idle |= too_long;
@@ -305,146 +396,197 @@ __global__ __launch_bounds__(kBeamThreads) void beam_select_kernel(BeamParams p)
     double sum = 0.0;
     uint32_t kept = 0;
     if (!idle) {
-        const float *lg = p.logits + row * p.ld;
-        float x[kBeamGroups][4];
+        if (t == 0) sh.count = 0;
+        float most = -INFINITY;                    /* this thread's maximum, and its sum of exp(l - that) */
+        double part = 0.0;
+        bool bad = false;
+        float least = -INFINITY;                   /* bound: n entries of the slice reach it (as a logit, and exactly) */
+        uint64_t bound = 0;
+        for (int b0 = s0; b0 < s1; b0 += B) {
+            int t4 = t * 4;
+            asm volatile("" : "+v"(t4));
+            if (b0 != s0) load(b0);
+            if (mw) {
+                uint32_t bits[GR];
 #pragma unroll
-        for (int j = 0; j < kBeamGroups; j++) {
-            const int i = s0 + (j * kBeamThreads + t) * 4;
-            if (i + 3 < p.V) {
-                const float4 v = load4(lg + i);
-                x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
-            } else {
+                for (int j = 0; j < GR; j++) bits[j] = mw[min(b0 + j * T * 4 + t4, s1 - 1) >> 5];
 #pragma unroll
-                for (int c = 0; c < 4; c++) x[j][c] = i + c < p.V ? lg[i + c] : -INFINITY;
+                for (int j = 0; j < GR; j++) {
+                    bits[j] >>= (b0 + j * T * 4 + t4) & 31;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) x[j][c] = allowed_or_ninf(x[j][c], bits[j], c);
+                }
             }
-        }
-        if (p.mask) {
-            const uint32_t *mw = p.mask + (int64_t)(p.mask_row ? p.mask_row[row] : row) * p.mask_ld;
+            if (HIST && hn > 0) {
+                for (int i = t; i < B / 8; i += T) ((uint4 *)times)[i] = make_uint4(0, 0, 0, 0);
+                __syncthreads();
+                for (int i = t; i < hn; i += T) {
+                    const int32_t id = hist[i];
+                    if (id >= b0 && id < s1 && id - b0 < B) atomicAdd(&times[(id - b0) >> 1], 1u << (16 * (id & 1)));
+                }
+                __syncthreads();
 #pragma unroll
-            for (int j = 0; j < kBeamGroups; j++) {
-                const int i = s0 + (j * kBeamThreads + t) * 4;
-                const uint32_t bits = i < p.V ? mw[i >> 5] >> (i & 31) : 0u;
-#pragma unroll
-                for (int c = 0; c < 4; c++) x[j][c] = (bits >> c) & 1u ? x[j][c] : -INFINITY;
-            }
-        }
-        if (HIST && hn > 0) {
-            for (int i = t; i < kBeamSlice / 8; i += kBeamThreads) ((uint4 *)times)[i] = make_uint4(0, 0, 0, 0);
-            __syncthreads();
-            for (int i = t; i < hn; i += kBeamThreads) {
-                const int32_t id = hist[i];
-                if (id >= 0 && id < p.V && id >= s0 && id - s0 < kBeamSlice)
-                    atomicAdd(&times[(id - s0) >> 1], 1u << (16 * (id & 1)));
-            }
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < kBeamGroups; j++) {
-                const uint2 w = ((const uint2 *)times)[j * kBeamThreads + t];
-                if ((w.x | w.y) != 0) {
-                    const int n[4] = {(int)(w.x & 0xffff), (int)(w.x >> 16), (int)(w.y & 0xffff), (int)(w.y >> 16)};
+                for (int j = 0; j < GR; j++) {
+                    const uint2 w = ((const uint2 *)times)[j * T + t];
+                    if ((w.x | w.y) != 0) {
 #pragma unroll 1
-                    for (int c = 0; c < 4; c++) {
-                        const int nc = c == 0 ? n[0] : c == 1 ? n[1] : c == 2 ? n[2] : n[3];
-                        const float v = c == 0 ? x[j][0] : c == 1 ? x[j][1] : c == 2 ? x[j][2] : x[j][3];
-                        if (nc == 0 || v == -INFINITY) continue;
-                        const float y = beam_penalised(p, v, nc);
-                        x[j][0] = c == 0 ? y : x[j][0];
-                        x[j][1] = c == 1 ? y : x[j][1];
-                        x[j][2] = c == 2 ? y : x[j][2];
-                        x[j][3] = c == 3 ? y : x[j][3];
+                        for (int c = 0; c < 4; c++) {
+                            const int nc = (int)(((c < 2 ? w.x : w.y) >> (16 * (c & 1))) & 0xffff);
+                            const float v = c == 0 ? x[j][0] : c == 1 ? x[j][1] : c == 2 ? x[j][2] : x[j][3];
+                            if (nc == 0 || v == -INFINITY) continue;
+                            const float y = beam_penalised(p, v, nc);
+                            x[j][0] = c == 0 ? y : x[j][0];
+                            x[j][1] = c == 1 ? y : x[j][1];
+                            x[j][2] = c == 2 ? y : x[j][2];
+                            x[j][3] = c == 3 ? y : x[j][3];
+                        }
                     }
                 }
             }
-        }
-        float mine = -INFINITY;
-        bool bad = false;
+            float best = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < kBeamGroups; j++)
+            for (int j = 0; j < GR; j++) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                bad |= !(x[j][c] < INFINITY);
-                mine = fmaxf(mine, x[j][c]);
+                for (int c = 0; c < 4; c++) bad |= !(x[j][c] < INFINITY);
+                best = max3(max3(best, x[j][0], x[j][1]), x[j][2], x[j][3]);
             }
-        const float wtop = wave_max_dpp(mine);
-        const uint32_t akey = mine > -INFINITY ? ~desc_key(mine) : 0u;
-        const uint32_t kw = wave_rth(akey, (p.n + 3) / 4);
-        bad = ballot(bad) != 0;
-        if (lane == 0) {
-            sh.part[wave] = (double)wtop;
-            sh.wave_key[wave] = kw;
-            sh.wave_n[wave] = bad;
-        }
-        if (t == 0) sh.count = 0;
-        __syncthreads();
-        uint32_t bound = sh.wave_key[0];
-        top = (float)sh.part[0];
-        bad = sh.wave_n[0] != 0;
+            if (b0 == s0) {
+                /* the bound: in each wave n / 4 lanes have an entry that reaches it */
+                const uint32_t kw = wave_rth(best > -INFINITY ? ~desc_key(best) : 0u, (p.n + 3) / 4);
+                if (lane == 0) sh.wave_key[wave] = kw;
+                __syncthreads();
+                uint32_t k = sh.wave_key[0];
 #pragma unroll
-        for (int w = 1; w < kBeamThreads / 64; w++) {
-            bound = min(bound, sh.wave_key[w]);
-            top = fmaxf(top, (float)sh.part[w]);
-            bad |= sh.wave_n[w] != 0;
-        }
-        __syncthreads();
-        if (bad) {
-            top = -INFINITY;
-            kept = 0xffffffffu;
-        } else if (top > -INFINITY) {
+                for (int w = 1; w < T / 64; w++) k = min(k, sh.wave_key[w]);
+                if (k != 0) least = key_value(~k);           /* (0: every continuation is an entry) */
+                bound = (uint64_t)k << 32;
+            }
+            const int had = sh.count;
+            if (b0 != s0) __syncthreads();                   /* (everyone has read it) */
+            if (best >= least) {
+                uint32_t at_least = 0;                       /* bit 4 j + c */
+#pragma unroll
+                for (int j = 0; j < GR; j++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) at_least |= x[j][c] >= least && x[j][c] > -INFINITY ? 1u << (4 * j + c) : 0u;
+                for (; at_least; at_least &= at_least - 1) {
+                    const int k = __builtin_ctz(at_least);
+                    float v = x[0][0];
+#pragma unroll
+                    for (int q = 1; q < 4 * GR; q++) v = k == q ? x[q >> 2][q & 3] : v;
+                    const uint64_t e = entry_of(v, b0 + (k >> 2) * T * 4 + t4 + (k & 3));
+                    if (e >= bound) {
+                        const int at = atomicAdd(&sh.count, 1);
+                        if (at < kBeamList) sh.key[at] = e;
+                    }
+                }
+            }
+            /* (-inf counts as exp(-700) of the maximum: nothing) */
+            const float to = fmaxf(fmaxf(most, best), -3.40282347e38f);
             double s = 0.0;
 #pragma unroll
-            for (int j = 0; j < kBeamGroups; j++)
+            for (int j = 0; j < GR; j++) {
 #pragma unroll
-                for (int c = 0; c < 4; c++)
-                    if (x[j][c] > -INFINITY) s += exp_neg((double)x[j][c] - (double)top);
-            sum = block_sum(s, sh.part);
-            /* the entries at or above the bound */
-            auto collect = [&](uint64_t least) {
-                if (mine > -INFINITY && entry_of(mine, 0) >= least) {
-#pragma unroll
-                    for (int j = 0; j < kBeamGroups; j++)
-#pragma unroll
-                        for (int c = 0; c < 4; c++) {
-                            const uint64_t e = entry_of(x[j][c], s0 + (j * kBeamThreads + t) * 4 + c);
-                            if (x[j][c] > -INFINITY && e >= least) {
-                                const int at = atomicAdd(&sh.count, 1);
-                                if (at < kBeamList) sh.key[at] = e;
-                            }
-                        }
-                }
-                __syncthreads();
-                return sh.count;
-            };
-            int C = collect((uint64_t)bound << 32);
+                for (int c = 0; c < 4; c++) s += exp_neg((double)x[j][c] - (double)to);
+                asm volatile("" : "+v"(s));                  /* (here and in order, not past the barrier below) */
+            }
+            part = part * exp_neg((double)most - (double)to) + s;
+            most = fmaxf(most, best);
+            __syncthreads();
+            const int C = sh.count;
             if (DLK_COLD(C > kBeamList)) {
-                /* too many: the n-th largest entry exactly, bit by bit (entries are all unlike) */
-                uint64_t least = 0;
-                for (uint64_t bit = 1ull << 63; bit; bit >>= 1) {
+                /* more than the list takes: of this batch only its n largest (there is room for them,
+                 * below), found bit by bit: the n-th largest value, then the last place of that value */
+                auto count = [&](auto holds) {
                     int c = 0;
 #pragma unroll
-                    for (int j = 0; j < kBeamGroups; j++)
+                    for (int j = 0; j < GR; j++)
 #pragma unroll
-                        for (int q = 0; q < 4; q++)
-                            c += x[j][q] > -INFINITY &&
-                                 entry_of(x[j][q], s0 + (j * kBeamThreads + t) * 4 + q) >= (least | bit) ? 1 : 0;
+                        for (int q = 0; q < 4; q++) {
+                            float v = x[j][q];
+                            asm volatile("" : "+v"(v));      /* (made anew each time: kept, the keys are registers) */
+                            c += v > -INFINITY && holds(~desc_key(v), j * T * 4 + t4 + q) ? 1 : 0;
+                        }
                     c = wave_sum_i32(c);
+                    __syncthreads();
                     if (lane == 0) sh.wave_n[wave] = c;
                     __syncthreads();
                     c = sh.wave_n[0];
 #pragma unroll
-                    for (int w = 1; w < kBeamThreads / 64; w++) c += sh.wave_n[w];
-                    __syncthreads();
-                    if (c >= p.n) least |= bit;
-                }
-                if (t == 0) sh.count = 0;
+                    for (int w = 1; w < T / 64; w++) c += sh.wave_n[w];
+                    return c;
+                };
+                uint32_t value = 0;
+#pragma unroll 1
+                for (uint32_t bit = 1u << 31; bit; bit >>= 1)
+                    if (count([&](uint32_t k, int) { return k >= (value | bit); }) >= p.n) value |= bit;
+                const int need = p.n - count([&](uint32_t k, int) { return k > value; });
+                int place = 0;                               /* the places below it hold fewer than `need` of that value */
+#pragma unroll 1
+                for (int bit = B >> 1; bit; bit >>= 1)
+                    if (count([&](uint32_t k, int i) { return k == value && i < place + bit; }) < need) place += bit;
+                uint64_t nth = (uint64_t)value << 32 | (uint32_t)~(b0 + place);
+                nth = max(nth, bound);
+                if (t == 0) sh.count = had;
                 __syncthreads();
-                C = collect(least);
+#pragma unroll
+                for (int j = 0; j < GR; j++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const uint64_t e = entry_of(x[j][c], b0 + j * T * 4 + t4 + c);
+                        if (x[j][c] > -INFINITY && e >= nth) sh.key[atomicAdd(&sh.count, 1)] = e;      /* at most n */
+                    }
+                __syncthreads();
             }
+            if (DLK_COLD(sh.count > kBeamList - DLK_MAX_BEAMS) && b0 + B < s1) {
+                /* the list's n largest, in order, and the last of them as the bound from here on */
+                const int c0 = sh.count;
+#pragma unroll 1
+                for (int i = t; i < c0; i += T) {
+                    const uint64_t e = sh.key[i];
+                    int equal;
+                    const int rank = rank_in(sh.key, c0, e, equal);
+                    if (rank < p.n) sh.ent[rank] = e;
+                }
+                __syncthreads();
+                for (int i = t; i < p.n; i += T) sh.key[i] = sh.ent[i];
+                if (t == 0) sh.count = p.n;
+                __syncthreads();
+                bound = sh.key[p.n - 1];
+                least = entry_logit(bound);
+            }
+        }
+        const float wtop = wave_max_dpp(most);
+        bad = ballot(bad) != 0;
+        if (lane == 0) {
+            sh.top[wave] = wtop;
+            sh.wave_n[wave] = bad;
+        }
+        __syncthreads();
+        top = sh.top[0];
+        bad = sh.wave_n[0] != 0;
+#pragma unroll
+        for (int w = 1; w < T / 64; w++) {
+            top = fmaxf(top, sh.top[w]);
+            bad |= sh.wave_n[w] != 0;
+        }
+        if (bad) {
+            top = -INFINITY;
+            kept = 0xffffffffu;
+        } else if (top > -INFINITY) {
+            const double s = wave_incl_scan_d(part * exp_neg((double)fmaxf(most, -3.40282347e38f) - (double)top));
+            if (lane == 63) sh.part[wave] = s;
+            __syncthreads();
+            sum = sh.part[0];
+#pragma unroll
+            for (int w = 1; w < T / 64; w++) sum += sh.part[w];
+            const int C = sh.count;
             kept = (uint32_t)min(C, p.n);
             uint64_t *out = p.cands + ((int64_t)rl * p.slices + slice) * p.n;
-            for (int a = t; a < C; a += kBeamThreads) {
+            for (int a = t; a < C; a += T) {
                 const uint64_t e = sh.key[a];
-                int rank = 0;
-                for (int c = 0; c < C; c++) rank += sh.key[c] > e ? 1 : 0;
+                int equal;
+                const int rank = rank_in(sh.key, C, e, equal);
                 if (rank < p.n) bpub64(&out[rank], e);
             }
         }

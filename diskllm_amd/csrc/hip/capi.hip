@@ -689,7 +689,7 @@ extern "C" int dlk_beam_select(const dlk_beam_batch *b, int groups, int vocab, c
     if (!(fabsf(prm->length_penalty) <= 16.0f)) return DLK_ERR_INVALID;
     if (((uintptr_t)b->logits & 3) != 0) return DLK_ERR_INVALID;
     if (prm->beams > DLK_MAX_BEAMS || prm->n_out > DLK_MAX_BEAMS) return DLK_ERR_UNSUPPORTED;
-    if (prm->max_history > 65535 || vocab > 0x7fffffff - kBeamSlice) return DLK_ERR_UNSUPPORTED;
+    if (prm->max_history > 65535 || vocab > 0x7fffffff - (1 << 20)) return DLK_ERR_UNSUPPORTED;
     if ((int64_t)groups * prm->beams > 0x7fffffff || (int64_t)groups * prm->n_out > 0x7fffffff) return DLK_ERR_UNSUPPORTED;
     if (groups == 0) return DLK_OK;
     BeamParams p;
@@ -706,7 +706,8 @@ extern "C" int dlk_beam_select(const dlk_beam_batch *b, int groups, int vocab, c
     p.alpha = prm->length_penalty;
     p.order = prm->penalty_order;
     p.rep = prm->repeat_penalty; p.freq = prm->frequency_penalty; p.pres = prm->presence_penalty;
-    p.slices = (vocab + kBeamSlice - 1) / kBeamSlice;
+    p.batches = beam_batches((int64_t)groups * p.beams, p.beams, vocab);
+    p.slices = (int)(((int64_t)vocab + (int64_t)kBeamBatch * p.batches - 1) / ((int64_t)kBeamBatch * p.batches));
     /* per group: its rows' slots, then their lists */
     const size_t lists = (size_t)p.beams * p.slices, per = lists * (sizeof(BeamSlot) + (size_t)p.n * 8);
     int64_t most = (int64_t)(kBeamWorkspace / per);

@@ -323,7 +323,7 @@ typedef struct {
  * dlk_sample does; its continuation by id v has
  *   score = scores[r] + (l_v - max l) - log(sum_u exp(l_u - max l)),  length = lengths[r] + 1,
  * computed in 64 bits and rounded once.  A finished row has one continuation: eos_id,
- * with its score and length as they are (its logits are not read).  Ids with logit
+ * with its score and length as they are (whatever its logits hold).  Ids with logit
  * -inf are no continuations, nor are those of rows with score -inf.
  * Of each group's continuations the n_out with the largest score / max(length,
  * 1)^length_penalty (before rounding) are written, largest first; of equal ones the
