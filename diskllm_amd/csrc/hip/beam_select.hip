@@ -107,6 +107,14 @@ DLK_DEV uint32_t wave_rth(uint32_t a, int r) {
     return K;
 }
 
+/* Maximum over each row of 16 lanes (every lane gets its row's). */
+DLK_DEV float row_max(float v) {
+    v = fmaxf(v, shfl_xor(v, 1));
+    v = fmaxf(v, shfl_xor(v, 2));
+    v = fmaxf(v, shfl_xor(v, 4));
+    return fmaxf(v, shfl_xor(v, 8));
+}
+
 struct BeamShared {
     __align__(16) uint64_t key[kBeamList];      /* merge: keys; slice: entries */
     uint64_t ent[kBeamList];
@@ -149,11 +157,16 @@ DLK_DEV int rank_in(const uint64_t *list, int n, uint64_t v, int &equal) {
     return above;
 }
 
-/* The continuation (row b, entry e) in 64 bits. */
-DLK_DEV double beam_score(const BeamShared &sh, int b, uint64_t e) {
-    if (sh.kind[b] == 2) return (double)sh.cum[b];
-    return (double)sh.cum[b] + (((double)entry_logit(e) - (double)sh.top[b]) - sh.base[b]);
-}
+/* What a row adds to its continuations, out of LDS once for many of them. */
+struct BeamRow {
+    double base, norm, top, cum;
+    bool over;
+    DLK_DEV BeamRow(const BeamShared &sh, int b)
+        : base(sh.base[b]), norm(sh.norm[b]), top((double)sh.top[b]), cum((double)sh.cum[b]), over(sh.kind[b] == 2) {}
+    /* the score of entry e in 64 bits, and its key */
+    DLK_DEV double score(uint64_t e) const { return over ? cum : cum + (((double)entry_logit(e) - top) - base); }
+    DLK_DEV uint64_t key(uint64_t e) const { return double_key(score(e) * norm); }
+};
 
 DLK_DEV void write_continuation(const BeamParams &p, const BeamShared &sh, int g, int j, int b, uint64_t e) {
     const int64_t o = (int64_t)g * p.n + j, row = (int64_t)g * p.beams + b;
@@ -162,7 +175,7 @@ DLK_DEV void write_continuation(const BeamParams &p, const BeamShared &sh, int g
     const int len = p.lengths ? p.lengths[row] : 0;
     p.out_tokens[o] = id;
     p.out_parents[o] = (int32_t)row;
-    p.out_scores[o] = (float)beam_score(sh, b, e);
+    p.out_scores[o] = (float)BeamRow(sh, b).score(e);
     if (p.out_lengths) p.out_lengths[o] = len + (over ? 0 : 1);
     if (p.out_finished) p.out_finished[o] = over || id == p.eos ? 1 : 0;
 }
@@ -180,7 +193,7 @@ DLK_DEV void write_none(const BeamParams &p, int g, int j) {
  * slots and each list's first entries are asked for at once: a round trip to the other
  * workgroups' words is most of what a merge takes. */
 DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
-    constexpr int T = kBeamThreads, PRE = 4;
+    constexpr int T = kBeamThreads, PRE = 8;
     const int t = threadIdx.x, lane = lane_id(), wave = wave_id(), g = p.g0 + gl;
     const int L = p.beams * p.slices;
     const BeamSlot *slots = p.slots + (int64_t)gl * L;
@@ -189,24 +202,25 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
      * that the waves share few lists evenly */
     const int mine = (t & 63) * 4 + (t >> 6);
     const bool once = L <= T;
-    uint64_t pre[PRE] = {0, 0, 0, 0}, sum0 = 0, mk0 = 0;
+    uint64_t pre[PRE], sum0 = 0, mk0 = 0;
     if (once && mine < L) {
         sum0 = bget64(&slots[mine].sum);
         mk0 = bget64(&slots[mine].max_kept);
 #pragma unroll
-        for (int j = 0; j < PRE; j++)
-            if (j < p.n) pre[j] = bget64(&cands[(int64_t)mine * p.n + j]);
+        for (int j = 0; j < PRE; j++) pre[j] = bget64(&cands[(int64_t)mine * p.n + min(j, p.n - 1)]);
         sh.key[mine] = sum0;
         sh.ent[mine] = mk0;
     }
     if (t == 0) sh.count = 0;
     __syncthreads();
-    /* the rows' sums, a wave each */
-    for (int b = wave; b < p.beams; b += T / 64) {
+    /* the rows' sums: 16 lanes each where they have 16 slices at most, else a wave each */
+    const int width = p.slices <= 16 ? 16 : 64, sub = t & (width - 1);
+    for (int b0 = 0; b0 < p.beams; b0 += T / width) {
+        const int b = b0 + t / width;
         float top = -INFINITY;
         double sum = 0.0;
         bool bad = false;
-        for (int s = lane; s < p.slices; s += 64) {
+        for (int s = sub; b < p.beams && s < p.slices; s += width) {
             const int i = b * p.slices + s;
             const uint64_t sm = once ? sh.key[i] : bget64(&slots[i].sum), mk = once ? sh.ent[i] : bget64(&slots[i].max_kept);
             const float m = u2f((uint32_t)(mk >> 32));
@@ -218,14 +232,15 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
                 top = to;
             }
         }
-        const float all = wave_max_dpp(top);
+        float all = row_max(top);
+        if (width == 64) all = wave_max_dpp(all);
         sum = top > -INFINITY ? sum * exp_neg((double)top - (double)all) : 0.0;
-        sum = wave_incl_scan_d(sum);
-        bad = ballot(bad) != 0;
-        if (lane == 63) {
+        sum = width == 64 ? wave_incl_scan_d(sum) : row_scan_d(sum);
+        const uint64_t bads = width == 64 ? ballot(bad) : ballot(bad) >> (lane & 48) & 0xffff;
+        if (sub == width - 1 && b < p.beams) {
             sh.top[b] = all;
             sh.base[b] = sum;
-            sh.kind[b] = bad ? -1 : all > -INFINITY ? 1 : 0;
+            sh.kind[b] = bads ? -1 : all > -INFINITY ? 1 : 0;
         }
     }
     __syncthreads();
@@ -244,8 +259,7 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
         if (p.status && (!(cum < INFINITY) || (alive && !over && kind < 0))) atomicOr(p.status, DLK_STATUS_NOT_FINITE);
     }
     __syncthreads();
-    /* list i of row b: its entries (a finished row's first list holds its one continuation), and
-     * their keys */
+    /* list i of row b: its entries (a finished row's first list holds its one continuation) */
     auto listed = [&](int i, int b) {
         const int kind = sh.kind[b];
         if (kind != 1) return kind == 2 && i == b * p.slices ? 1 : 0;
@@ -254,11 +268,10 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
     auto entry = [&](int i, int b, int j) -> uint64_t {
         return sh.kind[b] == 2 ? ~(uint64_t)0 : bget64(&cands[(int64_t)i * p.n + j]);
     };
-    auto key = [&](int b, uint64_t e) { return double_key(beam_score(sh, b, e) * sh.norm[b]); };
     uint64_t head = 0;
     for (int i = mine; i < L; i += T) {
         const int b = i / p.slices;
-        if (listed(i, b) > 0) head = max(head, key(b, once ? pre[0] : entry(i, b, 0)));
+        if (listed(i, b) > 0) head = max(head, BeamRow(sh, b).key(once ? pre[0] : entry(i, b, 0)));
     }
     /* a bound that n heads, thus n continuations, reach */
     const uint32_t kw = wave_rth((uint32_t)(head >> 32), (p.n + 3) / 4);
@@ -269,7 +282,9 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
     for (int w = 1; w < T / 64; w++) bound = min(bound, sh.wave_key[w]);
     for (int i = mine; i < L; i += T) {
         const int b = i / p.slices, n = listed(i, b);
-        bool more = n > 0;
+        if (n == 0) continue;
+        const BeamRow row(sh, b);
+        bool more = true;
         for (int j = 0; more && j < n; j += PRE) {
             if (!once || j > 0) {                         /* the next few entries, in one round trip */
 #pragma unroll
@@ -278,7 +293,7 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
 #pragma unroll
             for (int q = 0; q < PRE; q++) {
                 if (!more || j + q >= n) break;
-                const uint64_t k = key(b, pre[q]);
+                const uint64_t k = row.key(pre[q]);
                 more = (uint32_t)(k >> 32) >= bound;      /* (the list is in order) */
                 if (more) {
                     const int at = atomicAdd(&sh.count, 1);
@@ -315,7 +330,7 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
             for (int i = mine; i < L; i += T) {
                 const int b = i / p.slices, n = listed(i, b);
                 for (int q = 0; q < n; q++) {
-                    const uint64_t e = entry(i, b, q), k = key(b, e);
+                    const uint64_t e = entry(i, b, q), k = BeamRow(sh, b).key(e);
                     if (!before(lk, lb, le, k, b, e)) continue;               /* written */
                     if (bi < 0 || before(k, b, e, bk, bi, be)) { bk = k; be = e; bi = b; }
                     break;                                                    /* (the list is in order) */
