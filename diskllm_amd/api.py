@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from math import prod
 from typing import Optional
 
 import numpy as np
@@ -310,7 +311,8 @@ def beam_state(src: torch.Tensor, dst: Optional[torch.Tensor] = None, row_dim: i
     dimensions before the rows, those up to length_dim and those from it on have to be one stride each.  The
     caller keeps the tensors."""
     shape = list(src.shape)
-    nd, rows, dst_rows = len(shape), shape[row_dim] if row_dim < len(shape) else 0, 0
+    nd = len(shape)
+    rows = shape[row_dim] if row_dim < nd else 0
     cut = row_dim + 1 if length_dim is None else length_dim
     _want(0 <= row_dim < nd and (length_dim is None or row_dim < cut < nd), "length_dim: a dimension after the rows is wanted")
     if length_dim is not None and length is not None:
@@ -326,6 +328,14 @@ def beam_state(src: torch.Tensor, dst: Optional[torch.Tensor] = None, row_dim: i
             other[cut] = shape[cut]
         _want(other == shape, "dst: another shape than src's")
     item = src.element_size()
+    if dst is None and src.is_contiguous():
+        full = src.shape                           # (by the sizes: strides of single rows or heads may be anything)
+        at, row = src.data_ptr(), prod(full[row_dim + 1:]) * item
+        outer, inner = row * rows, prod(full[cut:]) * item
+        s = _lib.BeamState(at, at, prod(shape[cut:]) * item if 0 not in shape else 0, row, outer, inner, row, outer, inner,
+                           prod(shape[:row_dim]), prod(shape[row_dim + 1:cut]))
+        s.rows = (rows, rows, src.get_device(), src.get_device())
+        return s
 
     def layout(t):
         st = t.stride()

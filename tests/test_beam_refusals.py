@@ -158,3 +158,11 @@ def test_state_layouts():
     d = api.beam_state(torch.zeros((8, 3, 2, 16, 4)), length_dim=3, length=16)
     assert (d.bytes, d.n_outer, d.n_inner, d.src_inner) == (16 * 4 * 4, 1, 6, 16 * 4 * 4)
     assert api.beam_state(c, row_dim=1, length_dim=3, length=0).bytes == 0
+    # a single row or head whose stride says nothing
+    one = torch.zeros((3, 8, 2, 16, 4)).as_strided((3, 1, 1, 16, 4), (64, 7, 5, 4, 1))
+    assert one.is_contiguous()
+    u = api.beam_state(one, row_dim=1, length_dim=3, length=5)
+    assert (u.bytes, u.n_outer, u.n_inner, u.src_outer) == (5 * 4 * 4, 3, 1, 64 * 4)
+    # rows that lie apart
+    v = api.beam_state(torch.zeros((8, 3, 40))[:, 1])
+    assert (v.bytes, v.n_outer, v.n_inner, v.src_row) == (160, 1, 1, 480)
