@@ -476,7 +476,7 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
                 if (k != 0) least = key_value(~k);           /* (0: every continuation is an entry) */
                 bound = (uint64_t)k << 32;
             }
-            const int had = sh.count;
+            const int had = b0 == s0 ? 0 : sh.count;          /* (in the first batch others may be adding to it) */
             if (b0 != s0) __syncthreads();                   /* (everyone has read it) */
             if (best >= least) {
                 uint32_t at_least = 0;                       /* bit 4 j + c */

@@ -235,6 +235,17 @@ def test_select_equal_logits(cuda, V, n_out):
     check(torch, lg[:, ::-1].copy(), 4, n_out)
 
 
+def test_select_equal_logits_many_rows(cuda):
+    """Every row's first batch overflows its list: a row's entries are counted once each, whichever wave is first."""
+    import torch
+    from diskllm_amd import api
+    lg = torch.zeros((96, 50257), device="cuda")
+    for _ in range(20):
+        out = api.beam_select(lg, 3, 64)
+        assert (out["tokens"].view(32, 64).cpu() == torch.arange(64)).all()
+        assert (out["parents"].view(32, 64).cpu() == torch.arange(0, 96, 3)[:, None]).all()
+
+
 def test_select_all_finished(cuda):
     """A group whose beams have all ended keeps them, ordered by their normalised scores."""
     import torch
