@@ -177,6 +177,8 @@ def _rows2d(t: torch.Tensor, dev: int, dtype, what: str):
     if t.dim() != 2 or (dtype is not None and t.dtype is not dtype) or t.get_device() != dev:
         raise ValueError(f"{what}: [rows, n] of {dtype} on the call's device is wanted")
     rows, n = t.shape
+    if rows > 0x7fffffff or n > 0x7fffffff:
+        raise ValueError(f"{what}: more rows or entries than 32 bits count")
     ld, one = t.stride()
     if rows <= 1 and ld < n:
         ld = n

@@ -22,6 +22,7 @@ namespace dlk {
 
 constexpr int kMoveThreads = 256;
 constexpr int kMoveStates = 8;                   /* states of one launch */
+constexpr int64_t kMoveBlocks = 0xffffff;        /* workgroups of one launch: 2^32 threads and over are refused */
 
 typedef uint32_t u4_any __attribute__((ext_vector_type(4), aligned(1)));
 
@@ -161,6 +162,8 @@ bool apart(int64_t bytes, int64_t rows, int64_t row, int64_t no, int64_t outer, 
     return true;
 }
 
+int64_t tiles_of(int64_t bytes) { return (bytes + kMoveThreads * 16 - 1) / (kMoveThreads * 16); }
+
 }  // namespace dlk
 
 extern "C" int dlk_beam_reorder(const int32_t *parents, int groups, int beams, int n_out, const dlk_beam_state *states,
@@ -169,13 +172,14 @@ extern "C" int dlk_beam_reorder(const int32_t *parents, int groups, int beams, i
     if (!parents || groups < 0 || beams <= 0 || n_out <= 0 || n_states < 0 || (n_states && !states)) return DLK_ERR_INVALID;
     if (beams > DLK_MAX_BEAMS || n_out > DLK_MAX_BEAMS) return DLK_ERR_UNSUPPORTED;
     const int64_t rows = (int64_t)groups * n_out, rows_in = (int64_t)groups * beams;
-    if (rows > 0x3fffffff || rows_in > 0x3fffffff) return DLK_ERR_UNSUPPORTED;
+    if (rows > 0x3fffffff || rows_in > 0x3fffffff || (history && rows > kMoveBlocks)) return DLK_ERR_UNSUPPORTED;
     for (int i = 0; i < n_states; i++) {
         const dlk_beam_state &s = states[i];
-        if (!s.src || !s.dst || s.bytes < 0 || s.n_outer < 0 || s.n_inner < 0) return DLK_ERR_INVALID;
+        if (s.bytes < 0 || s.n_outer < 0 || s.n_inner < 0) return DLK_ERR_INVALID;
         if (s.src_row < 0 || s.src_outer < 0 || s.src_inner < 0 || s.dst_row < 0 || s.dst_outer < 0 || s.dst_inner < 0)
             return DLK_ERR_INVALID;
         if (s.bytes == 0 || s.n_outer == 0 || s.n_inner == 0 || groups == 0) continue;
+        if (!s.src || !s.dst) return DLK_ERR_INVALID;          /* (empty ones may be nowhere) */
         if (!apart(s.bytes, rows, s.dst_row, s.n_outer, s.dst_outer, s.n_inner, s.dst_inner)) return DLK_ERR_INVALID;
         const unsigned char *a = (const unsigned char *)s.src, *d = (const unsigned char *)s.dst;
         if (a == d) {
@@ -186,6 +190,13 @@ extern "C" int dlk_beam_reorder(const int32_t *parents, int groups, int beams, i
             const int64_t ed = (rows - 1) * s.dst_row + (s.n_outer - 1) * s.dst_outer + (s.n_inner - 1) * s.dst_inner + s.bytes;
             if (a < d + ed && d < a + ea) return DLK_ERR_INVALID;
         }
+        /* one buffer twice, or two that change places (what else overlaps is the caller's to know:
+         * the strides of two states may interleave) */
+        for (int j = 0; j < i; j++)
+            if (states[j].bytes > 0 && states[j].n_outer > 0 && states[j].n_inner > 0 &&
+                (d == states[j].dst || d == states[j].src || a == states[j].dst))
+                return DLK_ERR_INVALID;
+        if ((double)tiles_of(s.bytes) * s.n_outer * s.n_inner * groups > (double)kMoveBlocks) return DLK_ERR_UNSUPPORTED;
     }
     const dlk_beam_history *h = history;
     if (h) {
@@ -212,26 +223,24 @@ extern "C" int dlk_beam_reorder(const int32_t *parents, int groups, int beams, i
             m.dst_row = s.dst_row; m.dst_outer = s.dst_outer; m.dst_inner = s.dst_inner;
             m.n_outer = s.n_outer; m.n_inner = s.n_inner;
             m.in_place = s.src == s.dst;
-            const int64_t tiles = (s.bytes + kMoveThreads * 16 - 1) / (kMoveThreads * 16);
-            if (tiles > 0x7fffffff) return DLK_ERR_UNSUPPORTED;
-            m.tiles = (int)tiles;
+            m.tiles = (int)tiles_of(s.bytes);
             m.first = blocks;
-            const double all = (double)tiles * s.n_outer * s.n_inner * groups;
-            if (all > 0x3fffffff) return DLK_ERR_UNSUPPORTED;
-            if (blocks + (int64_t)all > 0x3fffffff) break;
-            blocks += (int64_t)all;
+            const int64_t all = (int64_t)m.tiles * s.n_outer * s.n_inner * groups;
+            if (blocks + all > kMoveBlocks) break;
+            blocks += all;
             p.n_states++;
         }
         p.hist_first = blocks;
-        if (h && at == n_states) {
+        if (h && at == n_states && blocks + rows <= kMoveBlocks) {
             p.off = h->off; p.ids = h->ids; p.tokens = h->tokens;
             p.out_off = h->out_off; p.out_ids = h->out_ids;
             p.keep = h->max_history;
             blocks += rows;
+            h = nullptr;
         }
         if (blocks == 0) continue;
         const int rc = launch_moves(p, blocks, stream);
         if (rc != DLK_OK) return rc;
-    } while (at < n_states);
+    } while (at < n_states || h);
     return DLK_OK;
 }

@@ -688,6 +688,10 @@ extern "C" int dlk_beam_select(const dlk_beam_batch *b, int groups, int vocab, c
     if (prm->eos_id < -1 || prm->eos_id >= vocab || (b->finished && prm->eos_id < 0)) return DLK_ERR_INVALID;
     if (!(fabsf(prm->length_penalty) <= 16.0f)) return DLK_ERR_INVALID;
     if (((uintptr_t)b->logits & 3) != 0) return DLK_ERR_INVALID;
+    /* the next state over the last one: rows would be read after others of their group are written */
+    if (b->out_scores == b->scores || (b->lengths && b->out_lengths == b->lengths) ||
+        (b->finished && b->out_finished == b->finished))
+        return DLK_ERR_INVALID;
     if (prm->beams > DLK_MAX_BEAMS || prm->n_out > DLK_MAX_BEAMS) return DLK_ERR_UNSUPPORTED;
     if (prm->max_history > 65535 || vocab > 0x7fffffff - (1 << 20)) return DLK_ERR_UNSUPPORTED;
     if ((int64_t)groups * prm->beams > 0x7fffffff || (int64_t)groups * prm->n_out > 0x7fffffff) return DLK_ERR_UNSUPPORTED;

@@ -405,7 +405,7 @@ __global__ __launch_bounds__(512, 2) void logits_i8_wide_kernel(I8Params p) {
 /* One launch of `kernel`, tiles of BM x BN; the grid a multiple of the XCDs. */
 int launch_tiles(void (*kernel)(I8Params), int bm, int bn, int threads, const I8Params &p, hipStream_t stream) {
     const int64_t tiles = (((int64_t)p.vocab + bn - 1) / bn) * (((int64_t)p.rows + bm - 1) / bm);
-    if (tiles > 0x3fffffff) return DLK_ERR_UNSUPPORTED;
+    if ((tiles + 7) / 8 * 8 * threads > 0xffffffffLL) return DLK_ERR_UNSUPPORTED;      /* (no launch) */
     hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 7) / 8 * 8)), dim3(threads), 0, stream, p);
     return hipGetLastError() == hipSuccess ? DLK_OK : DLK_ERR_HIP;
 }

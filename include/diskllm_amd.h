@@ -271,8 +271,8 @@ int dlk_quantize_rows(const void *x, int dtype, int64_t ldx, int rows, int n, in
 /* logits[r * ld + v] = (sum_i x[r * ldx + i] * w[v * ldw + i]) * x_scale[r] * w_scale[v],
  * the sum exact in 32-bit integers (n <= 131,071, else DLK_ERR_UNSUPPORTED), then
  * three float roundings (the sum's, and one per scale); softcap > 0: then softcap *
- * tanh(logit / softcap) to 2^-20 of it (not libm's bits, which dlk_softcap gives);
- * softcap must be finite.  Any strides and byte alignment of x and w.  Entries past
+ * tanh(logit / softcap) to 2^-20 of it, or to 2^-148 * softcap where that is more (not
+ * libm's bits, which dlk_softcap gives); softcap must be finite.  Any strides and byte alignment of x and w.  Entries past
  * vocab in a row of logits are left as they are. */
 int dlk_logits_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw,
                   const float *w_scale, int rows, int vocab, int n, float softcap, float *logits, int64_t ld,
@@ -328,7 +328,7 @@ typedef struct {
  * Of each group's continuations the n_out with the largest score / max(length,
  * 1)^length_penalty (before rounding) are written, largest first; of equal ones the
  * lower row first, then the larger logit, then the lower id.  Outputs may not overlap
- * inputs.  Takes workspace as dlk_sample does (dlk_release_stream; one call on the
+ * inputs (an output that is its own input is refused).  Takes workspace as dlk_sample does (dlk_release_stream; one call on the
  * stream before capturing it, else DLK_ERR_HIP). */
 int dlk_beam_select(const dlk_beam_batch *batch, int groups, int vocab, const dlk_beam_params *params,
                     hipStream_t stream);
@@ -362,7 +362,8 @@ typedef struct {
  * (-1 among them) moves nothing: the row's states are left, its history is empty.
  * In-place states need n_out == beams; they move as if all rows were read before
  * any is written, and rows that are their own parents cost nothing.  Destinations of
- * one call may not overlap one another, nor any source but their own in place.
+ * one call may not overlap one another, nor any source but their own in place (states
+ * that begin at one address are refused).
  * n_states of any number; history may be NULL. */
 int dlk_beam_reorder(const int32_t *parents, int groups, int beams, int n_out, const dlk_beam_state *states,
                      int n_states, const dlk_beam_history *history, hipStream_t stream);

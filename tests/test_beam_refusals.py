@@ -26,7 +26,8 @@ QUANT = dict(x=A, dtype=_lib.BF16, ldx=64, rows=2, n=64, q=A, ldq=64, scale=A, s
     (dict(x=None), INV), (dict(q=None), INV), (dict(scale=None), INV), (dict(rows=-1), INV), (dict(n=0), INV),
     (dict(ldx=63), INV), (dict(ldq=63), INV), (dict(dtype=3), INV), (dict(dtype=-1), INV), (dict(x=A + 1), INV),
     (dict(x=A + 2, dtype=_lib.F32), INV), (dict(scale=A + 2), INV),
-    (dict(n=0x7fffffff, ldx=1 << 40, ldq=1 << 40), UNS), (dict(rows=0), OK)])
+    (dict(n=0x7fffffff, ldx=1 << 40, ldq=1 << 40), UNS), (dict(rows=0), OK),
+    (dict(n=2000, ldx=2000, ldq=2000, rows=1 << 24), UNS), (dict(rows=1 << 26), UNS)])      # 2^32 threads
 def test_quantize_rows(kw, rc):
     assert call(_lib.lib().dlk_quantize_rows, QUANT, **kw) == rc
 
@@ -39,13 +40,14 @@ LOGITS = dict(x=A, ldx=64, x_scale=A, w=A, ldw=64, w_scale=A, rows=2, vocab=100,
     (dict(x=None), INV), (dict(w=None), INV), (dict(x_scale=None), INV), (dict(w_scale=None), INV),
     (dict(logits=None), INV), (dict(rows=-1), INV), (dict(vocab=0), INV), (dict(n=0), INV), (dict(ldx=63), INV),
     (dict(ldw=63), INV), (dict(ld=99), INV), (dict(logits=A + 2), INV), (dict(w_scale=A + 1), INV),
-    (dict(n=131072, ldx=131072, ldw=131072), UNS), (dict(softcap=float("inf")), INV), (dict(vocab=0x7fffffff, ld=1 << 40), UNS), (dict(rows=0), OK)])
+    (dict(n=131072, ldx=131072, ldw=131072), UNS), (dict(softcap=float("inf")), INV), (dict(vocab=0x7fffffff, ld=1 << 40), UNS), (dict(rows=0), OK),
+    (dict(vocab=1 << 30, ld=1 << 30), UNS)])
 def test_logits_i8(kw, rc):
     assert call(_lib.lib().dlk_logits_i8, LOGITS, **kw) == rc
 
 
 def select(groups=1, vocab=100, batch=(), **prm):
-    b = _lib.BeamBatch(logits=A, ld=vocab, scores=A, out_tokens=A, out_parents=A, out_scores=A)
+    b = _lib.BeamBatch(logits=A, ld=vocab, scores=A + 4096, out_tokens=A, out_parents=A, out_scores=A)
     for k, v in dict(batch).items():
         setattr(b, k, v)
     p = _lib.BeamParams(beams=4, n_out=4, eos_id=-1, length_penalty=0.0, repeat_penalty=1.0)
@@ -63,7 +65,10 @@ def select(groups=1, vocab=100, batch=(), **prm):
     (dict(batch=dict(finished=A)), INV), (dict(length_penalty=float("nan")), INV),
     (dict(length_penalty=float("inf")), INV), (dict(length_penalty=17.0), INV), (dict(max_history=-1), INV),
     (dict(beams=65), UNS), (dict(n_out=65), UNS), (dict(max_history=65536), UNS),
-    (dict(vocab=0x7fffffff), UNS), (dict(groups=0x7fffffff), UNS), (dict(groups=0), OK)])
+    (dict(vocab=0x7fffffff), UNS), (dict(groups=0x7fffffff), UNS), (dict(groups=0), OK),
+    # an output that is its own input
+    (dict(batch=dict(out_scores=A, scores=A)), INV), (dict(batch=dict(out_lengths=A, lengths=A)), INV),
+    (dict(batch=dict(out_finished=A, finished=A), eos_id=3), INV)])
 def test_beam_select(kw, rc):
     assert select(**kw) == rc
     assert _lib.lib().dlk_beam_select(None, 1, 100, None, None) == INV
@@ -96,6 +101,11 @@ FAR = A + (1 << 20)
     # destinations that overlap themselves
     (dict(states=[state(bytes=65)]), INV), (dict(states=[state(src_row=64, dst_row=64)]), INV),
     (dict(states=[state(src_outer=512, dst_outer=512)]), INV),
+    # more than a launch takes
+    (dict(states=[state(n_outer=1 << 23, n_inner=1, src_outer=1024, dst_outer=1024)]), UNS),
+    # one buffer twice, in place or behind another source; two that change places
+    (dict(states=[state(), state()]), INV), (dict(states=[state(dst=FAR), state(src=A - 8192, dst=FAR)]), INV),
+    (dict(states=[state(dst=FAR), state(src=FAR, dst=A)]), INV), (dict(states=[state(), state(dst=FAR)]), INV),
     # two buffers that overlap
     (dict(states=[state(dst=A + 4096)]), INV), (dict(states=[state(dst=A - 4096)]), INV)])
 def test_beam_reorder(kw, rc):
@@ -105,12 +115,14 @@ def test_beam_reorder(kw, rc):
 @pytest.mark.parametrize("kw,rc", [
     (dict(off=None), INV), (dict(ids=None), INV), (dict(out_off=None), INV), (dict(out_ids=None), INV),
     (dict(max_history=0), INV), (dict(out_off=A), INV), (dict(out_ids=A + 256), INV),
-    (dict(max_history=0x10000000), UNS)])
+    (dict(max_history=0x10000000), UNS), (dict(groups=1 << 22, max_history=1), UNS)])
 def test_beam_history(kw, rc):
     h = _lib.BeamHistory(A, A + 256, A + 512, 16, FAR, FAR + 256)
+    groups = kw.get("groups", 2)
     for k, v in kw.items():
-        setattr(h, k, v)
-    assert reorder(history=C.byref(h)) == rc
+        if k != "groups":
+            setattr(h, k, v)
+    assert reorder(groups=groups, history=C.byref(h)) == rc
 
 
 def test_python_refusals():

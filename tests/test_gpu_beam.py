@@ -369,6 +369,7 @@ def test_reorder_nothing(cuda):
     cache = torch.randn((2, 3, 4), device="cuda")
     want = cache.clone()
     api.beam_reorder(p, 2, 2, [api.beam_state(cache, row_dim=0, length_dim=1, length=0)])
+    api.beam_reorder(p, 2, 2, [api.beam_state(torch.zeros((2, 0, 3), device="cuda")), api.beam_state(torch.zeros((2, 0), device="cuda"))])
     torch.cuda.synchronize()
     assert torch.equal(cache, want)
     many = [torch.full((2, 5), float(k), device="cuda") + torch.tensor([[0.0], [0.5]], device="cuda") for k in range(21)]
@@ -421,6 +422,28 @@ def test_reorder_far_rows(cuda):
     rows.copy_(x)
     api.beam_reorder(torch.tensor([2, 0, 2], dtype=torch.int32, device="cuda"), 3, 3, [api.beam_state(rows)])
     assert torch.equal(rows, x[[2, 0, 2]])
+
+
+@pytest.mark.parametrize("kind", ["bytes", "histories"])
+def test_reorder_past_a_launch(cuda, kind):
+    """More workgroups than a launch takes: the states, or the histories after them, go into a second one."""
+    import torch
+    from diskllm_amd import api
+    p = torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+    n = (1 << 24) - (1 if kind == "histories" else 1 << 20)
+    big = torch.zeros((n, 2), dtype=torch.uint8, device="cuda")            # a byte a row, n times
+    big[:, 1] = 7
+    small = torch.tensor([[1.0], [2.0]], device="cuda").repeat(1 << 21, 1, 1) if kind == "bytes" else torch.ones((2, 1), device="cuda")
+    off = torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda")
+    ids = torch.tensor([5, 6, 7], dtype=torch.int32, device="cuda")
+    out_off, out_ids = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.zeros(8, dtype=torch.int32, device="cuda")
+    states = [api.beam_state(big, row_dim=1)] + ([api.beam_state(small, row_dim=1)] if kind == "bytes" else [])
+    api.beam_reorder(p, 2, 2, states, api.beam_history(off, ids, None, 4, out_off, out_ids))
+    torch.cuda.synchronize()
+    assert (big[:, 0] == 7).all() and (big[:, 1] == 0).all()
+    if kind == "bytes":
+        assert (small[:, 0] == 2).all() and (small[:, 1] == 1).all()
+    assert out_off.tolist() == [0, 2, 3] and out_ids.tolist() == [6, 7, 5, 0, 0, 0, 0, 0]
 
 
 # ---- whole searches --------------------------------------------------------------
@@ -616,6 +639,57 @@ def test_capture_without_workspace_is_refused(cuda):
             api.beam_select(lg, 4, 4, out=out)
     g.replay()
     torch.cuda.synchronize()
+
+
+def test_calls_of_all_sizes_on_one_stream(cuda):
+    """Calls that share a workspace one after another, each smaller or larger than the last, and dlk_sample between
+    them; the same into a graph, replayed with such calls in between."""
+    import torch
+    from diskllm_amd import _lib, api
+    from diskllm_amd import workloads as W
+    g = torch.Generator("cuda").manual_seed(12)
+    sizes = [(4, 4, 4, 32000), (64, 8, 16, 50257), (2, 1, 64, 700), (16, 16, 3, 9001), (192, 64, 64, 30000)]
+    lg = [torch.randn((r, v), device="cuda", generator=g) for r, _, _, v in sizes]
+    db = api.to_device(W.c3(rows=4, vocab=4099))
+    api.sample(db)
+    ids = db.out_ids.clone()
+    alone = []
+    for x, (_, b, n, _) in zip(lg, sizes):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            st.wait_stream(torch.cuda.default_stream())
+            alone.append(api.beam_select(x, b, n))
+            st.synchronize()
+        _lib.check(_lib.lib().dlk_release_stream(st.cuda_stream), "dlk_release_stream")
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        for k in (0, 1, 2, 3, 4, 2, 0, 4, 1):
+            got = api.beam_select(lg[k], *sizes[k][1:3])
+            db.reset_rng()
+            api.sample(db)
+            assert torch.equal(db.out_ids, ids)
+            for name in got:
+                assert torch.equal(got[name], alone[k][name]), (k, name)
+    st.synchronize()
+    outs = [{k: torch.zeros_like(v) for k, v in a.items()} for a in alone]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        for x, (_, b, n, _), o in zip(lg, sizes, outs):
+            api.beam_select(x, b, n, out=o)
+    for k in (4, 0, 2):
+        for o in outs:
+            for v in o.values():
+                v.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            got = api.beam_select(lg[k], *sizes[k][1:3])
+            graph.replay()
+        torch.cuda.synchronize()
+        for a, o in zip(alone + [alone[k]], outs + [got]):
+            for name in a:
+                assert torch.equal(a[name], o[name]), name
+    del graph
+    _lib.check(_lib.lib().dlk_release_stream(st.cuda_stream), "dlk_release_stream")
 
 
 def test_streams_at_once(cuda):
