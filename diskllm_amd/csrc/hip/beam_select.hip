@@ -189,27 +189,28 @@ DLK_DEV void write_none(const BeamParams &p, int g, int j) {
     if (p.out_finished) p.out_finished[o] = 0;
 }
 
-/* The group's lists merged, by its last workgroup.  Up to one list per thread (256) the
- * slots and each list's first entries are asked for at once: a round trip to the other
- * workgroups' words is most of what a merge takes. */
+/* The group's lists merged, by its last workgroup.  Up to one list per thread (256) and 16
+ * entries of them all per thread (4,096) the slots and entries are asked for at once: a
+ * round trip to the other workgroups' words is most of what a merge takes. */
 DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
-    constexpr int T = kBeamThreads, PRE = 8;
+    constexpr int T = kBeamThreads, PRE = 16, AT_ONCE = 8;
     const int t = threadIdx.x, lane = lane_id(), wave = wave_id(), g = p.g0 + gl;
-    const int L = p.beams * p.slices;
+    const int L = p.beams * p.slices, E = L * p.n;
     const BeamSlot *slots = p.slots + (int64_t)gl * L;
     const uint64_t *cands = p.cands + (int64_t)gl * L * p.n;
-    /* list i, that of (row i / slices, slice i % slices), goes to thread (i % 4) * 64 + i / 4 % 64, so
-     * that the waves share few lists evenly */
+    /* list i is that of (row i / slices, slice i % slices).  List or entry i goes to thread
+     * (i % 4) * 64 + i / 4 % 64, so that the waves share few of them evenly */
     const int mine = (t & 63) * 4 + (t >> 6);
-    const bool once = L <= T;
-    uint64_t pre[PRE], sum0 = 0, mk0 = 0;
-    if (once && mine < L) {
-        sum0 = bget64(&slots[mine].sum);
-        mk0 = bget64(&slots[mine].max_kept);
+    const bool once = L <= T, flat = once && E <= PRE * T;
+    uint64_t pre[PRE];
+    if (once && t < L) {
+        sh.key[t] = bget64(&slots[t].sum);
+        sh.ent[t] = bget64(&slots[t].max_kept);
+    }
+    if (flat) {
 #pragma unroll
-        for (int j = 0; j < PRE; j++) pre[j] = bget64(&cands[(int64_t)mine * p.n + min(j, p.n - 1)]);
-        sh.key[mine] = sum0;
-        sh.ent[mine] = mk0;
+        for (int q = 0; q < PRE; q++)
+            if (q * T < E) pre[q] = bget64(&cands[min(q * T + mine, E - 1)]);
     }
     if (t == 0) sh.count = 0;
     __syncthreads();
@@ -260,48 +261,80 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
     }
     __syncthreads();
     /* list i of row b: its entries (a finished row's first list holds its one continuation) */
-    auto listed = [&](int i, int b) {
+    auto listed = [&](int i, int b, uint64_t max_kept) {
         const int kind = sh.kind[b];
-        if (kind != 1) return kind == 2 && i == b * p.slices ? 1 : 0;
-        return (int)(uint32_t)(once ? mk0 : bget64(&slots[i].max_kept));
+        return kind == 1 ? (int)(uint32_t)max_kept : kind == 2 && i == b * p.slices ? 1 : 0;
     };
     auto entry = [&](int i, int b, int j) -> uint64_t {
         return sh.kind[b] == 2 ? ~(uint64_t)0 : bget64(&cands[(int64_t)i * p.n + j]);
     };
-    uint64_t head = 0;
-    for (int i = mine; i < L; i += T) {
-        const int b = i / p.slices;
-        if (listed(i, b) > 0) head = max(head, BeamRow(sh, b).key(once ? pre[0] : entry(i, b, 0)));
-    }
-    /* a bound that n heads, thus n continuations, reach */
-    const uint32_t kw = wave_rth((uint32_t)(head >> 32), (p.n + 3) / 4);
-    if (lane == 0) sh.wave_key[wave] = kw;
-    __syncthreads();
-    uint32_t bound = sh.wave_key[0];
+    auto add = [&](uint64_t k, uint64_t e, int b) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kBeamList) {
+            sh.key[at] = k;
+            sh.ent[at] = e;
+            sh.place[at] = b;
+        }
+    };
+    /* a bound that n continuations reach: n / 4 of each wave's lanes have one that does, or,
+     * where a wave has fewer (lists of one or two entries), n of one wave's */
+    auto bound_of = [&](uint32_t best) {
+        uint32_t bound = 0;
+#pragma unroll 1
+        for (int all = 0; all < 2 && bound == 0; all++) {
+            const uint32_t kw = wave_rth(best, all ? p.n : (p.n + 3) / 4);
+            __syncthreads();
+            if (lane == 0) sh.wave_key[wave] = kw;
+            __syncthreads();
+            bound = sh.wave_key[0];
 #pragma unroll
-    for (int w = 1; w < T / 64; w++) bound = min(bound, sh.wave_key[w]);
-    for (int i = mine; i < L; i += T) {
-        const int b = i / p.slices, n = listed(i, b);
-        if (n == 0) continue;
-        const BeamRow row(sh, b);
-        bool more = true;
-        for (int j = 0; more && j < n; j += PRE) {
-            if (!once || j > 0) {                         /* the next few entries, in one round trip */
+            for (int w = 1; w < T / 64; w++) bound = all ? max(bound, sh.wave_key[w]) : min(bound, sh.wave_key[w]);
+        }
+        return bound;
+    };
+    if (flat) {
+        uint32_t key[PRE], best = 0;                         /* high words, 0: none */
+        const float per_n = 1.0f / (float)p.n, per_slices = 1.0f / (float)p.slices;
+        auto list_of = [&](int at) { return (int)(((float)at + 0.5f) * per_n); };          /* exact: below 2^12 */
+        auto row_of = [&](int i) { return (int)(((float)i + 0.5f) * per_slices); };
 #pragma unroll
-                for (int q = 0; q < PRE; q++) pre[q] = j + q < n ? entry(i, b, j + q) : 0;
-            }
+        for (int q = 0; q < PRE; q++) {                      /* (few entries: few instructions, fetched for the first time) */
+            key[q] = 0;
+            if (q * T >= E) continue;
+            const int at = min(q * T + mine, E - 1), i = list_of(at), b = row_of(i);
+            if (sh.kind[b] == 2) pre[q] = ~(uint64_t)0;
+            if (q * T + mine < E && at - i * p.n < listed(i, b, sh.ent[i])) key[q] = (uint32_t)(BeamRow(sh, b).key(pre[q]) >> 32);
+            best = max(best, key[q]);
+        }
+        const uint32_t bound = bound_of(best);               /* (sh.ent has been read) */
 #pragma unroll
-            for (int q = 0; q < PRE; q++) {
-                if (!more || j + q >= n) break;
-                const uint64_t k = row.key(pre[q]);
-                more = (uint32_t)(k >> 32) >= bound;      /* (the list is in order) */
-                if (more) {
-                    const int at = atomicAdd(&sh.count, 1);
-                    if (at < kBeamList) {
-                        sh.key[at] = k;
-                        sh.ent[at] = pre[q];
-                        sh.place[at] = b;
-                    }
+        for (int q = 0; q < PRE; q++) {
+            if (key[q] == 0 || key[q] < bound) continue;
+            const int b = row_of(list_of(q * T + mine));
+            add(BeamRow(sh, b).key(pre[q]), pre[q], b);
+        }
+    } else {
+        uint64_t head = 0;
+        for (int i = mine; i < L; i += T) {
+            const int b = i / p.slices;
+            if (listed(i, b, bget64(&slots[i].max_kept)) > 0) head = max(head, BeamRow(sh, b).key(entry(i, b, 0)));
+        }
+        const uint32_t bound = bound_of((uint32_t)(head >> 32));
+        for (int i = mine; i < L; i += T) {
+            const int b = i / p.slices, n = listed(i, b, bget64(&slots[i].max_kept));
+            if (n == 0) continue;
+            const BeamRow row(sh, b);
+            bool more = true;
+            for (int j = 0; more && j < n; j += AT_ONCE) {
+                uint64_t e[AT_ONCE];                         /* the next few entries, in one round trip */
+#pragma unroll
+                for (int q = 0; q < AT_ONCE; q++) e[q] = j + q < n ? entry(i, b, j + q) : 0;
+#pragma unroll
+                for (int q = 0; q < AT_ONCE; q++) {
+                    if (!more || j + q >= n) break;
+                    const uint64_t k = row.key(e[q]);
+                    more = (uint32_t)(k >> 32) >= bound;     /* (the list is in order) */
+                    if (more) add(k, e[q], b);
                 }
             }
         }
@@ -320,42 +353,49 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
         }
         for (int j = C + t; j < p.n; j += T) write_none(p, g, j);
     } else {
-        /* too many at or above the bound (few lists for n, or runs of equal keys): the best one
-         * still left, n times, the written ones known by the last one's place in the order */
-        uint64_t lk = ~0ull, le = ~0ull;
-        int lb = -1;
-        for (int j = 0; j < p.n; j++) {
-            uint64_t bk = 0, be = 0;
-            int bi = -1;
-            for (int i = mine; i < L; i += T) {
-                const int b = i / p.slices, n = listed(i, b);
-                for (int q = 0; q < n; q++) {
-                    const uint64_t e = entry(i, b, q), k = BeamRow(sh, b).key(e);
-                    if (!before(lk, lb, le, k, b, e)) continue;               /* written */
-                    if (bi < 0 || before(k, b, e, bk, bi, be)) { bk = k; be = e; bi = b; }
-                    break;                                                    /* (the list is in order) */
-                }
-            }
-            for (int m = 1; m < 64; m <<= 1) {
-                const uint64_t ok = shfl_xor(bk, m), oe = shfl_xor(be, m);
-                const int oi = shfl_xor(bi, m);
-                if (oi >= 0 && (bi < 0 || before(ok, oi, oe, bk, bi, be))) { bk = ok; be = oe; bi = oi; }
-            }
-            if (lane == 0) { sh.best_key[wave] = bk; sh.best_ent[wave] = be; sh.best_row[wave] = bi; }
-            __syncthreads();
+        /* too many at or above the bound (few lists for n, or runs of equal keys): the best of the
+         * lists' next entries, n times */
+        uint8_t *next = (uint8_t *)sh.key;                   /* each list's; L is 319 at most */
+        uint64_t bk, be;
+        int bi, bl = 0;
+        auto best_of_mine = [&]() {
+            bk = be = 0;
             bi = -1;
+            for (int i = mine; i < L; i += T) {
+                const int b = i / p.slices, q = next[i];
+                if (q >= listed(i, b, bget64(&slots[i].max_kept))) continue;
+                const uint64_t e = entry(i, b, q), k = BeamRow(sh, b).key(e);
+                if (bi < 0 || before(k, b, e, bk, bi, be)) { bk = k; be = e; bi = b; bl = i; }
+            }
+        };
+        for (int i = mine; i < L; i += T) next[i] = 0;
+        best_of_mine();
+        for (int j = 0; j < p.n; j++) {
+            uint64_t k = bk, e = be;
+            int r = bi;
+            for (int m = 1; m < 64; m <<= 1) {
+                const uint64_t ok = shfl_xor(k, m), oe = shfl_xor(e, m);
+                const int oi = shfl_xor(r, m);
+                if (oi >= 0 && (r < 0 || before(ok, oi, oe, k, r, e))) { k = ok; e = oe; r = oi; }
+            }
+            if (lane == 0) { sh.best_key[wave] = k; sh.best_ent[wave] = e; sh.best_row[wave] = r; }
+            __syncthreads();
+            r = -1;
             for (int w = 0; w < T / 64; w++) {
                 const int oi = sh.best_row[w];
-                if (oi >= 0 && (bi < 0 || before(sh.best_key[w], oi, sh.best_ent[w], bk, bi, be))) {
-                    bk = sh.best_key[w]; be = sh.best_ent[w]; bi = oi;
+                if (oi >= 0 && (r < 0 || before(sh.best_key[w], oi, sh.best_ent[w], k, r, e))) {
+                    k = sh.best_key[w]; e = sh.best_ent[w]; r = oi;
                 }
             }
             __syncthreads();
             if (t == 0) {
-                if (bi >= 0) write_continuation(p, sh, g, j, bi, be);
+                if (r >= 0) write_continuation(p, sh, g, j, r, e);
                 else write_none(p, g, j);
             }
-            if (bi >= 0) { lk = bk; le = be; lb = bi; }
+            if (bi >= 0 && bi == r && be == e) {             /* (an id of a row is in one list) */
+                next[bl]++;
+                best_of_mine();
+            }
         }
     }
 }
@@ -412,6 +452,13 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
     uint32_t kept = 0;
     if (!idle) {
         if (t == 0) sh.count = 0;
+        int32_t id0 = -1, id1 = -1;                /* the first ids, in registers for every batch */
+        if (HIST && hn > 0) {
+            for (int i = t; i < B / 8; i += T) ((uint4 *)times)[i] = make_uint4(0, 0, 0, 0);
+            if (t < hn) id0 = hist[t];
+            if (t + T < hn) id1 = hist[t + T];
+            __syncthreads();
+        }
         float most = -INFINITY;                    /* this thread's maximum, and its sum of exp(l - that) */
         double part = 0.0;
         bool bad = false;
@@ -433,17 +480,18 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
                 }
             }
             if (HIST && hn > 0) {
-                for (int i = t; i < B / 8; i += T) ((uint4 *)times)[i] = make_uint4(0, 0, 0, 0);
-                __syncthreads();
-                for (int i = t; i < hn; i += T) {
-                    const int32_t id = hist[i];
+                auto occurs = [&](int32_t id) {
                     if (id >= b0 && id < s1 && id - b0 < B) atomicAdd(&times[(id - b0) >> 1], 1u << (16 * (id & 1)));
-                }
+                };
+                occurs(id0);
+                occurs(id1);
+                for (int i = t + 2 * T; i < hn; i += T) occurs(hist[i]);
                 __syncthreads();
 #pragma unroll
                 for (int j = 0; j < GR; j++) {
                     const uint2 w = ((const uint2 *)times)[j * T + t];
                     if ((w.x | w.y) != 0) {
+                        ((uint2 *)times)[j * T + t] = make_uint2(0, 0);          /* for the next batch */
 #pragma unroll 1
                         for (int c = 0; c < 4; c++) {
                             const int nc = (int)(((c < 2 ? w.x : w.y) >> (16 * (c & 1))) & 0xffff);

@@ -246,6 +246,32 @@ def test_select_equal_logits_many_rows(cuda):
         assert (out["parents"].view(32, 64).cpu() == torch.arange(0, 96, 3)[:, None]).all()
 
 
+@pytest.mark.parametrize("beams,n_out,V", [(16, 16, 50257), (64, 64, 20000), (64, 64, 9001), (33, 64, 30000), (5, 11, 70000),
+                                           (1, 64, 40000)])
+def test_select_few_and_equal_entries(cuda, beams, n_out, V):
+    """Lists of one to three entries, groups of one live row, parts of the vocabulary that are masked, scores that
+    leave one row ahead, and equal logits throughout: the merges with few entries, and with too many at its bound."""
+    import torch
+    rng = np.random.default_rng(V + beams)
+    rows = 2 * beams
+    lg = logits(rng, rows, V)
+    first = np.full(rows, -INF, np.float32)
+    first[::beams] = 0
+    check(torch, lg, beams, n_out, scores=first)
+    for keep in (1, 3):
+        allow = np.zeros((rows, V), bool)
+        for at in range(0, V, 4096):
+            allow[:, at:at + 4096 * (at % 8192 == 0):97][:, :keep] = True
+        check(torch, lg, beams, n_out, mask=mask_of(allow))
+    check(torch, lg, beams, n_out, mask=mask_of(np.broadcast_to(np.arange(V) % 16384 < 12288, (rows, V))))
+    ahead = np.full(rows, -30, np.float32)
+    ahead[beams - 1::beams] = 0
+    check(torch, lg, beams, n_out, scores=ahead)
+    lg[:] = 1.0
+    check(torch, lg, beams, n_out)
+    check(torch, lg, beams, n_out, scores=ahead)
+
+
 def test_select_all_finished(cuda):
     """A group whose beams have all ended keeps them, ordered by their normalised scores."""
     import torch
