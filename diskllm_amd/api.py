@@ -218,12 +218,18 @@ def quantize_rows(x: torch.Tensor, q: Optional[torch.Tensor] = None, scale: Opti
     dev = x.get_device()
     rows, n, ldx = _rows2d(x, dev, None, "x")
     if q is None:
-        q = torch.empty((rows, (n + 15) // 16 * 16), dtype=_I8, device=x.device)[:, :n]
+        ldq = (n + 15) // 16 * 16
+        q = torch.empty((rows, ldq), dtype=_I8, device=x.device)
+        if ldq != n:
+            q = q[:, :n]
+    else:
+        q_rows, q_n, ldq = _rows2d(q, dev, _I8, "q")
+        _want(q_rows == rows and q_n == n, "q: x's shape is wanted")
     if scale is None:
         scale = torch.empty(rows, dtype=_F32, device=x.device)
-    q_rows, q_n, ldq = _rows2d(q, dev, _I8, "q")
-    _want(q_rows == rows and q_n == n, "q: x's shape is wanted")
-    at = _flat(scale, rows, dev, _F32, "scale")
+        at = scale.data_ptr()
+    else:
+        at = _flat(scale, rows, dev, _F32, "scale")
     if rows:
         _call(dev, stream, "dlk_quantize_rows", _lib.lib().dlk_quantize_rows, x.data_ptr(), dt, ldx, rows, n,
               q.data_ptr(), ldq, at)
@@ -239,9 +245,13 @@ def logits_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     V, w_n, ldw = _rows2d(w, dev, _I8, "w")
     _want(w_n == n, "x and w: rows of one length are wanted")
     if out is None:
-        out = torch.empty((rows, (V + 63) // 64 * 64), dtype=_F32, device=x.device)[:, :V]
-    o_rows, o_n, ld = _rows2d(out, dev, _F32, "out")
-    _want(o_rows == rows and o_n == V, "out: [rows, vocab] is wanted")
+        ld = (V + 63) // 64 * 64
+        out = torch.empty((rows, ld), dtype=_F32, device=x.device)
+        if ld != V:
+            out = out[:, :V]
+    else:
+        o_rows, o_n, ld = _rows2d(out, dev, _F32, "out")
+        _want(o_rows == rows and o_n == V, "out: [rows, vocab] is wanted")
     xs, ws = _flat(x_scale, rows, dev, _F32, "x_scale"), _flat(w_scale, V, dev, _F32, "w_scale")
     if rows:
         _call(dev, stream, "dlk_logits_i8", _lib.lib().dlk_logits_i8, x.data_ptr(), ldx, xs, w.data_ptr(), ldw, ws,

@@ -9,7 +9,16 @@
  * parents (a row may be parent to several and change its own place) with no second
  * buffer and no order among workgroups, since no two share a column.  Rows that are their
  * own parents are skipped in place: neither read nor written.  16-byte accesses of any
- * alignment.
+ * alignment.  A thread has as many rows' bytes in registers as a group has rows (rounded
+ * up to 4, 8, .. 64): the loads of a column are in flight together.
+ *
+ * 16 requests of 4 beams with 2.7 GB of cache, two thirds of the rows moving: 476-516 us, a large copy's
+ * 5.1 to 5.6 TB/s, read and written.  A request's few small states: 4-5 us (13.5 with the
+ * host's checks of the tensors), all of them and the histories in one launch.
+ *
+ * A history's place in the CSR is the sum of the lengths before it, which each row's
+ * workgroup sums anew (rows of a batch are few: 4,096 are 16 loads a thread) rather than
+ * waiting for another's.
  */
 #include <hip/hip_runtime.h>
 

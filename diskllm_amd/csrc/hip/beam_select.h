@@ -49,7 +49,7 @@ struct BeamParams {
  * resident together) where that takes at most six batches each, so that a workgroup's
  * fixed 5 us are paid few times (us by batches of each:
  *   64 x 151,936 with histories   1: 46, 2: 33.4, 3: 32.9, 4: 35, 8: 50
- *   128 x 50,257 in groups of 16  1: 39, 2: 32.5, 3: 31.6, 4: 38
+ *   128 x 50,257 in groups of 16  1: 39, 2: 32.5, 3: 31.6, 4: 38 (the merge has become 5 shorter since)
  *   512 x 262,144                 1: 302, 2: 185, 3: 156, 4: 145, 8: 145
  *   4 x 32,000                    1: 11.4, 2: 13.8);
  * more where the merge would meet over 256 lists a group, which it takes in one round trip. */

@@ -2,15 +2,25 @@
  * beam_select.hip -- one step of a beam search: of the continuations (row, id) of a group
  * of rows the n with the largest score + log softmax(l)[id] (dlk_beam_select).
  *
- * One workgroup reads a slice of 2,048 to 8,192 logits of a row once, into registers; masks and
- * penalises them; sums exp(l - slice maximum) in 64 bits; and lists the slice's n
- * largest entries in order.  Log softmax is increasing in l, so a row's n best
- * continuations are its n largest logits and none of the others is needed again.  The
- * group's last workgroup to finish (relaxed agent-scope atomics, as the top-k kernel's)
- * joins the slices' sums and merges the lists under the keys in 64 bits.
+ * One workgroup reads a slice of a row (beam_batches() times 4,096 logits) once, 4,096 at a
+ * time into registers; masks and penalises them; sums exp(l - its maximum so far) in 64
+ * bits; and lists the slice's n largest entries in order.  Log softmax is increasing in l,
+ * so a row's n best continuations are its n largest logits and none of the others is
+ * needed again.  The group's last workgroup to finish (relaxed agent-scope atomics, as the
+ * top-k kernel's) joins the slices' sums and merges the lists under the keys in 64 bits: one
+ * launch, and no order of arrival shows in the result.
  *
  * Sums and keys are 64-bit because the order of continuations of different rows hangs on
- * differences of their log-sums; 64-bit FMAs run at the plain 32-bit ones' rate here.
+ * differences of their log-sums, which a sum of 262,144 terms in 32 bits blurs by more than
+ * neighbouring candidates differ; 64-bit FMAs run at the plain 32-bit ones' rate here.
+ *
+ * Bounds.  Large calls: the vector units, with some 24 instructions a logit, 18 of them the
+ * exponential (512 x 262,144 masked: 136-146 us, 3.8 TB/s; 90 at a copy's rate).  Calls that fit the
+ * chip once: the chain of a slice and the merge (64 x 151,936 with penalties 32.5 us, of
+ * which 20 a slice's at the median, 28 at the last, 4-5 the merge's; 128 x 50,257 in groups
+ * of 16 25.6, 17 and 8).  Small ones: a dozen round trips one after another (4 x 32,000: 10.5 us).
+ * The next batch's loads ahead of this one's work changed nothing: waves of other
+ * workgroups fill that time.
  */
 #include "dlk_device.h"
 #include "beam_select.h"
