@@ -39,27 +39,26 @@ struct BeamParams {
     float rep, freq, pres;
     int g0;              /* first group of the launch */
     int slices;          /* workgroups per row */
-    int batches;         /* of each */
+    int batches;         /* of a row, shared out to them */
     uint32_t *counters;  /* [groups] zero between launches */
     BeamSlot *slots;     /* [rows][slices] */
     uint64_t *cands;     /* [rows][slices][n] */
 };
 
-/* Batches of each workgroup for rows of `vocab` logits: about 1,100 workgroups (some four a CU,
- * resident together) where that takes at most six batches each, so that a workgroup's
- * fixed 5 us are paid few times (us by batches of each:
- *   64 x 151,936 with histories   1: 46, 2: 33.4, 3: 32.9, 4: 35, 8: 50
- *   128 x 50,257 in groups of 16  1: 39, 2: 32.5, 3: 31.6, 4: 38 (the merge has become 5 shorter since)
- *   512 x 262,144                 1: 302, 2: 185, 3: 156, 4: 145, 8: 145
- *   4 x 32,000                    1: 11.4, 2: 13.8);
- * more where the merge would meet over 256 lists a group, which it takes in one round trip. */
-inline int beam_batches(int64_t rows, int beams, int vocab) {
-    const int64_t per_row = ((int64_t)vocab + kBeamBatch - 1) / kBeamBatch;
-    int64_t m = (rows * per_row + 1099) / 1100;
-    if (m > 6) m = 6;
-    if (m < (per_row * beams + 255) / 256) m = (per_row * beams + 255) / 256;
-    const int64_t slices = (per_row + m - 1) / m;
-    return (int)((per_row + slices - 1) / slices);
+/* Workgroups for each row of `vocab` logits: some 800 in all (three a CU: beyond that the
+ * fixed 2.6 us of each cost more than more waves give), where that leaves eight batches
+ * each at most, and 256 to a group at most, whose lists the merge takes in one round trip
+ * (us by workgroups a row:
+ *   64 x 151,936 with histories   10: 34.4, 12: 34.1, 13: 33.7, 16: 34.9, 20: 36.3
+ *   128 x 50,257 in groups of 16  4: 25.0, 6: 24.7, 8: 28.1, 10: 29.4
+ *   512 x 262,144 masked          4: 142, 5: 132, 8: 129, 10: 128, 14: 131
+ *   4 x 32,000                    4: 13.8, 8: 11.4). */
+inline int beam_slices(int64_t rows, int beams, int vocab) {
+    const int64_t batches = ((int64_t)vocab + kBeamBatch - 1) / kBeamBatch;
+    int64_t s = (800 + rows / 2) / rows;
+    if (s < (batches + 7) / 8) s = (batches + 7) / 8;
+    if (s > kBeamThreads / beams) s = kBeamThreads / beams;
+    return (int)(s < batches ? s : batches);
 }
 
 }  // namespace dlk

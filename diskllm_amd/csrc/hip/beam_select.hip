@@ -2,25 +2,28 @@
  * beam_select.hip -- one step of a beam search: of the continuations (row, id) of a group
  * of rows the n with the largest score + log softmax(l)[id] (dlk_beam_select).
  *
- * One workgroup reads a slice of a row (beam_batches() times 4,096 logits) once, 4,096 at a
- * time into registers; masks and penalises them; sums exp(l - its maximum so far) in 64
- * bits; and lists the slice's n largest entries in order.  Log softmax is increasing in l,
- * so a row's n best continuations are its n largest logits and none of the others is
- * needed again.  The group's last workgroup to finish (relaxed agent-scope atomics, as the
- * top-k kernel's) joins the slices' sums and merges the lists under the keys in 64 bits: one
- * launch, and no order of arrival shows in the result.
+ * One workgroup reads a slice of a row (beam_slices() to a row) once, 4,096 logits at a time
+ * into registers; masks and penalises them; sums exp(l - its maximum so far) in 64 bits;
+ * and lists the slice's n largest entries in order.  Log softmax is increasing in l, so a
+ * row's n best continuations are its n largest logits and none of the others is needed
+ * again.  Its four waves work alone from the first batch's bound (n entries of the
+ * workgroup reach it) to the end: each has a list of its own, counts its own history ids and
+ * sums its own logits, where a mask leaves few of them (512 of 1,024) packed side by side.
+ * The group's last workgroup to finish (relaxed agent-scope atomics, as the top-k kernel's)
+ * joins the slices' sums and merges the lists under the keys in 64 bits: one launch, and
+ * no order of arrival shows in the result.
  *
  * Sums and keys are 64-bit because the order of continuations of different rows hangs on
  * differences of their log-sums, which a sum of 262,144 terms in 32 bits blurs by more than
  * neighbouring candidates differ; 64-bit FMAs run at the plain 32-bit ones' rate here.
  *
- * Bounds.  Large calls: the vector units, with some 24 instructions a logit, 18 of them the
- * exponential (512 x 262,144 masked: 136-146 us, 3.8 TB/s; 90 at a copy's rate).  Calls that fit the
- * chip once: the chain of a slice and the merge (64 x 151,936 with penalties 32.5 us, of
- * which 20 a slice's at the median, 28 at the last, 4-5 the merge's; 128 x 50,257 in groups
- * of 16 25.6, 17 and 8).  Small ones: a dozen round trips one after another (4 x 32,000: 10.5 us).
- * The next batch's loads ahead of this one's work changed nothing: waves of other
- * workgroups fill that time.
+ * Bounds.  Large calls: reads, with what starts and ends a workgroup (512 x 262,144, 1 of 20
+ * allowed: 126 us, 4.4 TB/s; with a list and barriers common to the waves and every logit
+ * summed 145).  Calls that fit the chip once: the chain of a slice and the merge (64 x
+ * 151,936 with penalties 33 us, of which 20 a slice's at the median, 28 at the last, 5 the
+ * merge's; 128 x 50,257 in groups of 16 24.3, 16 and 8).  Small ones: a dozen round trips
+ * one after another (4 x 32,000: 10.5 us).  The next batch's loads ahead of this one's work
+ * changed nothing: other workgroups' waves fill that time.
  */
 #include "dlk_device.h"
 #include "beam_select.h"
@@ -28,7 +31,9 @@
 
 namespace dlk {
 
-constexpr int kBeamList = 512;         /* entries that a workgroup orders at once */
+constexpr int kBeamList = 512;         /* entries that a merge orders at once */
+constexpr int kBeamWaveList = 256;     /* and that a wave lists of a slice */
+constexpr int kBeamPacked = 512;       /* of a wave's 1,024 logits: so many allowed ones or fewer are packed */
 
 DLK_DEV void bpub64(uint64_t *a, uint64_t v) { __hip_atomic_store(a, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 DLK_DEV uint64_t bget64(const uint64_t *a) {
@@ -117,6 +122,17 @@ DLK_DEV uint32_t wave_rth(uint32_t a, int r) {
     return K;
 }
 
+/* Lane's place among the lanes of `who`, from `first` on. */
+DLK_DEV int place_in(uint64_t who, int first) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, (uint32_t)first));
+}
+
+/* LDS that only this wave writes and reads: its instructions go in order, the compiler has to keep it. */
+DLK_DEV void wave_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+}
+
 /* Maximum over each row of 16 lanes (every lane gets its row's). */
 DLK_DEV float row_max(float v) {
     v = fmaxf(v, shfl_xor(v, 1));
@@ -126,15 +142,20 @@ DLK_DEV float row_max(float v) {
 }
 
 struct BeamShared {
-    __align__(16) uint64_t key[kBeamList];      /* merge: keys; slice: entries */
-    uint64_t ent[kBeamList];
+    union {
+        __align__(16) uint64_t list[kBeamThreads / 64][kBeamWaveList];      /* slice: each wave's entries */
+        struct {
+            uint64_t key[kBeamList];            /* merge: keys and entries */
+            uint64_t ent[kBeamList];
+        };
+    };
     double base[DLK_MAX_BEAMS];         /* per row of the group: log-sum, norm, score, maximum */
     double norm[DLK_MAX_BEAMS];
     double part[kBeamThreads / 64];
     float cum[DLK_MAX_BEAMS];
     float top[DLK_MAX_BEAMS];
     uint32_t wave_key[kBeamThreads / 64];
-    int wave_n[kBeamThreads / 64];
+    int wave_n[kBeamThreads / 64], wave_listed[kBeamThreads / 64];
     int place[kBeamList];               /* row of each entry */
     int kind[DLK_MAX_BEAMS];            /* 0: none, 1: by its lists, 2: finished */
     int count, last;
@@ -199,9 +220,9 @@ DLK_DEV void write_none(const BeamParams &p, int g, int j) {
     if (p.out_finished) p.out_finished[o] = 0;
 }
 
-/* The group's lists merged, by its last workgroup.  Up to one list per thread (256) and 16
- * entries of them all per thread (4,096) the slots and entries are asked for at once: a
- * round trip to the other workgroups' words is most of what a merge takes. */
+/* The group's lists (256 at most, one per thread) merged, by its last workgroup.  The slots are
+ * asked for at once, up to 16 entries per thread (4,096 in all) the entries too: a round trip
+ * to the other workgroups' words is most of what a merge takes. */
 DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
     constexpr int T = kBeamThreads, PRE = 16, AT_ONCE = 8;
     const int t = threadIdx.x, lane = lane_id(), wave = wave_id(), g = p.g0 + gl;
@@ -211,9 +232,9 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
     /* list i is that of (row i / slices, slice i % slices).  List or entry i goes to thread
      * (i % 4) * 64 + i / 4 % 64, so that the waves share few of them evenly */
     const int mine = (t & 63) * 4 + (t >> 6);
-    const bool once = L <= T, flat = once && E <= PRE * T;
+    const bool flat = E <= PRE * T;
     uint64_t pre[PRE];
-    if (once && t < L) {
+    if (t < L) {
         sh.key[t] = bget64(&slots[t].sum);
         sh.ent[t] = bget64(&slots[t].max_kept);
     }
@@ -233,7 +254,7 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
         bool bad = false;
         for (int s = sub; b < p.beams && s < p.slices; s += width) {
             const int i = b * p.slices + s;
-            const uint64_t sm = once ? sh.key[i] : bget64(&slots[i].sum), mk = once ? sh.ent[i] : bget64(&slots[i].max_kept);
+            const uint64_t sm = sh.key[i], mk = sh.ent[i];
             const float m = u2f((uint32_t)(mk >> 32));
             bad |= (uint32_t)mk == 0xffffffffu;
             if (m > -INFINITY) {
@@ -324,28 +345,21 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
             add(BeamRow(sh, b).key(pre[q]), pre[q], b);
         }
     } else {
-        uint64_t head = 0;
-        for (int i = mine; i < L; i += T) {
-            const int b = i / p.slices;
-            if (listed(i, b, bget64(&slots[i].max_kept)) > 0) head = max(head, BeamRow(sh, b).key(entry(i, b, 0)));
-        }
-        const uint32_t bound = bound_of((uint32_t)(head >> 32));
-        for (int i = mine; i < L; i += T) {
-            const int b = i / p.slices, n = listed(i, b, bget64(&slots[i].max_kept));
-            if (n == 0) continue;
-            const BeamRow row(sh, b);
-            bool more = true;
-            for (int j = 0; more && j < n; j += AT_ONCE) {
-                uint64_t e[AT_ONCE];                         /* the next few entries, in one round trip */
+        /* by lists, which are in order: what a list's first entry does not reach it has none of */
+        const int i = min(mine, L - 1), b = i / p.slices, n = mine < L ? listed(i, b, sh.ent[i]) : 0;
+        const BeamRow row(sh, b);
+        const uint32_t bound = bound_of(n > 0 ? (uint32_t)(row.key(entry(i, b, 0)) >> 32) : 0);
+        bool more = true;
+        for (int j = 0; more && j < n; j += AT_ONCE) {
+            uint64_t e[AT_ONCE];                             /* the next few entries, in one round trip */
 #pragma unroll
-                for (int q = 0; q < AT_ONCE; q++) e[q] = j + q < n ? entry(i, b, j + q) : 0;
+            for (int q = 0; q < AT_ONCE; q++) e[q] = j + q < n ? entry(i, b, j + q) : 0;
 #pragma unroll
-                for (int q = 0; q < AT_ONCE; q++) {
-                    if (!more || j + q >= n) break;
-                    const uint64_t k = row.key(e[q]);
-                    more = (uint32_t)(k >> 32) >= bound;     /* (the list is in order) */
-                    if (more) add(k, e[q], b);
-                }
+            for (int q = 0; q < AT_ONCE; q++) {
+                if (!more || j + q >= n) break;
+                const uint64_t k = row.key(e[q]);
+                more = (uint32_t)(k >> 32) >= bound;
+                if (more) add(k, e[q], b);
             }
         }
     }
@@ -365,24 +379,14 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
     } else {
         /* too many at or above the bound (few lists for n, or runs of equal keys): the best of the
          * lists' next entries, n times */
-        uint8_t *next = (uint8_t *)sh.key;                   /* each list's; L is 319 at most */
-        uint64_t bk, be;
-        int bi, bl = 0;
-        auto best_of_mine = [&]() {
-            bk = be = 0;
-            bi = -1;
-            for (int i = mine; i < L; i += T) {
-                const int b = i / p.slices, q = next[i];
-                if (q >= listed(i, b, bget64(&slots[i].max_kept))) continue;
-                const uint64_t e = entry(i, b, q), k = BeamRow(sh, b).key(e);
-                if (bi < 0 || before(k, b, e, bk, bi, be)) { bk = k; be = e; bi = b; bl = i; }
-            }
-        };
-        for (int i = mine; i < L; i += T) next[i] = 0;
-        best_of_mine();
+        const int i = min(mine, L - 1), b = i / p.slices;
+        const int n = mine < L ? listed(i, b, bget64(&slots[i].max_kept)) : 0;
+        const BeamRow row(sh, b);
+        int q = 0;
+        uint64_t be = n > 0 ? entry(i, b, 0) : 0, bk = row.key(be);
         for (int j = 0; j < p.n; j++) {
             uint64_t k = bk, e = be;
-            int r = bi;
+            int r = q < n ? b : -1;
             for (int m = 1; m < 64; m <<= 1) {
                 const uint64_t ok = shfl_xor(k, m), oe = shfl_xor(e, m);
                 const int oi = shfl_xor(r, m);
@@ -402,26 +406,31 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
                 if (r >= 0) write_continuation(p, sh, g, j, r, e);
                 else write_none(p, g, j);
             }
-            if (bi >= 0 && bi == r && be == e) {             /* (an id of a row is in one list) */
-                next[bl]++;
-                best_of_mine();
+            if (q < n && b == r && be == e) {                /* (an id of a row is in one list) */
+                q++;
+                be = q < n ? entry(i, b, q) : 0;
+                bk = row.key(be);
             }
         }
     }
 }
 
-/* A slice in p.batches batches of four groups of four logits per thread. */
+/* A slice of a row: its share of the row's p.batches batches of four groups of four logits per
+ * thread (shares differ by one batch at most). */
 template <bool HIST>
 __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams p) {
     constexpr int T = kBeamThreads, GR = 4, B = kBeamBatch;
     __shared__ BeamShared sh;
+    __shared__ __align__(16) float packed[T / 64][kBeamPacked];
+    static_assert(sizeof(packed) >= sizeof(sh.list), "room for the lists side by side");
     __shared__ __align__(16) uint32_t times[HIST ? B / 2 : 4];               /* occurrences, 16 bits an id */
     const int t = threadIdx.x, lane = lane_id(), wave = wave_id();
     const int slice = blockIdx.x % p.slices, rl = blockIdx.x / p.slices;      /* rl: row of the launch */
     const int64_t row = (int64_t)p.g0 * p.beams + rl;
     const float *lg = p.logits + row * p.ld;
     const uint32_t *mw = p.mask ? p.mask + (int64_t)(p.mask_row ? p.mask_row[row] : row) * p.mask_ld : nullptr;
-    const int s0 = slice * p.batches * B, s1 = (int)min((int64_t)p.V, (int64_t)s0 + (int64_t)p.batches * B);
+    const int s0 = slice * p.batches / p.slices * B;
+    const int s1 = (int)min((int64_t)p.V, (int64_t)((slice + 1) * p.batches / p.slices) * B);
     float x[GR][4];
     auto load = [&](int b0) {
         int t4 = t * 4;
@@ -461,12 +470,42 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
     double sum = 0.0;
     uint32_t kept = 0;
     if (!idle) {
-        if (t == 0) sh.count = 0;
-        int32_t id0 = -1, id1 = -1;                /* the first ids, in registers for every batch */
+        uint64_t *list = sh.list[wave];
+        int listed = 0;
+        /* The history's ids among this wave's logits, a lane each, penalised once and put into their
+         * places batch by batch; more than 64 are counted in LDS in each batch. */
+        auto of_wave = [&](int32_t id) { return id >= s0 && id < s1 && (((id - s0) >> 8) & 3) == wave; };
+        int said = 0;
+        int32_t mine = -1;
+        float becomes = 0.0f;                      /* that id's logit with its penalties */
         if (HIST && hn > 0) {
             for (int i = t; i < B / 8; i += T) ((uint4 *)times)[i] = make_uint4(0, 0, 0, 0);
-            if (t < hn) id0 = hist[t];
-            if (t + T < hn) id1 = hist[t + T];
+            int32_t *some = (int32_t *)packed[wave];
+#pragma unroll 1
+            for (int i0 = 0; i0 < hn; i0 += 256) {
+                int32_t id[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) id[k] = hist[min(i0 + 64 * k + lane, hn - 1)];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const bool take = i0 + 64 * k + lane < hn && of_wave(id[k]);
+                    const uint64_t who = ballot(take);
+                    const int at = place_in(who, said);
+                    if (take && at < 64) some[at] = id[k];
+                    said += (int)__popcll(who);
+                }
+            }
+            wave_order();
+            if (lane < said && said <= 64) {
+                mine = some[lane];
+                becomes = lg[mine];
+            }
+            if (said <= 64) {
+                int cnt = 0;
+#pragma unroll 1
+                for (int k = 0; k < said; k++) cnt += __builtin_amdgcn_readlane(mine, k) == mine ? 1 : 0;
+                if (mine >= 0) becomes = beam_penalised(p, becomes, cnt);
+            }
             __syncthreads();
         }
         float most = -INFINITY;                    /* this thread's maximum, and its sum of exp(l - that) */
@@ -474,6 +513,13 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
         bool bad = false;
         float least = -INFINITY;                   /* bound: n entries of the slice reach it (as a logit, and exactly) */
         uint64_t bound = 0;
+        /* lists the lanes' entries side by side (past the list's end they are counted) */
+        auto put = [&](bool take, uint64_t e) {
+            const uint64_t who = ballot(take);
+            const int at = place_in(who, listed);
+            if (take && at < kBeamWaveList) list[at] = e;
+            listed += (int)__popcll(who);
+        };
         for (int b0 = s0; b0 < s1; b0 += B) {
             int t4 = t * 4;
             asm volatile("" : "+v"(t4));
@@ -489,14 +535,25 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
                     for (int c = 0; c < 4; c++) x[j][c] = allowed_or_ninf(x[j][c], bits[j], c);
                 }
             }
-            if (HIST && hn > 0) {
-                auto occurs = [&](int32_t id) {
-                    if (id >= b0 && id < s1 && id - b0 < B) atomicAdd(&times[(id - b0) >> 1], 1u << (16 * (id & 1)));
-                };
-                occurs(id0);
-                occurs(id1);
-                for (int i = t + 2 * T; i < hn; i += T) occurs(hist[i]);
-                __syncthreads();
+            auto in_batch = [&](int32_t id) { return id >= b0 && id < s1 && id - b0 < B; };
+            if (HIST && said > 0 && said <= 64) {
+                for (uint64_t who = ballot(in_batch(mine)); who; who &= who - 1) {
+                    const int k = __builtin_ctzll(who);
+                    const int at = __builtin_amdgcn_readlane(mine, k) - b0;
+                    const float y = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(becomes), k));
+                    const bool here = lane == (at >> 2 & 63);
+#pragma unroll
+                    for (int q = 0; q < 4 * GR; q++) {
+                        float &v = x[q >> 2][q & 3];
+                        v = here && q == ((at >> 10) << 2 | (at & 3)) && v != -INFINITY ? y : v;
+                    }
+                }
+            } else if (HIST && said > 64) {
+                for (int i = lane; i < hn; i += 64) {
+                    const int32_t id = hist[i];
+                    if (in_batch(id) && of_wave(id)) atomicAdd(&times[(id - b0) >> 1], 1u << (16 * (id & 1)));
+                }
+                wave_order();
 #pragma unroll
                 for (int j = 0; j < GR; j++) {
                     const uint2 w = ((const uint2 *)times)[j * T + t];
@@ -534,42 +591,64 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
                 if (k != 0) least = key_value(~k);           /* (0: every continuation is an entry) */
                 bound = (uint64_t)k << 32;
             }
-            const int had = b0 == s0 ? 0 : sh.count;          /* (in the first batch others may be adding to it) */
-            if (b0 != s0) __syncthreads();                   /* (everyone has read it) */
-            if (best >= least) {
+            const int had = listed;
+            if (ballot(best >= least) != 0) {
                 uint32_t at_least = 0;                       /* bit 4 j + c */
 #pragma unroll
                 for (int j = 0; j < GR; j++)
 #pragma unroll
                     for (int c = 0; c < 4; c++) at_least |= x[j][c] >= least && x[j][c] > -INFINITY ? 1u << (4 * j + c) : 0u;
-                for (; at_least; at_least &= at_least - 1) {
-                    const int k = __builtin_ctz(at_least);
+                while (ballot(at_least != 0) != 0) {
+                    const int k = at_least != 0 ? __builtin_ctz(at_least) : 0;
                     float v = x[0][0];
 #pragma unroll
                     for (int q = 1; q < 4 * GR; q++) v = k == q ? x[q >> 2][q & 3] : v;
                     const uint64_t e = entry_of(v, b0 + (k >> 2) * T * 4 + t4 + (k & 3));
-                    if (e >= bound) {
-                        const int at = atomicAdd(&sh.count, 1);
-                        if (at < kBeamList) sh.key[at] = e;
-                    }
+                    put(at_least != 0 && e >= bound, e);
+                    at_least &= at_least - 1;
                 }
             }
             /* (-inf counts as exp(-700) of the maximum: nothing) */
-            const float to = fmaxf(fmaxf(most, best), -3.40282347e38f);
+            const float up_to = mw ? wave_max_dpp(best) : best;
+            const float to = fmaxf(fmaxf(most, up_to), -3.40282347e38f);
             double s = 0.0;
+            int live = 64 * 4 * GR;
+            uint64_t who[4 * GR];
+            if (mw) {
+                live = 0;
 #pragma unroll
-            for (int j = 0; j < GR; j++) {
+                for (int q = 0; q < 4 * GR; q++) {
+                    who[q] = ballot(x[q >> 2][q & 3] > -INFINITY);
+                    live += (int)__popcll(who[q]);
+                }
+            }
+            if (live <= kBeamPacked) {
+                /* few allowed: those of the wave, side by side */
+                float *side = packed[wave];
+                int at = 0;
 #pragma unroll
-                for (int c = 0; c < 4; c++) s += exp_neg((double)x[j][c] - (double)to);
-                asm volatile("" : "+v"(s));                  /* (here and in order, not past the barrier below) */
+                for (int q = 0; q < 4 * GR; q++) {
+                    const int to_place = place_in(who[q], at);
+                    if (x[q >> 2][q & 3] > -INFINITY) side[to_place] = x[q >> 2][q & 3];
+                    at += (int)__popcll(who[q]);
+                }
+                wave_order();
+#pragma unroll 1
+                for (int i = lane; i - lane < live; i += 64) s += exp_neg((double)(i < live ? side[i] : -INFINITY) - (double)to);
+                wave_order();
+            } else {
+#pragma unroll
+                for (int j = 0; j < GR; j++) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++) s += exp_neg((double)x[j][c] - (double)to);
+                    asm volatile("" : "+v"(s));              /* (here and in order: all at once they spill) */
+                }
             }
             part = part * exp_neg((double)most - (double)to) + s;
-            most = fmaxf(most, best);
-            __syncthreads();
-            const int C = sh.count;
-            if (DLK_COLD(C > kBeamList)) {
-                /* more than the list takes: of this batch only its n largest (there is room for them,
-                 * below), found bit by bit: the n-th largest value, then the last place of that value */
+            most = fmaxf(most, up_to);
+            if (DLK_COLD(listed > kBeamWaveList)) {
+                /* more than the list takes: of this batch only the wave's n largest (there is room for
+                 * them, below), found bit by bit: the n-th largest value, then the last place of it */
                 auto count = [&](auto holds) {
                     int c = 0;
 #pragma unroll
@@ -578,15 +657,8 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
                         for (int q = 0; q < 4; q++) {
                             float v = x[j][q];
                             asm volatile("" : "+v"(v));      /* (made anew each time: kept, the keys are registers) */
-                            c += v > -INFINITY && holds(~desc_key(v), j * T * 4 + t4 + q) ? 1 : 0;
+                            c += (int)__popcll(ballot(v > -INFINITY && holds(~desc_key(v), j * T * 4 + t4 + q)));
                         }
-                    c = wave_sum_i32(c);
-                    __syncthreads();
-                    if (lane == 0) sh.wave_n[wave] = c;
-                    __syncthreads();
-                    c = sh.wave_n[0];
-#pragma unroll
-                    for (int w = 1; w < T / 64; w++) c += sh.wave_n[w];
                     return c;
                 };
                 uint32_t value = 0;
@@ -600,32 +672,34 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
                     if (count([&](uint32_t k, int i) { return k == value && i < place + bit; }) < need) place += bit;
                 uint64_t nth = (uint64_t)value << 32 | (uint32_t)~(b0 + place);
                 nth = max(nth, bound);
-                if (t == 0) sh.count = had;
-                __syncthreads();
+                listed = had;
 #pragma unroll
                 for (int j = 0; j < GR; j++)
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
                         const uint64_t e = entry_of(x[j][c], b0 + j * T * 4 + t4 + c);
-                        if (x[j][c] > -INFINITY && e >= nth) sh.key[atomicAdd(&sh.count, 1)] = e;      /* at most n */
+                        put(x[j][c] > -INFINITY && e >= nth, e);                   /* n at most */
                     }
-                __syncthreads();
             }
-            if (DLK_COLD(sh.count > kBeamList - DLK_MAX_BEAMS) && b0 + B < s1) {
+            if (DLK_COLD(listed > kBeamWaveList - DLK_MAX_BEAMS) && b0 + B < s1) {
                 /* the list's n largest, in order, and the last of them as the bound from here on */
-                const int c0 = sh.count;
-#pragma unroll 1
-                for (int i = t; i < c0; i += T) {
-                    const uint64_t e = sh.key[i];
+                uint64_t e[kBeamWaveList / 64];
+                int rank[kBeamWaveList / 64];
+                wave_order();
+#pragma unroll
+                for (int k = 0; k < kBeamWaveList / 64; k++) {
+                    const int i = lane + 64 * k;
                     int equal;
-                    const int rank = rank_in(sh.key, c0, e, equal);
-                    if (rank < p.n) sh.ent[rank] = e;
+                    e[k] = list[min(i, listed - 1)];
+                    rank[k] = i < listed ? rank_in(list, listed, e[k], equal) : p.n;
                 }
-                __syncthreads();
-                for (int i = t; i < p.n; i += T) sh.key[i] = sh.ent[i];
-                if (t == 0) sh.count = p.n;
-                __syncthreads();
-                bound = sh.key[p.n - 1];
+                wave_order();
+#pragma unroll
+                for (int k = 0; k < kBeamWaveList / 64; k++)
+                    if (rank[k] < p.n) list[rank[k]] = e[k];
+                wave_order();
+                listed = p.n;
+                bound = max(bound, list[p.n - 1]);
                 least = entry_logit(bound);
             }
         }
@@ -634,6 +708,7 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
         if (lane == 0) {
             sh.top[wave] = wtop;
             sh.wave_n[wave] = bad;
+            sh.wave_listed[wave] = listed;
         }
         __syncthreads();
         top = sh.top[0];
@@ -649,17 +724,26 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
         } else if (top > -INFINITY) {
             const double s = wave_incl_scan_d(part * exp_neg((double)fmaxf(most, -3.40282347e38f) - (double)top));
             if (lane == 63) sh.part[wave] = s;
+            /* the waves' lists in one */
+            uint64_t *joint = (uint64_t *)packed;
+            int first = 0, all = 0;
+#pragma unroll
+            for (int w = 0; w < T / 64; w++) {
+                const int c = sh.wave_listed[w];
+                first += w < wave ? c : 0;
+                all += c;
+            }
+            for (int a = lane; a < listed; a += 64) joint[first + a] = list[a];
             __syncthreads();
             sum = sh.part[0];
 #pragma unroll
             for (int w = 1; w < T / 64; w++) sum += sh.part[w];
-            const int C = sh.count;
-            kept = (uint32_t)min(C, p.n);
+            kept = (uint32_t)min(all, p.n);
             uint64_t *out = p.cands + ((int64_t)rl * p.slices + slice) * p.n;
-            for (int a = t; a < C; a += T) {
-                const uint64_t e = sh.key[a];
+            for (int a = t; a < all; a += T) {
+                const uint64_t e = joint[a];
                 int equal;
-                const int rank = rank_in(sh.key, C, e, equal);
+                const int rank = rank_in(joint, all, e, equal);
                 if (rank < p.n) bpub64(&out[rank], e);
             }
         }

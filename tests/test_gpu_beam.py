@@ -272,6 +272,39 @@ def test_select_few_and_equal_entries(cuda, beams, n_out, V):
     check(torch, lg, beams, n_out, scores=ahead)
 
 
+@pytest.mark.parametrize("n_out", [3, 64])
+def test_select_long_slices(cuda, n_out):
+    """Slices of several batches: each better than the last, or worse; equal ones; masks of all densities; histories of
+    a few ids to a slice and of many in one place."""
+    import torch
+    rng = np.random.default_rng(n_out)
+    V, rows = 70001, 64
+    lg = logits(rng, rows, V)
+    up = np.sort(lg, axis=1)
+    check(torch, up, 64, n_out)
+    check(torch, up[:, ::-1].copy(), 64, n_out)
+    check(torch, np.round(lg * 2) / 2, 64, n_out)
+    check(torch, np.round(up), 64, n_out)
+    dense = np.concatenate([[0.0, 0.001, 1.0], np.linspace(0.02, 0.98, 61)])
+    allow = rng.random((rows, V)) < dense[:, None]
+    allow[5, 20000:] = False
+    hidden = np.where(allow | (rng.random((rows, V)) < 0.9), lg, np.float32(np.nan))
+    check(torch, hidden, 64, n_out, mask=mask_of(allow))
+    best = np.argsort(-lg, axis=1)
+    hists = [np.concatenate([rng.integers(-1, V + 1, 300), best[r, :40]]) for r in range(rows)]
+    hists[3] = rng.integers(4096, 4300, 900)
+    hists[4] = np.concatenate([np.arange(256, 512), np.arange(256, 300)])
+    hists[6] = [best[6, 0]] * 64
+    hists[7] = [best[7, 0]] * 65
+    kw = dict(hists=hists, rep=1.2, freq=0.2, pres=0.1)
+    check(torch, lg, 64, n_out, **kw)
+    check(torch, hidden, 64, n_out, mask=mask_of(allow), **kw)
+    lg[9, best[9, 0]] = np.nan
+    lg[10, best[10, 3]] = np.inf
+    lg[11, best[11, 5]] = -np.inf
+    check(torch, lg, 64, n_out, **kw)
+
+
 def test_select_all_finished(cuda):
     """A group whose beams have all ended keeps them, ordered by their normalised scores."""
     import torch
