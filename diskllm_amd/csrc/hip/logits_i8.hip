@@ -127,15 +127,20 @@ DLK_DEV void write_logits(const I8Params &p, const i4 (&acc)[MF][NF], int m0, in
     for (int f = 0; f < NF; f++)
 #pragma unroll
         for (int c = 0; c < 4; c++) ws[f][c] = p.w_scale[min(v0 + f * 16 + lk * 4 + c, p.vocab - 1)];
+    float sx[MF];
+#pragma unroll
+    for (int m = 0; m < MF; m++) sx[m] = p.x_scale[min(m0 + m * 16 + lr, p.rows - 1)];
+    /* (here, before the first store: waited for later, a load waits for the stores before it too) */
+#pragma unroll
+    for (int m = 0; m < MF; m++) asm volatile("" : "+v"(sx[m]));
 #pragma unroll
     for (int m = 0; m < MF; m++) {
-        const float sx = p.x_scale[min(m0 + m * 16 + lr, p.rows - 1)];
 #pragma unroll
         for (int f = 0; f < NF; f++) {
             float y[4];
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-                y[c] = (float)acc[m][f][c] * sx * ws[f][c];
+                y[c] = (float)acc[m][f][c] * sx[m] * ws[f][c];
                 if (CAP) y[c] = capped(y[c], p.cap, p.recip);
             }
             if (WIDE) *(float4 *)&mine[lr * LD + f * 16 + lk * 4] = make_float4(y[0], y[1], y[2], y[3]);
