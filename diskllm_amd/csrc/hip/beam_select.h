@@ -12,6 +12,8 @@ namespace dlk {
 constexpr int kBeamThreads = 256;
 constexpr int kBeamBatch = kBeamThreads * 16;                   /* logits of a batch: four groups of four per thread */
 
+constexpr int kBeamEntries = kBeamThreads * 16;                  /* entries that a merge takes at once */
+
 /* What a workgroup says of its slice of a row. */
 struct BeamSlot {
     uint64_t sum;        /* sum of exp(l - max) over the slice (double) */
@@ -46,17 +48,23 @@ struct BeamParams {
 };
 
 /* Workgroups for each row of `vocab` logits: some 800 in all (three a CU: beyond that the
- * fixed 2.6 us of each cost more than more waves give), where that leaves eight batches
- * each at most, and 256 to a group at most, whose lists the merge takes in one round trip
- * (us by workgroups a row:
- *   64 x 151,936 with histories   10: 34.4, 12: 34.1, 13: 33.7, 16: 34.9, 20: 36.3
- *   128 x 50,257 in groups of 16  4: 25.0, 6: 24.7, 8: 28.1, 10: 29.4
- *   512 x 262,144 masked          4: 142, 5: 132, 8: 129, 10: 128, 14: 131
- *   4 x 32,000                    4: 13.8, 8: 11.4). */
-inline int beam_slices(int64_t rows, int beams, int vocab) {
-    const int64_t batches = ((int64_t)vocab + kBeamBatch - 1) / kBeamBatch;
+ * fixed 2.6 us of each cost more than more waves give), where that leaves five batches each
+ * at most; but no more than give a group 4,096 entries, which its merge takes in one round
+ * trip, unless each had more than eight batches then; and 256 to a group (us by workgroups a row:
+ *   64 x 151,936 with histories        10: 34.4, 12: 34.1, 13: 33.7, 16: 34.9, 20: 36.3
+ *   128 x 50,257, groups of 16         4: 25.0, 6: 24.7, 8: 28.1, 10: 29.4
+ *   512 x 262,144                      8: 141, 11: 143, 13: 142, 16: 146, 21: 153
+ *   512 x 262,144 masked               4: 142, 5: 132, 8: 129, 10: 128, 14: 131
+ *   256 x 128,256, 16 beams, 32 out    4: 86.7, 6: 74.6, 8: 65.1, 10: 72.9, 16: 103
+ *   48 x 151,936, 12 beams, 24 out     8: 37.1, 10: 36.7, 13: 29.5, 16: 37.8
+ *   16 x 128,256, 16 beams, 32 out     4: 62.5, 7: 36.9, 8: 34.7, 16: 39.3
+ *   4 x 32,000                         4: 13.8, 8: 11.4). */
+inline int beam_slices(int64_t rows, int beams, int n_out, int vocab) {
+    const int64_t batches = ((int64_t)vocab + kBeamBatch - 1) / kBeamBatch, least = (batches + 7) / 8;
+    const int64_t once = kBeamEntries / (beams * n_out);
     int64_t s = (800 + rows / 2) / rows;
-    if (s < (batches + 7) / 8) s = (batches + 7) / 8;
+    if (s < (batches + 4) / 5) s = (batches + 4) / 5;
+    if (s > once) s = once > least ? once : least;
     if (s > kBeamThreads / beams) s = kBeamThreads / beams;
     return (int)(s < batches ? s : batches);
 }

@@ -158,6 +158,7 @@ struct BeamShared {
     int wave_n[kBeamThreads / 64], wave_listed[kBeamThreads / 64];
     int place[kBeamList];               /* row of each entry */
     int kind[DLK_MAX_BEAMS];            /* 0: none, 1: by its lists, 2: finished */
+    uint8_t kept[kBeamThreads];         /* entries of each list */
     int count, last;
     uint64_t best_key[kBeamThreads / 64], best_ent[kBeamThreads / 64];
     int best_row[kBeamThreads / 64];
@@ -221,10 +222,10 @@ DLK_DEV void write_none(const BeamParams &p, int g, int j) {
 }
 
 /* The group's lists (256 at most, one per thread) merged, by its last workgroup.  The slots are
- * asked for at once, up to 16 entries per thread (4,096 in all) the entries too: a round trip
- * to the other workgroups' words is most of what a merge takes. */
+ * asked for at once, and 16 entries per thread (4,096) with them: a round trip to the other
+ * workgroups' words is most of what a merge takes. */
 DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
-    constexpr int T = kBeamThreads, PRE = 16, AT_ONCE = 8;
+    constexpr int T = kBeamThreads, PRE = kBeamEntries / T;
     const int t = threadIdx.x, lane = lane_id(), wave = wave_id(), g = p.g0 + gl;
     const int L = p.beams * p.slices, E = L * p.n;
     const BeamSlot *slots = p.slots + (int64_t)gl * L;
@@ -232,17 +233,19 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
     /* list i is that of (row i / slices, slice i % slices).  List or entry i goes to thread
      * (i % 4) * 64 + i / 4 % 64, so that the waves share few of them evenly */
     const int mine = (t & 63) * 4 + (t >> 6);
-    const bool flat = E <= PRE * T;
     uint64_t pre[PRE];
-    if (t < L) {
-        sh.key[t] = bget64(&slots[t].sum);
-        sh.ent[t] = bget64(&slots[t].max_kept);
-    }
-    if (flat) {
+    auto load = [&](int e0) {
 #pragma unroll
         for (int q = 0; q < PRE; q++)
-            if (q * T < E) pre[q] = bget64(&cands[min(q * T + mine, E - 1)]);
+            if (e0 + q * T < E) pre[q] = bget64(&cands[min(e0 + q * T + mine, E - 1)]);
+    };
+    if (t < L) {
+        const uint64_t mk = bget64(&slots[t].max_kept);
+        sh.key[t] = bget64(&slots[t].sum);
+        sh.ent[t] = mk;
+        sh.kept[t] = (uint8_t)mk;
     }
+    load(0);
     if (t == 0) sh.count = 0;
     __syncthreads();
     /* the rows' sums: 16 lanes each where they have 16 slices at most, else a wave each */
@@ -292,12 +295,9 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
     }
     __syncthreads();
     /* list i of row b: its entries (a finished row's first list holds its one continuation) */
-    auto listed = [&](int i, int b, uint64_t max_kept) {
+    auto listed = [&](int i, int b) {
         const int kind = sh.kind[b];
-        return kind == 1 ? (int)(uint32_t)max_kept : kind == 2 && i == b * p.slices ? 1 : 0;
-    };
-    auto entry = [&](int i, int b, int j) -> uint64_t {
-        return sh.kind[b] == 2 ? ~(uint64_t)0 : bget64(&cands[(int64_t)i * p.n + j]);
+        return kind == 1 ? (int)sh.kept[i] : kind == 2 && i == b * p.slices ? 1 : 0;
     };
     auto add = [&](uint64_t k, uint64_t e, int b) {
         const int at = atomicAdd(&sh.count, 1);
@@ -323,45 +323,37 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
         }
         return bound;
     };
-    if (flat) {
-        uint32_t key[PRE], best = 0;                         /* high words, 0: none */
-        const float per_n = 1.0f / (float)p.n, per_slices = 1.0f / (float)p.slices;
-        auto list_of = [&](int at) { return (int)(((float)at + 0.5f) * per_n); };          /* exact: below 2^12 */
-        auto row_of = [&](int i) { return (int)(((float)i + 0.5f) * per_slices); };
+    /* every entry's key for the bound, then those that reach it: PRE * T at a time, which are
+     * kept from one to the other where they are all */
+    uint32_t key[PRE], best = 0, bound = 0;                  /* high words, 0: none */
+    const float per_n = 1.0f / (float)p.n, per_slices = 1.0f / (float)p.slices;
+    auto list_of = [&](int at) { return (int)(((float)at + 0.5f) * per_n); };              /* exact: below 2^15 */
+    auto row_of = [&](int i) { return (int)(((float)i + 0.5f) * per_slices); };
+#pragma unroll 1
+    for (int pass = 0; pass < 2; pass++) {
+#pragma unroll 1
+        for (int e0 = 0; e0 < E; e0 += PRE * T) {
+            if (pass == 0 || E > PRE * T) {
+                if (pass > 0 || e0 > 0) load(e0);
 #pragma unroll
-        for (int q = 0; q < PRE; q++) {                      /* (few entries: few instructions, fetched for the first time) */
-            key[q] = 0;
-            if (q * T >= E) continue;
-            const int at = min(q * T + mine, E - 1), i = list_of(at), b = row_of(i);
-            if (sh.kind[b] == 2) pre[q] = ~(uint64_t)0;
-            if (q * T + mine < E && at - i * p.n < listed(i, b, sh.ent[i])) key[q] = (uint32_t)(BeamRow(sh, b).key(pre[q]) >> 32);
-            best = max(best, key[q]);
-        }
-        const uint32_t bound = bound_of(best);               /* (sh.ent has been read) */
+                for (int q = 0; q < PRE; q++) {              /* (few entries: few instructions, fetched for the first time) */
+                    key[q] = 0;
+                    if (e0 + q * T >= E) continue;
+                    const int at = min(e0 + q * T + mine, E - 1), i = list_of(at), b = row_of(i);
+                    if (sh.kind[b] == 2) pre[q] = ~(uint64_t)0;
+                    if (e0 + q * T + mine < E && at - i * p.n < listed(i, b)) key[q] = (uint32_t)(BeamRow(sh, b).key(pre[q]) >> 32);
+                    best = max(best, key[q]);
+                }
+            }
+            if (pass == 0) continue;
 #pragma unroll
-        for (int q = 0; q < PRE; q++) {
-            if (key[q] == 0 || key[q] < bound) continue;
-            const int b = row_of(list_of(q * T + mine));
-            add(BeamRow(sh, b).key(pre[q]), pre[q], b);
-        }
-    } else {
-        /* by lists, which are in order: what a list's first entry does not reach it has none of */
-        const int i = min(mine, L - 1), b = i / p.slices, n = mine < L ? listed(i, b, sh.ent[i]) : 0;
-        const BeamRow row(sh, b);
-        const uint32_t bound = bound_of(n > 0 ? (uint32_t)(row.key(entry(i, b, 0)) >> 32) : 0);
-        bool more = true;
-        for (int j = 0; more && j < n; j += AT_ONCE) {
-            uint64_t e[AT_ONCE];                             /* the next few entries, in one round trip */
-#pragma unroll
-            for (int q = 0; q < AT_ONCE; q++) e[q] = j + q < n ? entry(i, b, j + q) : 0;
-#pragma unroll
-            for (int q = 0; q < AT_ONCE; q++) {
-                if (!more || j + q >= n) break;
-                const uint64_t k = row.key(e[q]);
-                more = (uint32_t)(k >> 32) >= bound;
-                if (more) add(k, e[q], b);
+            for (int q = 0; q < PRE; q++) {
+                if (key[q] == 0 || key[q] < bound) continue;
+                const int b = row_of(list_of(e0 + q * T + mine));
+                add(BeamRow(sh, b).key(pre[q]), pre[q], b);
             }
         }
+        if (pass == 0) bound = bound_of(best);
     }
     __syncthreads();
     const int C = sh.count;
@@ -379,11 +371,13 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
     } else {
         /* too many at or above the bound (few lists for n, or runs of equal keys): the best of the
          * lists' next entries, n times */
-        const int i = min(mine, L - 1), b = i / p.slices;
-        const int n = mine < L ? listed(i, b, bget64(&slots[i].max_kept)) : 0;
+        const int i = min(mine, L - 1), b = i / p.slices, n = mine < L ? listed(i, b) : 0;
         const BeamRow row(sh, b);
+        auto entry = [&](int q) -> uint64_t {
+            return sh.kind[b] == 2 ? ~(uint64_t)0 : bget64(&cands[(int64_t)i * p.n + q]);
+        };
         int q = 0;
-        uint64_t be = n > 0 ? entry(i, b, 0) : 0, bk = row.key(be);
+        uint64_t be = n > 0 ? entry(0) : 0, bk = row.key(be);
         for (int j = 0; j < p.n; j++) {
             uint64_t k = bk, e = be;
             int r = q < n ? b : -1;
@@ -408,7 +402,7 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
             }
             if (q < n && b == r && be == e) {                /* (an id of a row is in one list) */
                 q++;
-                be = q < n ? entry(i, b, q) : 0;
+                be = q < n ? entry(q) : 0;
                 bk = row.key(be);
             }
         }

@@ -711,7 +711,7 @@ extern "C" int dlk_beam_select(const dlk_beam_batch *b, int groups, int vocab, c
     p.order = prm->penalty_order;
     p.rep = prm->repeat_penalty; p.freq = prm->frequency_penalty; p.pres = prm->presence_penalty;
     p.batches = (int)(((int64_t)vocab + kBeamBatch - 1) / kBeamBatch);
-    p.slices = beam_slices((int64_t)groups * p.beams, p.beams, vocab);
+    p.slices = beam_slices((int64_t)groups * p.beams, p.beams, p.n, vocab);
     /* per group: its rows' slots, then their lists */
     const size_t lists = (size_t)p.beams * p.slices, per = lists * (sizeof(BeamSlot) + (size_t)p.n * 8);
     int64_t most = (int64_t)(kBeamWorkspace / per);
