@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
-from math import prod
 from typing import Optional
 
 import numpy as np
@@ -322,13 +321,34 @@ def beam_state(src: torch.Tensor, dst: Optional[torch.Tensor] = None, row_dim: i
     first `length` entries of dimension length_dim where that is given (the filled part of a cache).  The
     dimensions before the rows, those up to length_dim and those from it on have to be one stride each.  The
     caller keeps the tensors."""
-    shape = list(src.shape)
-    nd = len(shape)
-    rows = shape[row_dim] if row_dim < nd else 0
+    size = src.shape
+    nd = len(size)
     cut = row_dim + 1 if length_dim is None else length_dim
-    _want(0 <= row_dim < nd and (length_dim is None or row_dim < cut < nd), "length_dim: a dimension after the rows is wanted")
-    if length_dim is not None and length is not None:
-        _want(0 <= length <= shape[cut], "length: more than the tensors hold")
+    if not (0 <= row_dim < nd and (length_dim is None or row_dim < cut < nd)):
+        raise ValueError("length_dim: a dimension after the rows is wanted")
+    if length is None or length_dim is None:
+        length = size[cut] if cut < nd else 1
+    elif not 0 <= length <= size[cut]:
+        raise ValueError("length: more than the tensors hold")
+    rows, item = size[row_dim], src.element_size()
+    if dst is None and src.is_contiguous():
+        # by the sizes: strides of single rows or heads may be anything
+        outer = inner = 1
+        for n in size[:row_dim]:
+            outer *= n
+        for n in size[row_dim + 1:cut]:
+            inner *= n
+        entry = item
+        for n in size[cut + 1:]:
+            entry *= n
+        room = entry * size[cut] if cut < nd else entry
+        row = room * inner
+        at, dev = src.data_ptr(), src.get_device()
+        s = _lib.BeamState(at, at, entry * length, row, row * rows, room, row, row * rows, room, outer, inner)
+        s.rows = (rows, rows, dev, dev)
+        return s
+    shape = list(size)
+    if length_dim is not None:
         shape[cut] = length
     dst_rows = rows
     if dst is not None:
@@ -339,15 +359,6 @@ def beam_state(src: torch.Tensor, dst: Optional[torch.Tensor] = None, row_dim: i
         if length_dim is not None and other[cut] >= shape[cut]:
             other[cut] = shape[cut]
         _want(other == shape, "dst: another shape than src's")
-    item = src.element_size()
-    if dst is None and src.is_contiguous():
-        full = src.shape                           # (by the sizes: strides of single rows or heads may be anything)
-        at, row = src.data_ptr(), prod(full[row_dim + 1:]) * item
-        outer, inner = row * rows, prod(full[cut:]) * item
-        s = _lib.BeamState(at, at, prod(shape[cut:]) * item if 0 not in shape else 0, row, outer, inner, row, outer, inner,
-                           prod(shape[:row_dim]), prod(shape[row_dim + 1:cut]))
-        s.rows = (rows, rows, src.get_device(), src.get_device())
-        return s
 
     def layout(t):
         st = t.stride()
@@ -356,9 +367,9 @@ def beam_state(src: torch.Tensor, dst: Optional[torch.Tensor] = None, row_dim: i
         _want(outer is not None and inner is not None and rest is not None and (rest[0] == 1 or rest[1] == 1),
               "strides that are not one per part, or rows whose entries are apart")
         return t.data_ptr(), st[row_dim] * item, outer, inner, rest[0] * item
-    at, row, outer, inner, size = layout(src)
-    d_at, d_row, d_outer, d_inner, _ = (at, row, outer, inner, size) if dst is None else layout(dst)
-    s = _lib.BeamState(at, d_at, 0 if 0 in shape else size, row, outer[1] * item, inner[1] * item, d_row,
+    at, row, outer, inner, width = layout(src)
+    d_at, d_row, d_outer, d_inner, _ = (at, row, outer, inner, width) if dst is None else layout(dst)
+    s = _lib.BeamState(at, d_at, 0 if 0 in shape else width, row, outer[1] * item, inner[1] * item, d_row,
                        d_outer[1] * item, d_inner[1] * item, outer[0], inner[0])
     s.rows = (rows, dst_rows, src.get_device(), src.get_device() if dst is None else dst.get_device())
     return s
@@ -369,10 +380,13 @@ def beam_history(off: torch.Tensor, ids: torch.Tensor, tokens: Optional[torch.Te
     """The rows' histories (CSR) and the tokens to append, for beam_reorder; out_ids has room for max_history ids
     of every new row.  The caller keeps the tensors."""
     dev = off.get_device()
-    at = _flat(off, 0, dev, _I32, "off")
-    h = _lib.BeamHistory(at, _flat(ids, 0, dev, _I32, "ids") or at,
-                         0 if tokens is None else _flat(tokens, 0, dev, _I32, "tokens"), max_history,
-                         _flat(out_off, 0, dev, _I32, "out_off"), _flat(out_ids, 0, dev, _I32, "out_ids"))
+    some = (off, ids, out_off, out_ids) if tokens is None else (off, ids, out_off, out_ids, tokens)
+    for t in some:
+        if t.dtype is not _I32 or t.get_device() != dev or not t.is_contiguous():
+            raise ValueError("history: contiguous values of int32 on one device are wanted")
+    at = off.data_ptr()
+    h = _lib.BeamHistory(at, ids.data_ptr() or at, 0 if tokens is None else tokens.data_ptr(), max_history,
+                         out_off.data_ptr(), out_ids.data_ptr())
     h.sizes = (off.numel(), None if tokens is None else tokens.numel(), out_off.numel(), out_ids.numel(), dev)
     return h
 
