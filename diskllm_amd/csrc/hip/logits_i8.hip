@@ -164,6 +164,21 @@ DLK_DEV void load_to_lds(const int8_t *src, int8_t *dst) {
                                      (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
 }
 
+/* Of a last, shorter step the chunks past n are copies of the last one (so that all lanes load):
+ * this lane's chunk of x at k, once it is in LDS, gets zeros for what is past n.  What w has
+ * there does not matter then. */
+DLK_DEV void end_row(int8_t *chunk, int k, int n) {
+    if (k + 16 <= n) return;
+    i4 v = *(const i4 *)chunk;
+    const int keep = max(n - k, 0);                /* bytes */
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const int b = keep - 4 * c;
+        v[c] = b >= 4 ? v[c] : b <= 0 ? 0 : v[c] & ((1 << (8 * b)) - 1);
+    }
+    *(i4 *)chunk = v;
+}
+
 /* One tile's place: workgroups go to the XCDs in turn, so each XCD gets a run of tiles, the
  * tiles of x for one tile of w side by side: w comes from memory once. */
 template <int BM, int BN>
@@ -215,7 +230,7 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void logits_i8_kernel(I8Params p
     constexpr int CPR = BK / 16, RPI = 64 / CPR;   /* chunks of a row; rows that a wave loads at once */
     constexpr int NI = (BM + BN) / RPI / W;        /* loads of a wave per stage */
     constexpr int STAGE = (BM + BN) * BK;
-    static_assert((BM + BN) % (RPI * W) == 0 && BM % RPI == 0 && BK >= 64 && BK <= 512, "tiles");
+    static_assert((BM + BN) % (RPI * W) == 0 && BM % (RPI * W) == 0 && BK >= 64 && BK <= 512, "tiles");
     __shared__ __align__(1024) int8_t lds[ST * STAGE];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
     int m0, v0;
@@ -229,19 +244,21 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void logits_i8_kernel(I8Params p
         src[j] = r < BM ? p.x + (int64_t)min(m0 + r, p.rows - 1) * p.ldx
                         : p.w + (int64_t)min(v0 + r - BM, p.vocab - 1) * p.ldw;
     }
+    const int last = (p.n - 1) & ~15;              /* (behind a row's end at most the rest of its last chunk is loaded) */
     auto fetch = [&](int it, int slot) {
 #pragma unroll
-        for (int j = 0; j < NI; j++) load_to_lds(src[j] + it * BK + at[j], &lds[slot * STAGE + (j * W + wave) * 1024]);
+        for (int j = 0; j < NI; j++)
+            load_to_lds(src[j] + min(it * BK + at[j], last), &lds[slot * STAGE + (j * W + wave) * 1024]);
     };
     const int wm = wave % WGM * WM, wn = wave / WGM * WN;
     i4 acc[MF][NF];
     clear(acc);
-    const int steps = p.n / BK;
+    const int whole = p.n / BK, steps = (p.n + BK - 1) / BK;
 #pragma unroll
     for (int s = 0; s < ST - 1; s++)
         if (s < steps) fetch(s, s);
     int slot = 0;
-    for (int it = 0; it < steps; it++) {
+    for (int it = 0; it < whole; it++) {
         if (it + ST - 2 < steps) wait_loads<NI *(ST - 2)>();
         else wait_loads<0>();
         __builtin_amdgcn_s_barrier();
@@ -251,17 +268,13 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void logits_i8_kernel(I8Params p
         multiply_stage<BK>(&lds[slot * STAGE + wm * BK], &lds[slot * STAGE + (BM + wn) * BK], acc);
         slot = slot == ST - 1 ? 0 : slot + 1;
     }
-    if (p.n % BK != 0) {                           /* what is left of n, through registers, zeros past it */
+    if (whole < steps) {                           /* a last, shorter step */
+        wait_loads<0>();
+#pragma unroll
+        for (int j = 0; j < BM / (RPI * W); j++)   /* (x's rows are the first loads) */
+            end_row(&lds[slot * STAGE + (j * W + wave) * 1024 + lane * 16], whole * BK + at[j], p.n);
         __syncthreads();
-#pragma unroll 1
-        for (int j = 0; j < NI; j++) {
-            const int r = (j * W + wave) * RPI + lane / CPR;
-            const int8_t *row = r < BM ? p.x + (int64_t)min(m0 + r, p.rows - 1) * p.ldx
-                                       : p.w + (int64_t)min(v0 + r - BM, p.vocab - 1) * p.ldw;
-            *(i4 *)&lds[(j * W + wave) * 1024 + lane * 16] = load16_to(row, steps * BK + place<BK>(r, lane % CPR) * 16, p.n);
-        }
-        __syncthreads();
-        multiply_stage<BK>(&lds[wm * BK], &lds[(BM + wn) * BK], acc);
+        multiply_stage<BK>(&lds[slot * STAGE + wm * BK], &lds[slot * STAGE + (BM + wn) * BK], acc);
     }
     constexpr bool WIDE = NF >= 4;
     static_assert(!WIDE || W * 16 * (WN + 4) * 4 <= ST * STAGE, "room for the output");
@@ -337,22 +350,23 @@ __global__ __launch_bounds__(512, 2) void logits_i8_wide_kernel(I8Params p) {
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
     int m0, v0;
     if (!tile_of<BM, BN>(p, m0, v0)) return;
-    const int8_t *sx[NX], *sw[NW];
+    const int8_t *sx[NX], *sw[NW];                 /* rows (a wave's loads have one row in eight: one place in all) */
+    const int at = place<BK>(lane / 8, lane % 8) * 16;
 #pragma unroll
-    for (int j = 0; j < NX; j++) {
-        const int r = (j * W + wave) * RPI + lane / 8;
-        sx[j] = p.x + (int64_t)min(m0 + r, p.rows - 1) * p.ldx + place<BK>(r, lane % 8) * 16;
-    }
+    for (int j = 0; j < NX; j++) sx[j] = p.x + (int64_t)min(m0 + (j * W + wave) * RPI + lane / 8, p.rows - 1) * p.ldx;
 #pragma unroll
-    for (int j = 0; j < NW; j++) {
-        const int r = (j * W + wave) * RPI + lane / 8;
-        sw[j] = p.w + (int64_t)min(v0 + r, p.vocab - 1) * p.ldw + place<BK>(r, lane % 8) * 16;
-    }
+    for (int j = 0; j < NW; j++) sw[j] = p.w + (int64_t)min(v0 + (j * W + wave) * RPI + lane / 8, p.vocab - 1) * p.ldw;
+    const int last = (p.n - 1) & ~15;              /* (behind a row's end at most the rest of its last chunk is loaded) */
     auto fetch = [&](int it, int slot) {
+        const int k = min(it * BK + at, last);
 #pragma unroll
-        for (int j = 0; j < NX; j++) load_to_lds(sx[j] + it * BK, &lds[slot * XST + (j * W + wave) * 1024]);
+        for (int j = 0; j < NX; j++) load_to_lds(sx[j] + k, &lds[slot * XST + (j * W + wave) * 1024]);
 #pragma unroll
-        for (int j = 0; j < NW; j++) load_to_lds(sw[j] + it * BK, &ldw[slot * WST + (j * W + wave) * 1024]);
+        for (int j = 0; j < NW; j++) load_to_lds(sw[j] + k, &ldw[slot * WST + (j * W + wave) * 1024]);
+    };
+    auto end_rows = [&](int it) {                  /* of a last, shorter step, once this wave's loads are there */
+#pragma unroll
+        for (int j = 0; j < NX; j++) end_row(&lds[(it & 1) * XST + (j * W + wave) * 1024 + lane * 16], it * BK + at, p.n);
     };
     const int lr = lane & 15, lk = lane >> 4, wm = wave % WGM * WM, wn = wave / WGM * WN;
     const int half0 = lr * BK + place<BK>(lr, lk) * 16, half1 = lr * BK + place<BK>(lr, 4 + lk) * 16;
@@ -381,46 +395,34 @@ __global__ __launch_bounds__(512, 2) void logits_i8_wide_kernel(I8Params p) {
         __builtin_amdgcn_sched_barrier(0);
     };
     i4 a0[NF], b0[MF], a1[NF], b1[MF];
-    const int steps = p.n / BK;
-    if (steps > 0) {
-        fetch(0, 0);
-        if (steps > 1) {
-            fetch(1, 1);
-            wait_loads<NX + NW>();
-        } else {
-            wait_loads<0>();
-        }
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        take(a0, b0, 0, half0);
-        for (int it = 0; it < steps; it++) {
-            take(a1, b1, it & 1, half1);
-            multiply(a0, b0);
-            if (it + 1 < steps) {
-                wait_loads<0>();                   /* step it + 1 is there; this wave has read all of step it */
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                if (it + 2 < steps) fetch(it + 2, it & 1);
-                take(a0, b0, (it + 1) & 1, half0);
-            }
-            multiply(a1, b1);
-        }
+    const int steps = (p.n + BK - 1) / BK, shorter = p.n % BK != 0 ? steps - 1 : -1;
+    fetch(0, 0);
+    if (steps > 1) {
+        fetch(1, 1);
+        wait_loads<NX + NW>();
+    } else {
+        wait_loads<0>();
+        if (shorter == 0) end_rows(0);
+        wait_loads<0>();
     }
-    if (p.n % BK != 0) {                           /* what is left of n, through registers, zeros past it */
-        __syncthreads();
-#pragma unroll 1
-        for (int j = 0; j < NX + NW; j++) {
-            const int r = ((j < NX ? j : j - NX) * W + wave) * RPI + lane / 8;
-            const int8_t *row = j < NX ? p.x + (int64_t)min(m0 + r, p.rows - 1) * p.ldx
-                                       : p.w + (int64_t)min(v0 + r, p.vocab - 1) * p.ldw;
-            int8_t *dst = j < NX ? &lds[(j * W + wave) * 1024] : &ldw[((j - NX) * W + wave) * 1024];
-            *(i4 *)&dst[lane * 16] = load16_to(row, steps * BK + place<BK>(r, lane % 8) * 16, p.n);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    take(a0, b0, 0, half0);
+    for (int it = 0; it < steps; it++) {
+        take(a1, b1, it & 1, half1);
+        multiply(a0, b0);
+        if (it + 1 < steps) {
+            wait_loads<0>();                       /* step it + 1 is there; this wave has read all of step it */
+            if (it + 1 == shorter) {
+                end_rows(it + 1);
+                wait_loads<0>();
+            }
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (it + 2 < steps) fetch(it + 2, it & 1);
+            take(a0, b0, (it + 1) & 1, half0);
         }
-        __syncthreads();
-        take(a0, b0, 0, half0);
-        multiply(a0, b0);
-        take(a0, b0, 0, half1);
-        multiply(a0, b0);
+        multiply(a1, b1);
     }
     __syncthreads();
     write_logits<CAP, true>(p, acc, m0 + wm, v0 + wn, (float *)lds + wave * 16 * (WN + 4));
