@@ -11,15 +11,17 @@
  * operands go straight into an LDS ring (global_load_lds, 16 bytes a lane), which costs no
  * registers and no waits but one barrier a step.  16 x 151,936 x 4,096 takes 114-116 us,
  * 5.5-5.7 TB/s (a large copy: 5.1); 1 x 32,000 x 2,048 11.5, 5.7 TB/s.  Above that the
- * products and what feeds them: 512 x 262,144 x 4,096 with the cap in 606-619 us,
- * 1,780-1,810 TOP/s, of which some 150 cap and write 537 MB of logits after each workgroup's
+ * products and what feeds them: 512 x 262,144 x 4,096 with the cap in 606-614 us,
+ * 1,790-1,810 TOP/s, of which some 150 cap and write 537 MB of logits after each workgroup's
  * loop; the loop alone runs at 2,440, as a library product of 16,384^3 does.  It has the
  * loads into LDS at about 12 TB/s, where shorter steps, a third stage of w, another order of n
  * and stores that bypass the caches gave nothing; tiles of 256 x 256 ask for the fewest bytes.
  *
  * Rows that are not 16-byte aligned cannot go that way: they go through registers
- * (logits_i8_any_kernel; 33 x 50,257 x 2,047 33.5 us, 3.3 TB/s: each 16-byte load touches two
- * lines' worth of requests, and half the bytes are in flight).
+ * (logits_i8_any_kernel; 33 x 50,257 x 2,047 33.5 us, 3.3 TB/s, in padded rows 27).  Their
+ * 16-byte loads are what it waits for: both stages wholly in flight (no branch in the loop) or
+ * steps twice as long were no faster, nor was loading the rows' own chunks into LDS and
+ * reading fragments at each row's shift (59 us: unaligned LDS reads).
  */
 #include <float.h>
 #include <math.h>
