@@ -16,9 +16,8 @@
  * 5.1 to 5.6 TB/s, read and written.  A request's few small states: 4-5 us (13.5 with the
  * host's checks of the tensors), all of them and the histories in one launch.
  *
- * A history's place in the CSR is the sum of the lengths before it, which each row's
- * workgroup sums anew (rows of a batch are few: 4,096 are 16 loads a thread) rather than
- * waiting for another's.
+ * A history's place in the CSR is the sum of the lengths before it, which the workgroups of
+ * few rows sum anew each rather than wait for another's.
  */
 #include <hip/hip_runtime.h>
 
@@ -31,6 +30,10 @@ namespace dlk {
 
 constexpr int kMoveThreads = 256;
 constexpr int kMoveStates = 8;                   /* states of one launch */
+/* Up to so many rows each history's workgroup sums the lengths before it, past that a launch
+ * of one workgroup does (us, summed and launched: 1,024 rows 5.4, 7.2; 2,048 9.4, 8.3; 4,096
+ * 20.8, 12.5; 65,536 2,782, 158). */
+constexpr int64_t kMoveSummed = 1536;
 constexpr int64_t kMoveBlocks = 0xffffff;        /* workgroups of one launch: 2^32 threads and over are refused */
 
 typedef uint32_t u4_any __attribute__((ext_vector_type(4), aligned(1)));
@@ -53,6 +56,7 @@ struct MoveParams {
     const int32_t *off, *ids, *tokens;
     int32_t *out_off, *out_ids;
     int keep;
+    int offsets;                                 /* out_off is there already (history_offsets_kernel) */
 };
 
 /* The row that new row r takes, -1 where its parent is none of its group's. */
@@ -74,21 +78,54 @@ DLK_DEV void move_history(const MoveParams &p, int64_t r) {
     const int t = threadIdx.x;
     int64_t before = 0;
     int q;
-    for (int64_t i = t; i < r; i += kMoveThreads) before += new_length(p, i, q);
-    for (int m = 1; m < 64; m <<= 1) before += shfl_xor(before, m);
-    if (lane_id() == 0) part[wave_id()] = before;
-    __syncthreads();
-    before = part[0] + part[1] + part[2] + part[3];
     const int n = new_length(p, r, q);
-    if (t == 0) {
-        p.out_off[r] = (int32_t)before;
-        if (r == (int64_t)p.groups * p.n_out - 1) p.out_off[r + 1] = (int32_t)(before + n);
+    if (p.offsets) {
+        before = p.out_off[r];
+    } else {
+        int other;
+        for (int64_t i = t; i < r; i += kMoveThreads) before += new_length(p, i, other);
+        for (int m = 1; m < 64; m <<= 1) before += shfl_xor(before, m);
+        if (lane_id() == 0) part[wave_id()] = before;
+        __syncthreads();
+        before = part[0] + part[1] + part[2] + part[3];
+        if (t == 0) {
+            p.out_off[r] = (int32_t)before;
+            if (r == (int64_t)p.groups * p.n_out - 1) p.out_off[r + 1] = (int32_t)(before + n);
+        }
     }
     if (n == 0) return;
     const int add = p.tokens && p.tokens[r] >= 0 ? 1 : 0;
     const int32_t *from = p.ids + p.off[q + 1] - (n - add);
     int32_t *to = p.out_ids + before;
     for (int i = t; i < n; i += kMoveThreads) to[i] = i < n - add ? from[i] : p.tokens[r];
+}
+
+/* The new histories' offsets, by one workgroup (their sum fits 31 bits). */
+__global__ __launch_bounds__(1024) void history_offsets_kernel(MoveParams p) {
+    __shared__ int part[16];
+    const int t = threadIdx.x, lane = lane_id(), wave = wave_id();
+    const int64_t rows = (int64_t)p.groups * p.n_out;
+    int before = 0;
+    for (int64_t r0 = 0; r0 < rows; r0 += 1024) {
+        int q;
+        const int n = r0 + t < rows ? new_length(p, r0 + t, q) : 0;
+        int upto = n;
+        for (int m = 1; m < 64; m <<= 1) {
+            const int o = __shfl_up(upto, m);
+            upto += lane >= m ? o : 0;
+        }
+        if (lane == 63) part[wave] = upto;
+        __syncthreads();
+        int waves = 0;
+        for (int w = 0; w < 16; w++) {
+            upto += w < wave ? part[w] : 0;
+            waves += part[w];
+        }
+        if (r0 + t < rows) p.out_off[r0 + t] = before + upto - n;
+        before += waves;
+        __syncthreads();
+    }
+    if (t == 0) p.out_off[rows] = before;
 }
 
 /* NB: the rows whose bytes a thread holds at once, at least n_out. */
@@ -244,6 +281,11 @@ extern "C" int dlk_beam_reorder(const int32_t *parents, int groups, int beams, i
             p.off = h->off; p.ids = h->ids; p.tokens = h->tokens;
             p.out_off = h->out_off; p.out_ids = h->out_ids;
             p.keep = h->max_history;
+            p.offsets = rows > kMoveSummed;
+            if (p.offsets) {
+                hipLaunchKernelGGL(history_offsets_kernel, dim3(1), dim3(1024), 0, stream, p);
+                if (hipGetLastError() != hipSuccess) return DLK_ERR_HIP;
+            }
             blocks += rows;
             h = nullptr;
         }

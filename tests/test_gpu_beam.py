@@ -331,6 +331,21 @@ def test_select_many_groups(cuda):
         assert torch.equal(out["scores"][k * 64:(k + 1) * 64], o["scores"])
 
 
+def test_select_many_rows(cuda):
+    """Far more rows than workgroups that run at once, of a few ids each."""
+    import torch
+    from diskllm_amd import api
+    g = torch.Generator("cuda").manual_seed(21)
+    lg = torch.randn((150001, 37), device="cuda", generator=g)
+    out = api.beam_select(lg, 1, 3)
+    v, i = torch.sort(lg, dim=1, descending=True, stable=True)
+    assert torch.equal(out["tokens"].view(-1, 3), i[:, :3].int())
+    want = torch.log_softmax(lg.double(), 1).gather(1, i[:, :3]).view(-1)
+    # one rounding to float, and 64-bit sums whose exponentials are good to 1e-10
+    assert ((out["scores"].double() - want).abs() <= 2.0 ** -24 * want.abs() + 2e-10).all()
+    assert torch.equal(out["parents"].view(-1, 3), torch.arange(150001, device="cuda").int()[:, None].expand(-1, 3))
+
+
 # ---- reordering ------------------------------------------------------------------
 
 def parents_of(rng, groups, beams, n_out, none=0.1):
@@ -443,7 +458,7 @@ def test_reorder_nothing(cuda):
 
 
 @pytest.mark.parametrize("groups,beams,n_out,keep", [(1, 1, 1, 1), (1, 4, 4, 5), (3, 2, 7, 40), (90, 4, 4, 300),
-                                                     (5, 64, 64, 16)])
+                                                     (5, 64, 64, 16), (384, 4, 4, 9), (385, 4, 4, 9), (5000, 1, 3, 2)])
 def test_reorder_histories(cuda, groups, beams, n_out, keep):
     import torch
     from diskllm_amd import api
