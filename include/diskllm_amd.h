@@ -327,9 +327,12 @@ typedef struct {
  * -inf are no continuations, nor are those of rows with score -inf.
  * Of each group's continuations the n_out with the largest score / max(length,
  * 1)^length_penalty (before rounding) are written, largest first; of equal ones the
- * lower row first, then the larger logit, then the lower id.  Outputs may not overlap
- * inputs (an output that is its own input is refused).  Takes workspace as dlk_sample does (dlk_release_stream; one call on the
- * stream before capturing it, else DLK_ERR_HIP). */
+ * lower row first, then the larger logit, then the lower id (continuations of two rows
+ * whose scores differ by no more than 64-bit sums' roundings, some 1e-13, may come in
+ * either order, the same in every call of these inputs).  Outputs may not overlap
+ * inputs (an output that is its own input is refused).  Takes workspace as dlk_sample
+ * does (dlk_release_stream; one call on the stream before capturing it, else
+ * DLK_ERR_HIP). */
 int dlk_beam_select(const dlk_beam_batch *batch, int groups, int vocab, const dlk_beam_params *params,
                     hipStream_t stream);
 
