@@ -481,7 +481,9 @@ extern "C" int dlk_logits_i8(const int8_t *x, int64_t ldx, const float *x_scale,
      *   200         128 x 256 47.9, 219; 128 x 128 58.1, 234; 256 x 256 62.2, 221
      *   300         128 x 256 76.5, 283; 256 x 256 67.5, 306
      *   512         256 x 256 (262,144 ids) 558; 128 x 256 657; 128 x 128 787 */
-    const bool chunks = (((uintptr_t)x | (uintptr_t)w | (uintptr_t)ldx | (uintptr_t)ldw) & 15) == 0;
+    /* (the stride of a single row says nothing) */
+    const int64_t strides = (rows > 1 ? ldx : 0) | (vocab > 1 ? ldw : 0);
+    const bool chunks = (((uintptr_t)x | (uintptr_t)w | (uintptr_t)strides) & 15) == 0;
     if (!chunks) {
         /* (33 x 50,257 x 2,047: 35.6; 300 x 100,001 x 4,097: 433, in tiles of 128 rows 562) */
         if (rows <= 16) return launch_i8_any<16, 64, 1, 4, 256>(p, stream);

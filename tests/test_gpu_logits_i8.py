@@ -122,6 +122,22 @@ def test_logits(cuda, rows, V, n, layout):
     assert (room[:, V:] == 123.0).all()
 
 
+@pytest.mark.parametrize("n", [5, 16, 100, 513, 1025, 2047])
+@pytest.mark.parametrize("rows,V", [(1, 300), (1, 1), (40, 1)])
+def test_logits_single_rows(cuda, rows, V, n):
+    """One row of x or of w whose stride is no multiple of 16, in a buffer that ends with it."""
+    import torch
+    from diskllm_amd import api
+    rng = np.random.default_rng(n)
+    pad = (n + 15) // 16 * 16
+    ldx, ldw = n if rows == 1 else pad, n if V == 1 else pad
+    xb, x = int8(rng, rows, n, ldx, 0)
+    wb, w = int8(rng, V, n, ldw, 0)
+    out = api.logits_i8(on_gpu(torch, xb, rows, n, ldx, 0), torch.ones(rows, device="cuda"),
+                        on_gpu(torch, wb, V, n, ldw, 0), torch.ones(V, device="cuda"))
+    np.testing.assert_array_equal(out.cpu().numpy(), product(x, np.ones(rows), w, np.ones(V)).astype(np.float32))
+
+
 def test_logits_extreme_sums(cuda):
     """-128 * -128 at the largest n: the sum's 32 bits are just enough."""
     import torch
