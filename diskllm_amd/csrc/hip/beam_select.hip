@@ -164,6 +164,23 @@ struct BeamShared {
     int best_row[kBeamThreads / 64];
 };
 
+/* A bound that n of the threads' keys reach: n / 4 of each wave's do, or, where a wave has too
+ * few (the end of a vocabulary, lists of one or two entries), n of one wave's.  0: none. */
+DLK_DEV uint32_t bound_of(BeamShared &sh, uint32_t key, int n) {
+    uint32_t bound = 0;
+#pragma unroll 1
+    for (int one = 0; one < 2 && bound == 0; one++) {
+        const uint32_t kw = wave_rth(key, one ? n : (n + 3) / 4);
+        if (one) __syncthreads();
+        if (lane_id() == 0) sh.wave_key[wave_id()] = kw;
+        __syncthreads();
+        bound = sh.wave_key[0];
+#pragma unroll
+        for (int w = 1; w < kBeamThreads / 64; w++) bound = one ? max(bound, sh.wave_key[w]) : min(bound, sh.wave_key[w]);
+    }
+    return __builtin_amdgcn_readfirstlane(bound);
+}
+
 /* a before b: larger key, lower row, larger entry. */
 DLK_DEV bool before(uint64_t ka, int ra, uint64_t ea, uint64_t kb, int rb, uint64_t eb) {
     if (ka != kb) return ka > kb;
@@ -307,22 +324,6 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
             sh.place[at] = b;
         }
     };
-    /* a bound that n continuations reach: n / 4 of each wave's lanes have one that does, or,
-     * where a wave has fewer (lists of one or two entries), n of one wave's */
-    auto bound_of = [&](uint32_t best) {
-        uint32_t bound = 0;
-#pragma unroll 1
-        for (int all = 0; all < 2 && bound == 0; all++) {
-            const uint32_t kw = wave_rth(best, all ? p.n : (p.n + 3) / 4);
-            __syncthreads();
-            if (lane == 0) sh.wave_key[wave] = kw;
-            __syncthreads();
-            bound = sh.wave_key[0];
-#pragma unroll
-            for (int w = 1; w < T / 64; w++) bound = all ? max(bound, sh.wave_key[w]) : min(bound, sh.wave_key[w]);
-        }
-        return bound;
-    };
     /* every entry's key for the bound, then those that reach it: PRE * T at a time, which are
      * kept from one to the other where they are all */
     uint32_t key[PRE], best = 0, bound = 0;                  /* high words, 0: none */
@@ -353,7 +354,7 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
                 add(BeamRow(sh, b).key(pre[q]), pre[q], b);
             }
         }
-        if (pass == 0) bound = bound_of(best);
+        if (pass == 0) bound = bound_of(sh, best, p.n);
     }
     __syncthreads();
     const int C = sh.count;
@@ -468,39 +469,39 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
         int listed = 0;
         /* The history's ids among this wave's logits, a lane each, penalised once and put into their
          * places batch by batch; more than 64 are counted in LDS in each batch. */
-        auto of_wave = [&](int32_t id) { return id >= s0 && id < s1 && (((id - s0) >> 8) & 3) == wave; };
+        auto wave_of = [&](int32_t id) { return ((id - s0) >> 8) & 3; };
         int said = 0;
         int32_t mine = -1;
         float becomes = 0.0f;                      /* that id's logit with its penalties */
         if (HIST && hn > 0) {
             for (int i = t; i < B / 8; i += T) ((uint4 *)times)[i] = make_uint4(0, 0, 0, 0);
-            int32_t *some = (int32_t *)packed[wave];
+            if (t < T / 64) sh.wave_n[t] = 0;
+            __syncthreads();
 #pragma unroll 1
-            for (int i0 = 0; i0 < hn; i0 += 256) {
+            for (int i0 = 0; i0 < hn; i0 += 4 * T) {
                 int32_t id[4];
 #pragma unroll
-                for (int k = 0; k < 4; k++) id[k] = hist[min(i0 + 64 * k + lane, hn - 1)];
+                for (int k = 0; k < 4; k++) id[k] = hist[min(i0 + k * T + t, hn - 1)];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const bool take = i0 + 64 * k + lane < hn && of_wave(id[k]);
-                    const uint64_t who = ballot(take);
-                    const int at = place_in(who, said);
-                    if (take && at < 64) some[at] = id[k];
-                    said += (int)__popcll(who);
-                }
+                for (int k = 0; k < 4; k++)
+                    if (i0 + k * T + t < hn && id[k] >= s0 && id[k] < s1) {
+                        const int w = wave_of(id[k]), at = atomicAdd(&sh.wave_n[w], 1);
+                        if (at < 64) ((int32_t *)packed[w])[at] = id[k];
+                    }
             }
-            wave_order();
-            if (lane < said && said <= 64) {
-                mine = some[lane];
-                becomes = lg[mine];
-            }
+            __syncthreads();
+            said = __builtin_amdgcn_readfirstlane(sh.wave_n[wave]);
             if (said <= 64) {
+                if (lane < said) {
+                    mine = ((int32_t *)packed[wave])[lane];
+                    becomes = lg[mine];
+                }
+                wave_order();
                 int cnt = 0;
 #pragma unroll 1
                 for (int k = 0; k < said; k++) cnt += __builtin_amdgcn_readlane(mine, k) == mine ? 1 : 0;
                 if (mine >= 0) becomes = beam_penalised(p, becomes, cnt);
             }
-            __syncthreads();
         }
         float most = -INFINITY;                    /* this thread's maximum, and its sum of exp(l - that) */
         double part = 0.0;
@@ -531,21 +532,31 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
             }
             auto in_batch = [&](int32_t id) { return id >= b0 && id < s1 && id - b0 < B; };
             if (HIST && said > 0 && said <= 64) {
-                for (uint64_t who = ballot(in_batch(mine)); who; who &= who - 1) {
-                    const int k = __builtin_ctzll(who);
-                    const int at = __builtin_amdgcn_readlane(mine, k) - b0;
-                    const float y = u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(becomes), k));
-                    const bool here = lane == (at >> 2 & 63);
+                const bool now = in_batch(mine);
+                if (ballot(now) != 0) {
+                    /* each id's lane + 1 at its place, where the logit's lane finds whose value it takes */
+                    uint16_t *whose = (uint16_t *)times;
+                    if (now) whose[mine - b0] = (uint16_t)(lane + 1);
+                    wave_order();
 #pragma unroll
-                    for (int q = 0; q < 4 * GR; q++) {
-                        float &v = x[q >> 2][q & 3];
-                        v = here && q == ((at >> 10) << 2 | (at & 3)) && v != -INFINITY ? y : v;
+                    for (int j = 0; j < GR; j++) {
+                        const uint2 w = ((const uint2 *)times)[j * T + t];
+                        if (ballot((w.x | w.y) != 0) == 0) continue;
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const int from = (int)(((c < 2 ? w.x : w.y) >> (16 * (c & 1))) & 0xffff);
+                            const float y = __shfl(becomes, (from - 1) & 63);
+                            x[j][c] = from != 0 && x[j][c] != -INFINITY ? y : x[j][c];
+                        }
                     }
+                    wave_order();
+                    if (now) whose[mine - b0] = 0;
+                    wave_order();
                 }
             } else if (HIST && said > 64) {
                 for (int i = lane; i < hn; i += 64) {
                     const int32_t id = hist[i];
-                    if (in_batch(id) && of_wave(id)) atomicAdd(&times[(id - b0) >> 1], 1u << (16 * (id & 1)));
+                    if (in_batch(id) && wave_of(id) == wave) atomicAdd(&times[(id - b0) >> 1], 1u << (16 * (id & 1)));
                 }
                 wave_order();
 #pragma unroll
@@ -575,13 +586,7 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
                 best = max3(max3(best, x[j][0], x[j][1]), x[j][2], x[j][3]);
             }
             if (b0 == s0) {
-                /* the bound: in each wave n / 4 lanes have an entry that reaches it */
-                const uint32_t kw = wave_rth(best > -INFINITY ? ~desc_key(best) : 0u, (p.n + 3) / 4);
-                if (lane == 0) sh.wave_key[wave] = kw;
-                __syncthreads();
-                uint32_t k = sh.wave_key[0];
-#pragma unroll
-                for (int w = 1; w < T / 64; w++) k = min(k, sh.wave_key[w]);
+                const uint32_t k = bound_of(sh, best > -INFINITY ? ~desc_key(best) : 0u, p.n);
                 if (k != 0) least = key_value(~k);           /* (0: every continuation is an entry) */
                 bound = (uint64_t)k << 32;
             }

@@ -272,6 +272,18 @@ def test_select_few_and_equal_entries(cuda, beams, n_out, V):
     check(torch, lg, beams, n_out, scores=ahead)
 
 
+@pytest.mark.parametrize("n_out", [1, 5, 64])
+@pytest.mark.parametrize("V", [4097, 4105, 4352, 4736, 5000, 8192 + 640])
+def test_select_short_ends(cuda, V, n_out):
+    """Vocabularies that end in a few ids of a batch, which are a workgroup's own."""
+    import torch
+    rng = np.random.default_rng(V)
+    check(torch, logits(rng, 8, V), 4, n_out)
+    lg = logits(rng, 8, V)
+    lg[:, 4096:] += 30
+    check(torch, lg, 4, n_out, hists=[rng.integers(0, V, 90) for _ in range(8)], rep=1.1)
+
+
 @pytest.mark.parametrize("n_out", [3, 64])
 def test_select_long_slices(cuda, n_out):
     """Slices of several batches: each better than the last, or worse; equal ones; masks of all densities; histories of
