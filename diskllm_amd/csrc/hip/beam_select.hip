@@ -7,8 +7,9 @@
  * and lists the slice's n largest entries in order.  Log softmax is increasing in l, so a
  * row's n best continuations are its n largest logits and none of the others is needed
  * again.  Its four waves work alone from the first batch's bound (n entries of the
- * workgroup reach it) to the end: each has a list of its own, counts its own history ids and
- * sums its own logits, where a mask leaves few of them (512 of 1,024) packed side by side.
+ * workgroup reach it) to the end: each has a list of its own, holds the history ids among its
+ * logits, penalised once, and sums its own logits, where a mask leaves few of them (512 of
+ * 1,024) packed side by side.
  * The group's last workgroup to finish (relaxed agent-scope atomics, as the top-k kernel's)
  * joins the slices' sums and merges the lists under the keys in 64 bits: one launch, and
  * no order of arrival shows in the result.
@@ -20,8 +21,10 @@
  * Bounds.  Large calls: reads, with what starts and ends a workgroup (512 x 262,144, 1 of 20
  * allowed: 126 us, 4.4 TB/s; with a list and barriers common to the waves and every logit
  * summed 145).  Calls that fit the chip once: the chain of a slice and the merge (64 x
- * 151,936 with penalties 33 us, of which 20 a slice's at the median, 28 at the last, 5 the
- * merge's; 128 x 50,257 in groups of 16 24.3, 16 and 8).  Small ones: a dozen round trips
+ * 151,936 with penalties 32 us, of which 20 a slice's at the median, 28 at the last, 5 the
+ * merge's; 128 x 50,257 in groups of 16 24.3, 16 and 8).  A history costs 12 us of 504 x
+ * 64,960 with 64 ids and 30 with 1,000 (57, 68, 87; with every wave looking through all of
+ * it and ids put into place one by one 154).  Small ones: a dozen round trips
  * one after another (4 x 32,000: 10.5 us).  The next batch's loads ahead of this one's work
  * changed nothing: other workgroups' waves fill that time.
  */
@@ -33,6 +36,7 @@ namespace dlk {
 
 constexpr int kBeamList = 512;         /* entries that a merge orders at once */
 constexpr int kBeamWaveList = 256;     /* and that a wave lists of a slice */
+constexpr int kBeamSaid = 128;         /* history ids that a wave holds */
 constexpr int kBeamPacked = 512;       /* of a wave's 1,024 logits: so many allowed ones or fewer are packed */
 
 DLK_DEV void bpub64(uint64_t *a, uint64_t v) { __hip_atomic_store(a, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -467,12 +471,12 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
     if (!idle) {
         uint64_t *list = sh.list[wave];
         int listed = 0;
-        /* The history's ids among this wave's logits, a lane each, penalised once and put into their
-         * places batch by batch; more than 64 are counted in LDS in each batch. */
+        /* The history's ids among this wave's logits, two a lane, penalised once and put into their places
+         * batch by batch; more than 128 are counted in LDS in each batch. */
         auto wave_of = [&](int32_t id) { return ((id - s0) >> 8) & 3; };
         int said = 0;
-        int32_t mine = -1;
-        float becomes = 0.0f;                      /* that id's logit with its penalties */
+        int32_t mine[2] = {-1, -1};
+        float becomes[2] = {0.0f, 0.0f};           /* those ids' logits with their penalties */
         if (HIST && hn > 0) {
             for (int i = t; i < B / 8; i += T) ((uint4 *)times)[i] = make_uint4(0, 0, 0, 0);
             if (t < T / 64) sh.wave_n[t] = 0;
@@ -486,21 +490,29 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
                 for (int k = 0; k < 4; k++)
                     if (i0 + k * T + t < hn && id[k] >= s0 && id[k] < s1) {
                         const int w = wave_of(id[k]), at = atomicAdd(&sh.wave_n[w], 1);
-                        if (at < 64) ((int32_t *)packed[w])[at] = id[k];
+                        if (at < kBeamSaid) ((int32_t *)packed[w])[at] = id[k];
                     }
             }
             __syncthreads();
             said = __builtin_amdgcn_readfirstlane(sh.wave_n[wave]);
-            if (said <= 64) {
-                if (lane < said) {
-                    mine = ((int32_t *)packed[wave])[lane];
-                    becomes = lg[mine];
-                }
+            if (said <= kBeamSaid) {
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (lane + 64 * h < said) {
+                        mine[h] = ((int32_t *)packed[wave])[lane + 64 * h];
+                        becomes[h] = lg[mine[h]];
+                    }
                 wave_order();
-                int cnt = 0;
+                int times_of[2] = {0, 0};
 #pragma unroll 1
-                for (int k = 0; k < said; k++) cnt += __builtin_amdgcn_readlane(mine, k) == mine ? 1 : 0;
-                if (mine >= 0) becomes = beam_penalised(p, becomes, cnt);
+                for (int k = 0; k < said; k++) {
+                    const int32_t id = __builtin_amdgcn_readlane(k < 64 ? mine[0] : mine[1], k & 63);
+                    times_of[0] += id == mine[0] ? 1 : 0;
+                    times_of[1] += id == mine[1] ? 1 : 0;
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (mine[h] >= 0) becomes[h] = beam_penalised(p, becomes[h], times_of[h]);
             }
         }
         float most = -INFINITY;                    /* this thread's maximum, and its sum of exp(l - that) */
@@ -531,12 +543,13 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
                 }
             }
             auto in_batch = [&](int32_t id) { return id >= b0 && id < s1 && id - b0 < B; };
-            if (HIST && said > 0 && said <= 64) {
-                const bool now = in_batch(mine);
-                if (ballot(now) != 0) {
-                    /* each id's lane + 1 at its place, where the logit's lane finds whose value it takes */
+            if (HIST && said > 0 && said <= kBeamSaid) {
+                const bool now0 = in_batch(mine[0]), now1 = in_batch(mine[1]);
+                if (ballot(now0 || now1) != 0) {
+                    /* each id's holder + 1 at its place, where the logit's lane finds whose value it takes */
                     uint16_t *whose = (uint16_t *)times;
-                    if (now) whose[mine - b0] = (uint16_t)(lane + 1);
+                    if (now0) whose[mine[0] - b0] = (uint16_t)(lane + 1);
+                    if (now1) whose[mine[1] - b0] = (uint16_t)(lane + 65);
                     wave_order();
 #pragma unroll
                     for (int j = 0; j < GR; j++) {
@@ -545,15 +558,20 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
 #pragma unroll
                         for (int c = 0; c < 4; c++) {
                             const int from = (int)(((c < 2 ? w.x : w.y) >> (16 * (c & 1))) & 0xffff);
-                            const float y = __shfl(becomes, (from - 1) & 63);
+                            float y = shfl(becomes[0], (from - 1) & 63);
+                            if (said > 64) {
+                                const float y1 = shfl(becomes[1], (from - 1) & 63);
+                                y = from > 64 ? y1 : y;
+                            }
                             x[j][c] = from != 0 && x[j][c] != -INFINITY ? y : x[j][c];
                         }
                     }
                     wave_order();
-                    if (now) whose[mine - b0] = 0;
+                    if (now0) whose[mine[0] - b0] = 0;
+                    if (now1) whose[mine[1] - b0] = 0;
                     wave_order();
                 }
-            } else if (HIST && said > 64) {
+            } else if (HIST && said > kBeamSaid) {
                 for (int i = lane; i < hn; i += 64) {
                     const int32_t id = hist[i];
                     if (in_batch(id) && wave_of(id) == wave) atomicAdd(&times[(id - b0) >> 1], 1u << (16 * (id & 1)));

@@ -308,6 +308,9 @@ def test_select_long_slices(cuda, n_out):
     hists[4] = np.concatenate([np.arange(256, 512), np.arange(256, 300)])
     hists[6] = [best[6, 0]] * 64
     hists[7] = [best[7, 0]] * 65
+    hists[8] = [best[8, 0]] * 60 + [best[8, 1]] * 68
+    hists[12] = [best[12, 0]] * 129
+    hists[13] = rng.choice(np.arange(512, 768), 120)
     kw = dict(hists=hists, rep=1.2, freq=0.2, pres=0.1)
     check(torch, lg, 64, n_out, **kw)
     check(torch, hidden, 64, n_out, mask=mask_of(allow), **kw)
