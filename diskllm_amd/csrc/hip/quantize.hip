@@ -158,7 +158,8 @@ extern "C" int dlk_quantize_rows(const void *x, int dtype, int64_t ldx, int rows
     if (!x || !q || !scale || rows < 0 || n <= 0 || ldx < n || ldq < n) return DLK_ERR_INVALID;
     if (((uintptr_t)scale & 3) != 0 || ((uintptr_t)x & (dtype == DLK_F32 ? 3 : 1)) != 0) return DLK_ERR_INVALID;
     /* int indices; 2^32 threads and over are no launch */
-    if (n > 0x7fffffff - 65536 || rows > (n <= 1024 ? 0x3ffffff : 0xffffff)) return DLK_ERR_UNSUPPORTED;
+    const int64_t blocks = n <= 1024 ? ((int64_t)rows + 3) / 4 : rows;
+    if (n > 0x7fffffff - 65536 || blocks * dlk::kQuantThreads > 0xffffffffLL) return DLK_ERR_UNSUPPORTED;
     if (dtype != DLK_F32 && dtype != DLK_BF16 && dtype != DLK_F16) return DLK_ERR_INVALID;
     if (rows == 0) return DLK_OK;
     if (dtype == DLK_F32) return dlk::launch_quantize<DLK_F32>(x, ldx, rows, n, q, ldq, scale, stream);

@@ -32,6 +32,13 @@ def test_quantize_rows(kw, rc):
     assert call(_lib.lib().dlk_quantize_rows, QUANT, **kw) == rc
 
 
+@pytest.mark.parametrize("n,most", [(64, 4 * 0xffffff), (1024, 4 * 0xffffff), (1025, 0xffffff)])
+@pytest.mark.parametrize("over", [1, 2, 3, 4])
+def test_quantize_rows_past_a_launch(n, most, over):
+    """Four rows to a workgroup of 256 threads up to 1,024 entries, one past that: 2^24 workgroups are no launch."""
+    assert call(_lib.lib().dlk_quantize_rows, QUANT, rows=most + over, n=n, ldx=n, ldq=n) == UNS
+
+
 LOGITS = dict(x=A, ldx=64, x_scale=A, w=A, ldw=64, w_scale=A, rows=2, vocab=100, n=64, softcap=0.0, logits=A, ld=100,
               stream=None)
 
