@@ -23,7 +23,6 @@
  * steps twice as long were no faster, nor was loading the rows' own chunks into LDS and
  * reading fragments at each row's shift (59 us: unaligned LDS reads).
  */
-#include <float.h>
 #include <math.h>
 
 #include <hip/hip_runtime.h>
@@ -92,7 +91,7 @@ DLK_DEV int place(int r, int c) {
  * series of tanh(t) / t to t^10 (what is left out: 2e-9 of it), above (1 - e) / (1 + e)
  * with e = exp(-2t).  At 0.35, the worst place, e is off by 3.4 half-steps, which 2 e / (1
  * + e)^2 / tanh makes 4.5; with t's own two and those of 1 + e, its reciprocal and the
- * products some 10 half-steps of the result at most.  recip: 1 / cap. */
+ * products some 10 half-steps of the result at most.  recip: 1 / cap, finite. */
 DLK_DEV float capped(float y, float cap, float recip) {
     const float q = y * recip, t = fabsf(q), t2 = t * t;
     float s = fmaf(t2, -1382.0f / 155925.0f, 62.0f / 2835.0f);
@@ -461,17 +460,24 @@ extern "C" int dlk_logits_i8(const int8_t *x, int64_t ldx, const float *x_scale,
                              hipStream_t stream) {
     using namespace dlk;
     if (!x || !x_scale || !w || !w_scale || !logits || rows < 0 || vocab <= 0 || n <= 0) return DLK_ERR_INVALID;
-    if (ldx < n || ldw < n || ld < vocab || softcap == INFINITY) return DLK_ERR_INVALID;
+    if (ldx < n || ldw < n || ld < vocab || !(fabsf(softcap) < INFINITY)) return DLK_ERR_INVALID;
     if ((((uintptr_t)x_scale | (uintptr_t)w_scale | (uintptr_t)logits) & 3) != 0) return DLK_ERR_INVALID;
     /* |sum| <= 128 * 128 * n in 32 bits; int indices */
     if (n > 131071 || vocab > 0x7fffffff - 65536 || rows > 0x7fffffff - 65536) return DLK_ERR_UNSUPPORTED;
     if (rows == 0) return DLK_OK;
+    /* a cap below 2^-128 has no reciprocal among the floats: the product without it, then the cap by exact quotients */
+    if (softcap > 0.0f && 1.0f / softcap == INFINITY) {
+        int rc = dlk_logits_i8(x, ldx, x_scale, w, ldw, w_scale, rows, vocab, n, 0.0f, logits, ld, stream);
+        for (int64_t r = 0; rc == DLK_OK && r < rows; r += 65535)
+            rc = dlk_softcap(logits + r * ld, ld, (int)(rows - r < 65535 ? rows - r : 65535), vocab, softcap, stream);
+        return rc;
+    }
     I8Params p;
     p.x = x; p.w = w; p.ldx = ldx; p.ldw = ldw; p.ld = ld;
     p.x_scale = x_scale; p.w_scale = w_scale; p.logits = logits;
     p.rows = rows; p.vocab = vocab; p.n = n;
     p.cap = softcap > 0.0f ? softcap : 0.0f;
-    p.recip = p.cap > 0.0f ? fminf(1.0f / p.cap, FLT_MAX) : 0.0f;
+    p.recip = p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
     /* Tiles by the rows (us at 32,000 and 151,936 ids of n = 4,096; the smallest tile that holds
      * the rows unless said otherwise):
      *   16 rows     64 ids of 512 bytes a step 27.4, 116; of 256 bytes and 4 stages 28.4, 119

@@ -271,9 +271,10 @@ int dlk_quantize_rows(const void *x, int dtype, int64_t ldx, int rows, int n, in
 /* logits[r * ld + v] = (sum_i x[r * ldx + i] * w[v * ldw + i]) * x_scale[r] * w_scale[v],
  * the sum exact in 32-bit integers (n <= 131,071, else DLK_ERR_UNSUPPORTED), then
  * three float roundings (the sum's, and one per scale); softcap > 0: then softcap *
- * tanh(logit / softcap) to 2^-20 of it, or to 2^-148 * softcap where that is more (not
- * libm's bits, which dlk_softcap gives); softcap must be finite.  Any strides and byte alignment of x and w.  Entries past
- * vocab in a row of logits are left as they are. */
+ * tanh(logit / softcap) to 2^-20 of it, or to 2^-148 * softcap or 2^-149 (the smallest
+ * float) where one of those is more (not libm's bits, which dlk_softcap gives); softcap
+ * must be finite.  Any strides and byte alignment of x and w.  Entries past vocab in a
+ * row of logits are left as they are. */
 int dlk_logits_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw,
                   const float *w_scale, int rows, int vocab, int n, float softcap, float *logits, int64_t ld,
                   hipStream_t stream);

@@ -48,7 +48,8 @@ LOGITS = dict(x=A, ldx=64, x_scale=A, w=A, ldw=64, w_scale=A, rows=2, vocab=100,
     (dict(logits=None), INV), (dict(rows=-1), INV), (dict(vocab=0), INV), (dict(n=0), INV), (dict(ldx=63), INV),
     (dict(ldw=63), INV), (dict(ld=99), INV), (dict(logits=A + 2), INV), (dict(w_scale=A + 1), INV),
     (dict(n=131072, ldx=131072, ldw=131072), UNS), (dict(softcap=float("inf")), INV), (dict(vocab=0x7fffffff, ld=1 << 40), UNS), (dict(rows=0), OK),
-    (dict(vocab=1 << 30, ld=1 << 30), UNS)])
+    (dict(vocab=1 << 30, ld=1 << 30), UNS),
+    (dict(softcap=float("nan")), INV), (dict(softcap=float("-inf")), INV)])
 def test_logits_i8(kw, rc):
     assert call(_lib.lib().dlk_logits_i8, LOGITS, **kw) == rc
 

@@ -176,6 +176,36 @@ def test_logits_softcap(cuda, rows, V, n, cap):
     assert float(err.max()) <= 16 * U, float(err.max()) / U
 
 
+@pytest.mark.parametrize("rows", [1, 20, 130, 400])
+@pytest.mark.parametrize("layout", ["padded", "packed"])
+@pytest.mark.parametrize("cap", [1e-45, 1e-40, 2.9387e-39, 2.0 ** -128, 3e-39, 1e-38, 3.4e38])
+def test_logits_softcap_extreme(cuda, rows, layout, cap):
+    """Caps whose reciprocal is no float, next to those that have one, and the largest; what lies past a row is left."""
+    import torch
+    from diskllm_amd import api
+    V, n = 261, 65
+    g = torch.Generator("cuda").manual_seed(rows)
+    ld = n if layout == "packed" else 80
+    x = torch.randint(-127, 128, (rows, ld), device="cuda", generator=g, dtype=torch.int8)[:, :n]
+    w = torch.randint(-127, 128, (V, ld), device="cuda", generator=g, dtype=torch.int8)[:, :n]
+    w[3] = 0
+    c = float(np.float32(cap))
+    # sums of some 5e4 by sqrt(c) / 3e2 twice: quotients about 1/2; some rows and ids far below and above
+    xs = torch.full((rows,), float(np.sqrt(c) / 300), device="cuda") * torch.exp(torch.randn(rows, device="cuda", generator=g))
+    ws = torch.full((V,), float(np.sqrt(c) / 300), device="cuda") * torch.exp(torch.randn(V, device="cuda", generator=g) * 4)
+    plain = api.logits_i8(x, xs, w, ws).double()
+    room = torch.full((rows, V + 3), 7.0, device="cuda")
+    api.logits_i8(x, xs, w, ws, softcap=cap, out=room[:, :V])
+    torch.cuda.synchronize()
+    got = room[:, :V].double()
+    want = c * torch.tanh(plain / c)
+    # 16 half-steps as above; the reciprocal of a cap past 2^126 is off by up to 4; a subnormal result's own rounding,
+    # and the quotient's where that is subnormal
+    room_for = (16 + (4 if cap > 2.0 ** 126 else 0)) * U * want.abs() + 2.0 ** -149 + 2.0 ** -148 * c
+    assert ((got - want).abs() <= room_for).all(), float(((got - want).abs() - room_for).max())
+    assert (room[:, V:] == 7.0).all()
+
+
 def test_hidden_states_to_logits(cuda):
     """The two calls as a decode step makes them; a token whose hidden state is not finite has NaN logits and leaves
     the others alone."""
