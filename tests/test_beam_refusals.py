@@ -186,3 +186,39 @@ def test_state_layouts():
     # rows that lie apart
     v = api.beam_state(torch.zeros((8, 3, 40))[:, 1])
     assert (v.bytes, v.n_outer, v.n_inner, v.src_row) == (160, 1, 1, 480)
+
+
+@pytest.fixture
+def on_no_device(monkeypatch):
+    """CPU or meta tensors taken for the GPU's, calls recorded and not made; returns what was called."""
+    calls = []
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    monkeypatch.setattr(api, "_call", lambda dev, stream, what, fn, *args: calls.append((what, stream, args)))
+    return calls
+
+
+def test_counts_past_32_bits(on_no_device):
+    """What ctypes would cut to its low 32 bits is refused."""
+    i, big = torch.int32, 1 << 32
+    z = torch.zeros
+    meta = lambda *shape, **kw: torch.empty(shape, device="meta", **kw)
+    spread = lambda n, m: torch.empty_strided((n, 4, m), (8 * m, 2 * m, 1), device="meta", dtype=torch.uint8)
+    hist = lambda n: api.beam_history(z(9, dtype=i), z(8, dtype=i), None, n, z(9, dtype=i), z(99, dtype=i))
+    for bad in (lambda: api.beam_state(meta(big + 1, 4, dtype=torch.uint8), row_dim=1),
+                lambda: api.beam_state(meta(4, big + 1, 1, dtype=torch.uint8), length_dim=2),
+                lambda: api.beam_state(spread(big + 1, 2), row_dim=1),
+                lambda: hist(big + 1), lambda: hist(-big + 8),
+                lambda: api.beam_select(z(8, 30), 4, 4, max_history=big + 8),
+                lambda: api.beam_select(z(8, 30), 4, 4, eos_id=big + 8),
+                lambda: api.beam_select(z(8, 30), 4, 4, eos_id=-big + 8),
+                lambda: api.beam_select(z(8, 30), 4, 4, order=big + 1),
+                lambda: api.beam_select(z(8, 30), 4, 4, order=-1),
+                lambda: api.beam_select(z(0, 30), big + 4, 4), lambda: api.beam_select(z(0, 30), 4, big + 4),
+                lambda: api.beam_reorder(meta(big + 4, dtype=i), 1, 1), lambda: api.beam_reorder(z(0, dtype=i), 4, big + 4)):
+        with pytest.raises(ValueError):
+            bad()
+    assert on_no_device == []
+    # what fits still goes through
+    assert api.beam_state(meta((1 << 31) - 1, 4, dtype=torch.uint8), row_dim=1).n_outer == (1 << 31) - 1
+    api.beam_select(z(8, 30), 4, 4, max_history=65535, eos_id=29, order=0xffffffff)
+    assert len(on_no_device) == 1
