@@ -159,8 +159,11 @@ def results(db: DeviceBatch) -> dict:
 
 
 # ---- 8-bit logits and beam search ------------------------------------------------
-# Tensors on one device, the call on that device's current stream unless `stream` says
-# otherwise; what does not fit raises ValueError before anything is launched.
+# Tensors on one device, the call on that device's current stream unless `stream` (a raw
+# handle) says otherwise; what does not fit raises ValueError before anything is launched.
+# Tensors that a call makes belong to the stream it runs on, as those made under
+# torch.cuda.stream: another stream waits for it first, and record_stream tells the
+# allocator where they outlive that wait.
 
 _F32, _I32, _I8, _U8 = torch.float32, torch.int32, torch.int8, torch.uint8
 _DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
@@ -200,6 +203,17 @@ def _flat(t: torch.Tensor, n: int, dev: int, dtype, what: str) -> int:
     return t.data_ptr()
 
 
+def _empty(shape, dtype, like: torch.Tensor, dev: int, stream) -> torch.Tensor:
+    """An output on like's device, of the memory that belongs to the call's stream: the allocator gives a block to
+    one stream at a time, so one of the current stream's might still be in use there, or given away again while
+    the kernel on `stream` writes it."""
+    if stream is None or dev < 0 or stream == torch._C._cuda_getCurrentRawStream(dev):
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    on = torch.cuda.ExternalStream(stream, device=like.device) if stream else torch.cuda.default_stream(like.device)
+    with torch.cuda.stream(on):
+        return torch.empty(shape, dtype=dtype, device=like.device)
+
+
 def _call(dev: int, stream, what: str, fn, *args) -> None:
     """fn(*args, stream) with device `dev` current (the kernels run there)."""
     if dev < 0:
@@ -225,14 +239,14 @@ def quantize_rows(x: torch.Tensor, q: Optional[torch.Tensor] = None, scale: Opti
     rows, n, ldx = _rows2d(x, dev, None, "x")
     if q is None:
         ldq = (n + 15) // 16 * 16
-        q = torch.empty((rows, ldq), dtype=_I8, device=x.device)
+        q = _empty((rows, ldq), _I8, x, dev, stream)
         if ldq != n:
             q = q[:, :n]
     else:
         q_rows, q_n, ldq = _rows2d(q, dev, _I8, "q")
         _want(q_rows == rows and q_n == n, "q: x's shape is wanted")
     if scale is None:
-        scale = torch.empty(rows, dtype=_F32, device=x.device)
+        scale = _empty(rows, _F32, x, dev, stream)
         at = scale.data_ptr()
     else:
         at = _flat(scale, rows, dev, _F32, "scale")
@@ -252,7 +266,7 @@ def logits_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     _want(w_n == n, "x and w: rows of one length are wanted")
     if out is None:
         ld = (V + 63) // 64 * 64
-        out = torch.empty((rows, ld), dtype=_F32, device=x.device)
+        out = _empty((rows, ld), _F32, x, dev, stream)
         if ld != V:
             out = out[:, :V]
     else:
@@ -283,9 +297,9 @@ def beam_select(logits: torch.Tensor, beams: int, n_out: int, *, scores: Optiona
     groups = rows // beams
     n = groups * n_out
     if out is None:
-        i32, at = torch.empty((3, n), dtype=_I32, device=logits.device), logits.device
-        out = dict(tokens=i32[0], parents=i32[1], lengths=i32[2], scores=torch.empty(n, dtype=_F32, device=at),
-                   finished=torch.empty(n, dtype=_U8, device=at))
+        i32 = _empty((3, n), _I32, logits, dev, stream)
+        out = dict(tokens=i32[0], parents=i32[1], lengths=i32[2], scores=_empty(n, _F32, logits, dev, stream),
+                   finished=_empty(n, _U8, logits, dev, stream))
     sc = 0 if scores is None else _flat(scores, rows, dev, _F32, "scores")
     ln = 0 if lengths is None else _flat(lengths, rows, dev, _I32, "lengths")
     fi = 0 if finished is None else _flat(finished, rows, dev, _U8, "finished")

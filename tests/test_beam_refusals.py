@@ -222,3 +222,31 @@ def test_counts_past_32_bits(on_no_device):
     assert api.beam_state(meta((1 << 31) - 1, 4, dtype=torch.uint8), row_dim=1).n_outer == (1 << 31) - 1
     api.beam_select(z(8, 30), 4, 4, max_history=65535, eos_id=29, order=0xffffffff)
     assert len(on_no_device) == 1
+
+
+@pytest.mark.parametrize("current,stream,made_on", [(111, 222, 222), (111, 0, 0), (0, 222, 222), (111, 111, None),
+                                                    (111, None, None), (0, 0, None)])
+def test_outputs_are_made_on_the_calls_stream(on_no_device, monkeypatch, current, stream, made_on):
+    """Outputs that a call makes come from the memory of the stream that writes them: a block of the current stream's
+    may still be in use there, and goes back to it while the kernel writes."""
+    import contextlib
+    now, made = [None], []
+
+    @contextlib.contextmanager
+    def on(s):
+        before, now[0] = now[0], s
+        yield
+        now[0] = before
+    empty = torch.empty
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda at, device=None: at)
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: current, raising=False)
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: made.append(now[0]) or empty(*a, **kw))
+    b = torch.int8
+    api.quantize_rows(torch.zeros(4, 8), stream=stream)
+    api.quantize_rows(torch.zeros(4, 8), q=torch.zeros((4, 8), dtype=b), stream=stream)
+    api.logits_i8(torch.zeros((4, 8), dtype=b), torch.zeros(4), torch.zeros((9, 8), dtype=b), torch.zeros(9), stream=stream)
+    api.beam_select(torch.zeros(8, 30), 4, 4, stream=stream)
+    assert [s for _, s, _ in on_no_device] == [stream] * 4
+    assert made == [made_on] * 7 and now == [None]

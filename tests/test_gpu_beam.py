@@ -801,3 +801,34 @@ def test_streams_at_once(cuda):
             assert torch.equal(w[k], o[k]), k
     for st in streams:
         _lib.check(_lib.lib().dlk_release_stream(st.cuda_stream), "dlk_release_stream")
+
+
+def test_outputs_on_a_given_stream(cuda):
+    """A stream by its handle while the current one still has work for blocks of the outputs' sizes, just freed: the
+    outputs are other memory.  The same from a side stream onto the default one."""
+    import torch
+    from diskllm_amd import api
+    g = torch.Generator("cuda").manual_seed(2)
+    h = torch.randn((40, 320), device="cuda", generator=g)
+    w, ws = api.quantize_rows(torch.randn((1000, 320), device="cuda", generator=g))
+    want_q, want_s = api.quantize_rows(h)
+    want_l = api.logits_i8(want_q, want_s, w, ws)
+    want_b = api.beam_select(want_l, 4, 4)
+    busy = torch.empty(1 << 28, dtype=torch.float32, device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for current, other in ((torch.cuda.default_stream(), side.cuda_stream), (side, 0)):
+        with torch.cuda.stream(current):
+            held = [torch.empty_like(t) for t in (want_q, want_s, want_l, *want_b.values())]
+            held.append(torch.empty((3, 40), dtype=torch.int32, device="cuda"))
+            for _ in range(20):
+                busy.fill_(1.0)
+            for t in held:
+                t.fill_(3)
+            del held, t
+            q, s = api.quantize_rows(h, stream=other)
+            logits = api.logits_i8(q, s, w, ws, stream=other)
+            out = api.beam_select(logits, 4, 4, stream=other)
+        torch.cuda.synchronize()
+        assert torch.equal(q, want_q) and torch.equal(s, want_s) and torch.equal(logits, want_l)
+        assert all(torch.equal(out[k], want_b[k]) for k in out)
