@@ -323,14 +323,15 @@ typedef struct {
 /* One step of a beam search.  Row r's logits l are masked, then penalised, as
  * dlk_sample does; its continuation by id v has
  *   score = scores[r] + (l_v - max l) - log(sum_u exp(l_u - max l)),  length = lengths[r] + 1,
- * computed in 64 bits and rounded once.  A finished row has one continuation: eos_id,
+ * computed in 64 bits (exponentials to 4e-15 of each) and rounded once.  A finished row has one continuation: eos_id,
  * with its score and length as they are (whatever its logits hold).  Ids with logit
  * -inf are no continuations, nor are those of rows with score -inf.
  * Of each group's continuations the n_out with the largest score / max(length,
  * 1)^length_penalty (before rounding) are written, largest first; of equal ones the
  * lower row first, then the larger logit, then the lower id (continuations of two rows
- * whose scores differ by no more than 64-bit sums' roundings, some 1e-13, may come in
- * either order, the same in every call of these inputs).  Outputs may not overlap
+ * whose scores over length^length_penalty differ by no more than what those roundings come
+ * to, 2^-42 and 2^-50 of their size at up to 262,144 logits a row, may come in either
+ * order, the same in every call of these inputs).  Outputs may not overlap
  * inputs (an output that is its own input is refused).  Takes workspace as dlk_sample
  * does (dlk_release_stream; one call on the stream before capturing it, else
  * DLK_ERR_HIP). */

@@ -832,3 +832,49 @@ def test_outputs_on_a_given_stream(cuda):
         torch.cuda.synchronize()
         assert torch.equal(q, want_q) and torch.equal(s, want_s) and torch.equal(logits, want_l)
         assert all(torch.equal(out[k], want_b[k]) for k in out)
+
+
+@pytest.mark.parametrize("V,shape", [(2, "pair"), (40, "pair"), (5000, "spread"), (20000, "rising"), (20000, "falling"),
+                                     (100000, "rising"), (50257, "level")])
+def test_select_orders_near_rows(cuda, V, shape):
+    """A row of one continuation beside a row of many, their best scores a few times the header's bound apart, in
+    either direction.  The gap is set by one logit of the second row and is known from sums in 64 bits."""
+    import torch
+    from diskllm_amd import api
+    rng = np.random.default_rng(V)
+    if shape == "pair":
+        base, grid, at = np.zeros(1, np.float32), -rng.uniform(0.05, 3.0, 1 << 22).astype(np.float32), 1
+    else:
+        base = {"spread": lambda: rng.normal(0, 2.5, V - 1), "rising": lambda: np.linspace(-20, 0, V - 1),
+                "falling": lambda: np.linspace(0, -20, V - 1), "level": lambda: np.full(V - 1, -1e-3)}[shape]().astype(np.float32)
+        base -= base.max()
+        base[0 if shape == "falling" else -1] = 0.0
+        grid, at = -rng.uniform(0.05, 3.0, 1 << 22).astype(np.float32), V // 2
+    import math
+    rest = math.fsum(np.exp(base.astype(np.float64))) - 1.0
+    best = -np.log1p(rest + np.exp(grid.astype(np.float64)))          # the second row's best score, for each value
+    other = best.astype(np.float32)                                   # the first row's, a float beside it
+    gap = best - other.astype(np.float64)
+    size = np.abs(best)
+    # past the bound, and past what this sum in 64 bits may be off by
+    room = 2.0 ** -42 + 2.0 ** -50 * size
+    pick = np.flatnonzero((np.abs(gap) > 1.25 * room) & (np.abs(gap) < 1.25 * room + 4e-12))
+    assert len(pick) >= 24
+    pick = np.concatenate([pick[gap[pick] > 0][:64], pick[gap[pick] < 0][:64]])
+    groups = len(pick)
+    lg = np.full((2 * groups, V), -np.inf, np.float32)
+    lg[0::2, 0] = 0.0
+    lg[1::2, :at] = base[:at]
+    lg[1::2, at] = grid[pick]
+    if V > at + 1:
+        lg[1::2, at + 1:at + 1 + len(base) - at] = base[at:]
+    top = int(lg[1].argmax())
+    scores = np.zeros(2 * groups, np.float32)
+    scores[0::2] = other[pick]
+    got = api.beam_select(torch.from_numpy(lg).cuda(), 2, 2, scores=torch.from_numpy(scores).cuda())
+    torch.cuda.synchronize()
+    parents, tokens = got["parents"].cpu().numpy().reshape(groups, 2), got["tokens"].cpu().numpy().reshape(groups, 2)
+    second_first = gap[pick] > 0
+    np.testing.assert_array_equal(parents[:, 0] & 1, second_first)
+    np.testing.assert_array_equal(tokens[:, 0], np.where(second_first, top, 0))
+    assert second_first.any() and not second_first.all()
