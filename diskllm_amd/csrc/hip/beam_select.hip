@@ -167,6 +167,7 @@ struct BeamShared {
     double part[kBeamThreads / 64];
     float cum[DLK_MAX_BEAMS];
     float top[DLK_MAX_BEAMS];
+    float best_score;                   /* of the group, over the lengths' norm */
     uint32_t wave_key[kBeamThreads / 64];
     int wave_n[kBeamThreads / 64], wave_listed[kBeamThreads / 64];
     int place[kBeamList];               /* row of each entry */
@@ -228,6 +229,8 @@ struct BeamRow {
     /* the score of entry e in 64 bits, and its key */
     DLK_DEV double score(uint64_t e) const { return over ? cum : cum + (((double)entry_logit(e) - top) - base); }
     DLK_DEV uint64_t key(uint64_t e) const { return double_key(score(e) * norm); }
+    /* that as a word, by its distance from the group's best (to 2^-11 of it, whatever the scores' size is); never 0 */
+    DLK_DEV uint32_t word(uint64_t e, double best) const { return ~f2u(fmaxf((float)(best - score(e) * norm), 0.0f)); }
 };
 
 DLK_DEV void write_continuation(const BeamParams &p, const BeamShared &sh, int g, int j, int b, uint64_t e) {
@@ -309,7 +312,9 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
         }
     }
     __syncthreads();
-    /* what each row adds to its continuations, a lane each */
+    /* what each row adds to its continuations, a lane each; and the group's best key, rounded to float: a row's best
+     * entry is its maximum */
+    float most = -INFINITY;
     if (t < p.beams) {
         const int64_t row = (int64_t)g * p.beams + t;
         const float cum = p.scores ? p.scores[row] : 0.0f;
@@ -317,13 +322,22 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
         const int kind = sh.kind[t];
         const bool alive = cum > -INFINITY && cum < INFINITY;
         const double length = fmax((double)(p.lengths ? p.lengths[row] : 0) + (over ? 0.0 : 1.0), 1.0);
+        const double base = kind == 1 ? log(sh.base[t]) : 0.0;
+        const double norm = p.alpha == 0.0f ? 1.0 : 1.0 / pow(length, (double)p.alpha);
+        const int by = !alive ? 0 : over ? 2 : kind == 1 ? 1 : 0;
         sh.cum[t] = cum;
-        sh.base[t] = kind == 1 ? log(sh.base[t]) : 0.0;
-        sh.norm[t] = p.alpha == 0.0f ? 1.0 : 1.0 / pow(length, (double)p.alpha);
-        sh.kind[t] = !alive ? 0 : over ? 2 : kind == 1 ? 1 : 0;
+        sh.base[t] = base;
+        sh.norm[t] = norm;
+        sh.kind[t] = by;
+        if (by != 0) most = (float)(((double)cum - base) * norm);
         if (p.status && (!(cum < INFINITY) || (alive && !over && kind < 0))) atomicOr(p.status, DLK_STATUS_NOT_FINITE);
     }
+    if (wave == 0) {
+        most = wave_max_dpp(most);
+        if (t == 0) sh.best_score = most;
+    }
     __syncthreads();
+    const double best_score = (double)sh.best_score;
     /* list i of row b: its entries (a finished row's first list holds its one continuation) */
     auto listed = [&](int i, int b) {
         const int kind = sh.kind[b];
@@ -337,9 +351,12 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
             sh.place[at] = b;
         }
     };
-    /* every entry's key for the bound, then those that reach it: PRE * T at a time, which are
-     * kept from one to the other where they are all */
-    uint32_t key[PRE], best = 0, bound = 0;                  /* high words, 0: none */
+    /* every entry's word for the bound, then those that reach it: PRE * T at a time, which are
+     * kept from one to the other where they are all.  The bound has a word's 20 leading bits: of the
+     * distance from the best, so that it is as close where scores are large (16 x 16 x 128,256
+     * of 32: 73 us at scores of -20, 76 at -2,500; bits of the scores themselves were 8 apart there,
+     * more reached it than are ranked at once, and it took 125). */
+    uint32_t word[PRE], best = 0, bound = 0;                 /* 0: none */
     const float per_n = 1.0f / (float)p.n, per_slices = 1.0f / (float)p.slices;
     auto list_of = [&](int at) { return (int)(((float)at + 0.5f) * per_n); };              /* exact: below 2^15 */
     auto row_of = [&](int i) { return (int)(((float)i + 0.5f) * per_slices); };
@@ -351,18 +368,18 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
                 if (pass > 0 || e0 > 0) load(e0);
 #pragma unroll
                 for (int q = 0; q < PRE; q++) {              /* (few entries: few instructions, fetched for the first time) */
-                    key[q] = 0;
+                    word[q] = 0;
                     if (e0 + q * T >= E) continue;
                     const int at = min(e0 + q * T + mine, E - 1), i = list_of(at), b = row_of(i);
                     if (sh.kind[b] == 2) pre[q] = ~(uint64_t)0;
-                    if (e0 + q * T + mine < E && at - i * p.n < listed(i, b)) key[q] = (uint32_t)(BeamRow(sh, b).key(pre[q]) >> 32);
-                    best = max(best, key[q]);
+                    if (e0 + q * T + mine < E && at - i * p.n < listed(i, b)) word[q] = BeamRow(sh, b).word(pre[q], best_score);
+                    best = max(best, word[q]);
                 }
             }
             if (pass == 0) continue;
 #pragma unroll
             for (int q = 0; q < PRE; q++) {
-                if (key[q] == 0 || key[q] < bound) continue;
+                if (word[q] == 0 || word[q] < bound) continue;
                 const int b = row_of(list_of(e0 + q * T + mine));
                 add(BeamRow(sh, b).key(pre[q]), pre[q], b);
             }

@@ -878,3 +878,51 @@ def test_select_orders_near_rows(cuda, V, shape):
     np.testing.assert_array_equal(parents[:, 0] & 1, second_first)
     np.testing.assert_array_equal(tokens[:, 0], np.where(second_first, top, 0))
     assert second_first.any() and not second_first.all()
+
+
+def late(rng, groups, beams, score):
+    """Scores of beams late in a long search: far from 0 and near one another."""
+    return (score - rng.uniform(0, 0.6, (groups, beams)).cumsum(1)).astype(np.float32).reshape(-1)
+
+
+@pytest.mark.parametrize("score", [-600.0, -1200.0, -4000.0, -1e6, -1e30])
+@pytest.mark.parametrize("groups,beams,n_out,V", [(2, 4, 4, 9000), (2, 16, 16, 50257), (2, 8, 16, 50257), (1, 16, 32, 128256),
+                                                  (1, 64, 64, 20000), (3, 1, 64, 151936)])
+def test_select_far_scores(cuda, groups, beams, n_out, V, score):
+    import torch
+    rng = np.random.default_rng(V + beams)
+    lg = logits(rng, groups * beams, V)
+    sc = late(rng, groups, beams, score)
+    if score > -1e5:
+        check(torch, lg, beams, n_out, scores=sc)
+        check(torch, lg, beams, n_out, scores=sc, lengths=rng.integers(300, 900, groups * beams).astype(np.int32), alpha=0.7,
+              eos=7, finished=(rng.random(groups * beams) < 0.3).astype(np.uint8))
+        check(torch, lg + np.float32(1000), beams, n_out, scores=sc)
+    else:
+        # (a score's 64 bits no longer tell all entries apart: equal ones by the lower row, the larger logit, the lower id)
+        check(torch, lg, beams, n_out, scores=sc)
+
+
+@pytest.mark.parametrize("groups,beams,n_out,V", [(8, 16, 16, 50257), (8, 8, 16, 50257), (16, 16, 32, 128256)])
+def test_select_far_scores_cost_no_more(cuda, groups, beams, n_out, V):
+    """How far the scores are from 0 does not decide how the lists are merged: taken one by one, 16 continuations cost
+    half of the whole call again."""
+    import torch
+    from diskllm_amd import api
+    rng = np.random.default_rng(4)
+    g = torch.Generator("cuda").manual_seed(3)
+    lg = torch.randn((groups * beams, V), device="cuda", generator=g) * 2.5
+    near, far = (torch.from_numpy(late(rng, groups, beams, s)).cuda() for s in (-2.0, -2500.0))
+    out = api.beam_select(lg, beams, n_out, scores=near)
+    best = {}
+    for _ in range(15):
+        for name, sc in (("near", near), ("far", far)):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            api.beam_select(lg, beams, n_out, scores=sc, out=out)
+            start.record()
+            for _ in range(20):
+                api.beam_select(lg, beams, n_out, scores=sc, out=out)
+            end.record()
+            end.synchronize()
+            best[name] = min(best.get(name, 1e9), start.elapsed_time(end))
+    assert best["far"] < 1.25 * best["near"], best
