@@ -267,10 +267,19 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
      * (i % 4) * 64 + i / 4 % 64, so that the waves share few of them evenly */
     const int mine = (t & 63) * 4 + (t >> 6);
     uint64_t pre[PRE];
+    /* which of the T entries from e on: dealt anew for each T, or a thread would hold the same places
+     * of many lists (n a power of two), the best of the threads be those of a few places, and
+     * more reach their bound than are ranked at once (16 x 2 x 151,936 of 64, beams near one another:
+     * 36 us, 102 that way; 16 x 4 52, 142) */
+    auto place_of = [&](int e) {
+        int m = mine;
+        asm volatile("" : "+v"(m));                          /* (places kept are 16 registers) */
+        return e + ((m + e / T * 37) & (T - 1));
+    };
     auto load = [&](int e0) {
 #pragma unroll
         for (int q = 0; q < PRE; q++)
-            if (e0 + q * T < E) pre[q] = bget64(&cands[min(e0 + q * T + mine, E - 1)]);
+            if (e0 + q * T < E) pre[q] = bget64(&cands[min(place_of(e0 + q * T), E - 1)]);
     };
     if (t < L) {
         const uint64_t mk = bget64(&slots[t].max_kept);
@@ -370,9 +379,9 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
                 for (int q = 0; q < PRE; q++) {              /* (few entries: few instructions, fetched for the first time) */
                     word[q] = 0;
                     if (e0 + q * T >= E) continue;
-                    const int at = min(e0 + q * T + mine, E - 1), i = list_of(at), b = row_of(i);
+                    const int place = place_of(e0 + q * T), at = min(place, E - 1), i = list_of(at), b = row_of(i);
                     if (sh.kind[b] == 2) pre[q] = ~(uint64_t)0;
-                    if (e0 + q * T + mine < E && at - i * p.n < listed(i, b)) word[q] = BeamRow(sh, b).word(pre[q], best_score);
+                    if (place < E && at - i * p.n < listed(i, b)) word[q] = BeamRow(sh, b).word(pre[q], best_score);
                     best = max(best, word[q]);
                 }
             }
@@ -380,7 +389,7 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
 #pragma unroll
             for (int q = 0; q < PRE; q++) {
                 if (word[q] == 0 || word[q] < bound) continue;
-                const int b = row_of(list_of(e0 + q * T + mine));
+                const int b = row_of(list_of(place_of(e0 + q * T)));
                 add(BeamRow(sh, b).key(pre[q]), pre[q], b);
             }
         }

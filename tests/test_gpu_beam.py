@@ -908,15 +908,20 @@ def test_select_far_scores_cost_no_more(cuda, groups, beams, n_out, V):
     """How far the scores are from 0 does not decide how the lists are merged: taken one by one, 16 continuations cost
     half of the whole call again."""
     import torch
-    from diskllm_amd import api
     rng = np.random.default_rng(4)
+    assert_costs_alike(torch, groups, beams, n_out, V, *(late(rng, groups, beams, s) for s in (-2.0, -2500.0)))
+
+
+def assert_costs_alike(torch, groups, beams, n_out, V, few, many):
+    """A selection with the scores `many` takes no more than a quarter longer than with `few`, by their best of 15 turns."""
+    from diskllm_amd import api
     g = torch.Generator("cuda").manual_seed(3)
     lg = torch.randn((groups * beams, V), device="cuda", generator=g) * 2.5
-    near, far = (torch.from_numpy(late(rng, groups, beams, s)).cuda() for s in (-2.0, -2500.0))
-    out = api.beam_select(lg, beams, n_out, scores=near)
-    best = {}
+    scores = [torch.from_numpy(s).cuda() for s in (few, many)]
+    out = api.beam_select(lg, beams, n_out, scores=scores[0])
+    best = [1e9, 1e9]
     for _ in range(15):
-        for name, sc in (("near", near), ("far", far)):
+        for k, sc in enumerate(scores):
             start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
             api.beam_select(lg, beams, n_out, scores=sc, out=out)
             start.record()
@@ -924,5 +929,13 @@ def test_select_far_scores_cost_no_more(cuda, groups, beams, n_out, V):
                 api.beam_select(lg, beams, n_out, scores=sc, out=out)
             end.record()
             end.synchronize()
-            best[name] = min(best.get(name, 1e9), start.elapsed_time(end))
-    assert best["far"] < 1.25 * best["near"], best
+            best[k] = min(best[k], start.elapsed_time(end))
+    assert best[1] < 1.25 * best[0], best
+
+
+@pytest.mark.parametrize("groups,beams,V", [(16, 2, 151936), (16, 4, 151936)])
+def test_select_near_beams_cost_no_more(cuda, groups, beams, V):
+    """64 continuations that may come from any beam of a group, beside those of one beam alone."""
+    import torch
+    few = np.tile(np.where(np.arange(beams) == 0, -5.0, -5000.0), groups).astype(np.float32)
+    assert_costs_alike(torch, groups, beams, 64, V, few, late(np.random.default_rng(4), groups, beams, -5.0))
