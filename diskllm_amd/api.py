@@ -174,11 +174,7 @@ def _want(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _ints(what: str, *values: int) -> None:
-    """Refuses what does not fit the C int it goes to (ctypes keeps its low bits)."""
-    for v in values:
-        if not -0x80000000 <= v <= 0x7fffffff:
-            raise ValueError(f"{what}: {v} takes more than 32 bits")
+_WIDE = "{}: integers of 32 bits are wanted"          # (of a C int ctypes keeps the low bits)
 
 
 def _rows2d(t: torch.Tensor, dev: int, dtype, what: str):
@@ -291,9 +287,10 @@ def beam_select(logits: torch.Tensor, beams: int, n_out: int, *, scores: Optiona
     lengths (int32), scores (float32) and finished (uint8) of the n_out best continuations of each group."""
     dev = logits.get_device()
     rows, V, ld = _rows2d(logits, dev, _F32, "logits")
-    _ints("beam_select", beams, n_out, eos_id, max_history)
-    _want(0 <= order <= 0xffffffff, "order: a word of DLK_OP_* is wanted")
     _want(beams > 0 and n_out > 0 and rows % beams == 0, "logits: whole groups of beams are wanted")
+    if ((beams | n_out) >> 31 or order >> 32 or not -0x80000000 <= eos_id <= 0x7fffffff or
+            not -0x80000000 <= max_history <= 0x7fffffff):
+        raise ValueError(_WIDE.format("beam_select"))
     groups = rows // beams
     n = groups * n_out
     if out is None:
@@ -364,7 +361,8 @@ def beam_state(src: torch.Tensor, dst: Optional[torch.Tensor] = None, row_dim: i
         entry = item
         for n in size[cut + 1:]:
             entry *= n
-        _ints("beam_state", outer, inner)
+        if (outer | inner) >> 31:
+            raise ValueError(_WIDE.format("beam_state"))
         room = entry * size[cut] if cut < nd else entry
         row = room * inner
         at, dev = src.data_ptr(), src.get_device()
@@ -393,7 +391,7 @@ def beam_state(src: torch.Tensor, dst: Optional[torch.Tensor] = None, row_dim: i
         return t.data_ptr(), st[row_dim] * item, outer, inner, rest[0] * item
     at, row, outer, inner, width = layout(src)
     d_at, d_row, d_outer, d_inner, _ = (at, row, outer, inner, width) if dst is None else layout(dst)
-    _ints("beam_state", outer[0], inner[0])
+    _want((outer[0] | inner[0]) >> 31 == 0, _WIDE.format("beam_state"))
     s = _lib.BeamState(at, d_at, 0 if 0 in shape else width, row, outer[1] * item, inner[1] * item, d_row,
                        d_outer[1] * item, d_inner[1] * item, outer[0], inner[0])
     s.rows = (rows, dst_rows, src.get_device(), src.get_device() if dst is None else dst.get_device())
@@ -404,7 +402,8 @@ def beam_history(off: torch.Tensor, ids: torch.Tensor, tokens: Optional[torch.Te
                  out_off: torch.Tensor, out_ids: torch.Tensor) -> _lib.BeamHistory:
     """The rows' histories (CSR) and the tokens to append, for beam_reorder; out_ids has room for max_history ids
     of every new row.  The caller keeps the tensors."""
-    _ints("beam_history", max_history)
+    if not -0x80000000 <= max_history <= 0x7fffffff:
+        raise ValueError(_WIDE.format("beam_history"))
     dev = off.get_device()
     some = (off, ids, out_off, out_ids) if tokens is None else (off, ids, out_off, out_ids, tokens)
     for t in some:
@@ -429,7 +428,8 @@ def beam_reorder(parents: torch.Tensor, beams: int, n_out: int, states=(), histo
     total = parents.numel()
     _want(beams > 0 and n_out > 0 and total % n_out == 0, "parents: whole groups of n_out are wanted")
     groups = total // n_out
-    _ints("beam_reorder", beams, n_out, groups)
+    if (beams | n_out | groups) >> 31:
+        raise ValueError(_WIDE.format("beam_reorder"))
     for s in states:
         _want(s.rows[0] >= groups * beams and s.rows[1] >= total, "states: fewer rows than the groups have")
         _want(s.rows[2] == dev and s.rows[3] == dev, "states: tensors on the call's device are wanted")
