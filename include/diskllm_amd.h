@@ -261,10 +261,11 @@ int dlk_softcap(float *logits, int64_t ld, int rows, int vocab, float cap, hipSt
 
 /* Row-wise symmetric quantisation: scale[r] = max_i |x[r * ldx + i]| / 127 (one
  * float rounding), q[r * ldq + i] = x / scale[r] to the nearest integer, halves to
- * even, decided exactly; within +-127.  A row of zeros: scale 0 and zeros.  A row
- * that holds NaN or infinity: scale NaN and zeros, so its logits are NaN.  Hidden
- * states take it per token, weights [vocab, n] once per channel.  x, q and scale
- * need the alignment of their elements only; strides are in elements. */
+ * even, decided exactly; within +-127.  A row of zeros, or of values so small that the
+ * scale rounds to 0: scale 0 and zeros.  A row that holds NaN or infinity: scale NaN and
+ * zeros, so its logits are NaN.  Hidden states take it per token, weights [vocab, n] once
+ * per channel.  x, q and scale need the alignment of their elements only and may not
+ * overlap; strides are in elements. */
 int dlk_quantize_rows(const void *x, int dtype, int64_t ldx, int rows, int n, int8_t *q, int64_t ldq, float *scale,
                       hipStream_t stream);
 
@@ -273,8 +274,10 @@ int dlk_quantize_rows(const void *x, int dtype, int64_t ldx, int rows, int n, in
  * three float roundings (the sum's, and one per scale); softcap > 0: then softcap *
  * tanh(logit / softcap) to 2^-20 of it, or to 2^-148 * softcap or 2^-149 (the smallest
  * float) where one of those is more (not libm's bits, which dlk_softcap gives); softcap
- * must be finite.  Any strides and byte alignment of x and w.  Entries past vocab in a
- * row of logits are left as they are. */
+ * must be finite.  Any strides and byte alignment of x and w; where both are 16-byte
+ * aligned with strides that are multiples of 16, the 16 bytes that hold a row's last entry
+ * are read to their end (what stands there does not matter).  Entries past vocab in a
+ * row of logits are left as they are; logits may not overlap the inputs. */
 int dlk_logits_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8_t *w, int64_t ldw,
                   const float *w_scale, int rows, int vocab, int n, float softcap, float *logits, int64_t ld,
                   hipStream_t stream);
