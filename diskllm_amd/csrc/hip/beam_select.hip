@@ -22,13 +22,15 @@
  * neighbouring candidates differ; 64-bit FMAs run at the plain 32-bit ones' rate here.
  *
  * Bounds.  Large calls: reads, with what starts and ends a workgroup (512 x 262,144, 1 of 20
- * allowed: 126 us, 4.4 TB/s; with a list and barriers common to the waves and every logit
+ * allowed: 129 us, 4.3 TB/s; with a list and barriers common to the waves and every logit
  * summed 145).  Calls that fit the chip once: the chain of a slice and the merge (64 x
  * 151,936 with penalties 32 us, of which 20 a slice's at the median, 28 at the last, 5 the
- * merge's; 128 x 50,257 in groups of 16 24.3, 16 and 8).  A history costs 12 us of 504 x
- * 64,960 with 64 ids and 30 with 1,000 (57, 68, 87; with every wave looking through all of
- * it and ids put into place one by one 154).  Small ones: a dozen round trips
- * one after another (4 x 32,000: 10.5 us).  The next batch's loads ahead of this one's work
+ * merge's; 128 x 50,257 in groups of 16 25.5, 16 and 8).  A history costs 13 us of 504 x
+ * 64,960 with 64 ids and 31 with 1,000 of no order (53, 65, 84; with every wave looking through
+ * all of it and ids put into place one by one 154); 107 where they are Zipf's and the common ones
+ * the lowest, so that they are some few waves' (64 x 151,936: none 27, 256 ids 32 and 37,
+ * 1,000 35 and 59), as a wave holds 128 occurrences and looks through the history in
+ * every batch past that.  Small ones: a dozen round trips one after another (4 x 32,000: 11.5 us).  The next batch's loads ahead of this one's work
  * changed nothing: other workgroups' waves fill that time.
  */
 #include "dlk_device.h"
@@ -39,7 +41,7 @@ namespace dlk {
 
 constexpr int kBeamList = 512;         /* entries that a merge orders at once */
 constexpr int kBeamWaveList = 256;     /* and that a wave lists of a slice */
-constexpr int kBeamSaid = 128;         /* history ids that a wave holds */
+constexpr int kBeamSaid = 128;         /* occurrences of a history's ids that a wave holds */
 constexpr int kBeamPacked = 512;       /* of a wave's 1,024 logits: so many allowed ones or fewer are packed */
 
 DLK_DEV void bpub64(uint64_t *a, uint64_t v) { __hip_atomic_store(a, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -167,7 +169,7 @@ struct BeamShared {
     double part[kBeamThreads / 64];
     float cum[DLK_MAX_BEAMS];
     float top[DLK_MAX_BEAMS];
-    float best_score;                   /* of the group, over the lengths' norm */
+    float above;                        /* no key of the group is above it */
     uint32_t wave_key[kBeamThreads / 64];
     int wave_n[kBeamThreads / 64], wave_listed[kBeamThreads / 64];
     int place[kBeamList];               /* row of each entry */
@@ -229,8 +231,9 @@ struct BeamRow {
     /* the score of entry e in 64 bits, and its key */
     DLK_DEV double score(uint64_t e) const { return over ? cum : cum + (((double)entry_logit(e) - top) - base); }
     DLK_DEV uint64_t key(uint64_t e) const { return double_key(score(e) * norm); }
-    /* that as a word, by its distance from the group's best (to 2^-11 of it, whatever the scores' size is); never 0 */
-    DLK_DEV uint32_t word(uint64_t e, double best) const { return ~f2u(fmaxf((float)(best - score(e) * norm), 0.0f)); }
+    /* that as a word, by its distance from a float that no key of the group is above (to 2^-11 of it, whatever the scores'
+     * size is); never 0 */
+    DLK_DEV uint32_t word(uint64_t e, double above) const { return ~f2u((float)(above - score(e) * norm)); }
 };
 
 DLK_DEV void write_continuation(const BeamParams &p, const BeamShared &sh, int g, int j, int b, uint64_t e) {
@@ -321,8 +324,8 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
         }
     }
     __syncthreads();
-    /* what each row adds to its continuations, a lane each; and the group's best key, rounded to float: a row's best
-     * entry is its maximum */
+    /* what each row adds to its continuations, a lane each; and the float after the group's best key (a row's best entry
+     * is its maximum) */
     float most = -INFINITY;
     if (t < p.beams) {
         const int64_t row = (int64_t)g * p.beams + t;
@@ -343,10 +346,11 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
     }
     if (wave == 0) {
         most = wave_max_dpp(most);
-        if (t == 0) sh.best_score = most;
+        const uint32_t u = f2u(most);
+        if (t == 0) sh.above = u2f(most > 0.0f ? (most < INFINITY ? u + 1 : u) : most < 0.0f ? u - 1 : 1u);
     }
     __syncthreads();
-    const double best_score = (double)sh.best_score;
+    const double above = (double)sh.above;
     /* list i of row b: its entries (a finished row's first list holds its one continuation) */
     auto listed = [&](int i, int b) {
         const int kind = sh.kind[b];
@@ -381,7 +385,7 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
                     if (e0 + q * T >= E) continue;
                     const int place = place_of(e0 + q * T), at = min(place, E - 1), i = list_of(at), b = row_of(i);
                     if (sh.kind[b] == 2) pre[q] = ~(uint64_t)0;
-                    if (place < E && at - i * p.n < listed(i, b)) word[q] = BeamRow(sh, b).word(pre[q], best_score);
+                    if (place < E && at - i * p.n < listed(i, b)) word[q] = BeamRow(sh, b).word(pre[q], above);
                     best = max(best, word[q]);
                 }
             }
@@ -506,8 +510,8 @@ __global__ __launch_bounds__(kBeamThreads, 5) void beam_select_kernel(BeamParams
     if (!idle) {
         uint64_t *list = sh.list[wave];
         int listed = 0;
-        /* The history's ids among this wave's logits, two a lane, penalised once and put into their places
-         * batch by batch; more than 128 are counted in LDS in each batch. */
+        /* The history's ids among this wave's logits, two a lane (each as often as it occurs), penalised once
+         * and put into their places batch by batch; more than 128 are counted in LDS in each batch. */
         auto wave_of = [&](int32_t id) { return ((id - s0) >> 8) & 3; };
         int said = 0;
         int32_t mine[2] = {-1, -1};

@@ -939,3 +939,20 @@ def test_select_near_beams_cost_no_more(cuda, groups, beams, V):
     import torch
     few = np.tile(np.where(np.arange(beams) == 0, -5.0, -5000.0), groups).astype(np.float32)
     assert_costs_alike(torch, groups, beams, 64, V, few, late(np.random.default_rng(4), groups, beams, -5.0))
+
+
+def test_select_scores_beside_zero(cuda):
+    """Scores so small, on both sides of 0, that their distances over the lengths are no floats: still in order."""
+    import torch
+    rng = np.random.default_rng(8)
+    rows = 64
+    lg = np.full((rows, 3), -np.inf, np.float32)
+    lg[:, 1] = rng.normal(0, 3, rows)                  # one continuation a row, its log-softmax 0
+    for sign in (1.0, -1.0, 0.0):
+        s = (10.0 ** rng.uniform(-44, -36, rows) * (sign or rng.choice([-1, 1], rows))).astype(np.float32)
+        s = np.unique(s)
+        s = rng.permutation(s)[:len(s) // 16 * 16]
+        n = len(s)
+        check(torch, lg[:n], 16, 5, scores=s, lengths=np.full(n, 500, np.int32), alpha=16.0)
+        check(torch, lg[:n], 16, 16, scores=s, lengths=np.full(n, 500, np.int32), alpha=16.0)
+        check(torch, lg[:n], 16, 5, scores=s)
