@@ -12,8 +12,9 @@
  * alignment.  A thread has as many rows' bytes in registers as a group has rows (rounded
  * up to 4, 8, .. 64): the loads of a column are in flight together.
  *
- * 16 requests of 4 beams with 2.7 GB of cache, two thirds of the rows moving: 476-516 us, a large copy's
- * 5.1 to 5.6 TB/s, read and written.  A request's few small states: 4-5 us (13.5 with the
+ * 16 requests of 4 beams with two caches of 1.07 GB, two thirds of the rows moving, 2.7 GB read and
+ * written: 476-565 us by the parents and the box (531-561 under the profiler), 4.8 to 5.6 TB/s, a large
+ * copy's rate (5.1).  A request's few small states: 4-5 us (13.5 with the
  * host's checks of the tensors), all of them and the histories in one launch.
  *
  * A history's place in the CSR is the sum of the lengths before it, which the workgroups of

@@ -6,19 +6,25 @@
  * of n matters: no tile or split changes a bit.  w is the instruction's first operand: a
  * lane's four results are then four neighbouring ids of one row, one 16-byte store.
  *
- * Bounds.  Up to some 256 rows w's bytes: each is read from memory once (the tiles of x for
+ * Bounds.  Up to 128 rows w's bytes: each is read from memory once (the tiles of x for
  * one tile of w lie side by side on one XCD), and what it takes is loads in flight: both
  * operands go straight into an LDS ring (global_load_lds, 16 bytes a lane), which costs no
  * registers and no waits but one barrier a step.  16 x 151,936 x 4,096 takes 114-116 us,
  * 5.5-5.7 TB/s (a large copy: 5.1); 1 x 32,000 x 2,048 11.5, 5.7 TB/s.  Above that the
- * products and what feeds them: 512 x 262,144 x 4,096 with the cap in 606-614 us,
- * 1,790-1,810 TOP/s, of which some 150 cap and write 537 MB of logits after each workgroup's
+ * products and what feeds them: 512 x 262,144 x 4,096 with the cap in 605-639 us (by the box and its
+ * clock), 1,720-1,820 TOP/s, of which some 150 cap and write 537 MB of logits after each workgroup's
  * loop; the loop alone runs at 2,440, as a library product of 16,384^3 does.  It has the
  * loads into LDS at about 12 TB/s, where shorter steps, a third stage of w, another order of n
  * and stores that bypass the caches gave nothing; tiles of 256 x 256 ask for the fewest bytes.
  *
+ * Between 129 and 511 rows neither is reached: tiles leave rows empty (300 are computed as 384),
+ * and 147 KB of stages leave one workgroup a CU, with nothing beside its epilogue: 200 x
+ * 151,936 x 4,096 215 us and 300 rows 282, where the bytes are 147 and 159 at a copy's rate.  And
+ * tiles go by the rows alone, not by the rounds of the CUs that they make: 512 x 100,000 x 1,200,
+ * 3.05 rounds, takes 131 where the operations are 64.
+ *
  * Rows that are not 16-byte aligned cannot go that way: they go through registers
- * (logits_i8_any_kernel; 33 x 50,257 x 2,047 33.5 us, 3.3 TB/s, in padded rows 27).  Their
+ * (logits_i8_any_kernel; 33 x 50,257 x 2,047 33.3-35.9 us, 3.1-3.3 TB/s, in padded rows 27).  Their
  * 16-byte loads are what it waits for: both stages wholly in flight (no branch in the loop) or
  * steps twice as long were no faster, nor was loading the rows' own chunks into LDS and
  * reading fragments at each row's shift (59 us: unaligned LDS reads).

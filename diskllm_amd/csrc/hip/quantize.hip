@@ -11,8 +11,8 @@
  *
  * Bound by memory for many rows, by latency for few: each row is read once into
  * registers (the maximum, then the values), up to 8,192 entries; longer rows are read
- * a second time.  50,257 x 4,096 float32 takes 200 us, 5.1 TB/s read and written (a large
- * copy's rate); 1 x 4,096 bf16 3.3, a launch and one round trip.  A workgroup a row, so
+ * a second time.  50,257 x 4,096 takes 181-202 us in float32, 5.1-5.7 TB/s read and written (a
+ * large copy: 5.1), 131-135 in bfloat16 and float16, 4.6-4.7; 1 x 4,096 bf16 3.3, a launch and one round trip.  A workgroup a row, so
  * that one row has 256 threads' loads in flight; rows of up to 1,024 entries, of which that
  * would leave most threads idle, a wave each.  Rows of any stride: 16-byte loads need no
  * more than the type's own alignment here.
