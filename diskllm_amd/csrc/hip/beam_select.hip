@@ -274,15 +274,17 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
      * of many lists (n a power of two), the best of the threads be those of a few places, and
      * more reach their bound than are ranked at once (16 x 2 x 151,936 of 64, beams near one another:
      * 36 us, 102 that way; 16 x 4 52, 142) */
-    auto place_of = [&](int e) {
+    auto place_of = [&](int m, int e0, int q) { return e0 + q * T + (m ^ (q * 37 & (T - 1))); };
+    auto this_thread = [&]() {
         int m = mine;
-        asm volatile("" : "+v"(m));                          /* (places kept are 16 registers) */
-        return e + ((m + e / T * 37) & (T - 1));
+        asm volatile("" : "+v"(m));                          /* (places kept from loop to loop are 16 registers) */
+        return m;
     };
     auto load = [&](int e0) {
+        const int m = this_thread();
 #pragma unroll
         for (int q = 0; q < PRE; q++)
-            if (e0 + q * T < E) pre[q] = bget64(&cands[min(place_of(e0 + q * T), E - 1)]);
+            if (e0 + q * T < E) pre[q] = bget64(&cands[min(place_of(m, e0, q), E - 1)]);
     };
     if (t < L) {
         const uint64_t mk = bget64(&slots[t].max_kept);
@@ -379,21 +381,23 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
         for (int e0 = 0; e0 < E; e0 += PRE * T) {
             if (pass == 0 || E > PRE * T) {
                 if (pass > 0 || e0 > 0) load(e0);
+                const int m = this_thread();
 #pragma unroll
                 for (int q = 0; q < PRE; q++) {              /* (few entries: few instructions, fetched for the first time) */
                     word[q] = 0;
                     if (e0 + q * T >= E) continue;
-                    const int place = place_of(e0 + q * T), at = min(place, E - 1), i = list_of(at), b = row_of(i);
+                    const int place = place_of(m, e0, q), at = min(place, E - 1), i = list_of(at), b = row_of(i);
                     if (sh.kind[b] == 2) pre[q] = ~(uint64_t)0;
                     if (place < E && at - i * p.n < listed(i, b)) word[q] = BeamRow(sh, b).word(pre[q], above);
                     best = max(best, word[q]);
                 }
             }
             if (pass == 0) continue;
+            const int m = this_thread();
 #pragma unroll
             for (int q = 0; q < PRE; q++) {
                 if (word[q] == 0 || word[q] < bound) continue;
-                const int b = row_of(list_of(place_of(e0 + q * T)));
+                const int b = row_of(list_of(place_of(m, e0, q)));
                 add(BeamRow(sh, b).key(pre[q]), pre[q], b);
             }
         }
