@@ -369,7 +369,7 @@ DLK_DEV void merge_group(const BeamParams &p, int gl, BeamShared &sh) {
     /* every entry's word for the bound, then those that reach it: PRE * T at a time, which are
      * kept from one to the other where they are all.  The bound has a word's 20 leading bits: of the
      * distance from the best, so that it is as close where scores are large (16 x 16 x 128,256
-     * of 32: 73 us at scores of -20, 76 at -2,500; bits of the scores themselves were 8 apart there,
+     * of 32: 71 us at scores of -20, 72 at -2,500; bits of the scores themselves were 8 apart there,
      * more reached it than are ranked at once, and it took 125). */
     uint32_t word[PRE], best = 0, bound = 0;                 /* 0: none */
     const float per_n = 1.0f / (float)p.n, per_slices = 1.0f / (float)p.slices;
