@@ -1,9 +1,9 @@
 """The LM head in 4 bits and the scoring of its answers, and what they are measured on.
 
-  quantise   dlk_quantize_mx and dlk_dequantize_mx: blocks of 32 values with a power-of-two scale, in 4 or 8 bits, and
+  quantise   dlk_quantize_mx and dlk_dequantize_mx: blocks of 32 values with a power-of-two scale, in 4 or 6 bits, and
              the values they stand for
   embed      dlk_dequantize_mx by token ids: rows of a tied 4-bit table
-  logits     dlk_logits_mx: the LM head's product with 4-bit weights and 4- or 8-bit hidden states, soft-cap
+  logits     dlk_logits_mx: the LM head's product with 4-bit weights and 4- or 6-bit hidden states, soft-cap
   logprobs   dlk_token_logprobs: log-probabilities of given tokens, entropy, the most likely alternatives
   grad       dlk_token_logprobs_grad: the logits' gradient of those log-probabilities and of the entropy
 
@@ -41,7 +41,7 @@ def _grad(name, rows, vocab, dtype, given=1, entropy=True, allowed=0.0, temp=1.0
 def listed():
     return [
         # one token's hidden state before the LM head: latency alone
-        _quantise("quantise 1x4096 bf16 fp8", 1, 4096, "bf16", "fp8"),
+        _quantise("quantise 1x4096 bf16 fp6", 1, 4096, "bf16", "fp6"),
         # an LM head's weights when a model is loaded, rows that end inside a block
         _quantise("quantise 100001x4090 bf16 fp4", 100001, 4090, "bf16", "fp4"),
         # the embedding rows of a decode step's tokens, of a tied table
@@ -50,8 +50,8 @@ def listed():
         _embed("embed 8192x4096 f32", 8192, 151936, 4096, "f32"),
         # one token of a small model
         _product("logits 1x32000x2048 fp4", 1, 32000, 2048, "fp4"),
-        # a decode step of a small batch, hidden states in 8 bits: the weights are streamed once
-        _product("logits 16x151936x4096 fp8", 16, 151936, 4096, "fp8"),
+        # a decode step of a small batch, hidden states in 6 bits: the weights are streamed once
+        _product("logits 16x151936x4096 fp6", 16, 151936, 4096, "fp6"),
         # a large decode step of a model with soft-capped logits
         _product("logits 512x262144x4096 cap", 512, 262144, 4096, "fp4", cap=30.0),
         # one sampled token and its alternatives, as a chat request asks for them
@@ -87,15 +87,15 @@ def draw(rng):
     op = rng.choice(["quantise", "embed", "logits", "logits", "logprobs", "logprobs", "grad"])
     if op == "quantise":
         rows = min(_log_int(rng, 1, 100001), MOST_VALUES // n)
-        c = _quantise("", rows, n, rng.choice(["bf16", "f16", "f32"]), rng.choice(["fp4", "fp4", "fp8"]))
+        c = _quantise("", rows, n, rng.choice(["bf16", "f16", "f32"]), rng.choice(["fp4", "fp4", "fp6"]))
     elif op == "embed":
         vocab = min(vocab, MOST_WEIGHTS // n)
         rows = min(_log_int(rng, 1, 8192), MOST_EMBEDDED // n)
         c = _embed("", rows, vocab, n, rng.choice(["bf16", "f16", "f32"]))
     elif op == "logits":
         vocab = min(vocab, MOST_WEIGHTS // n)
-        fmt = rng.choice(["fp4", "fp8"])
-        rows = max(1, min(_log_int(rng, 1, 512), MOST_PRODUCT // (n * vocab * (2 if fmt == "fp8" else 1))))
+        fmt = rng.choice(["fp4", "fp6"])
+        rows = max(1, min(_log_int(rng, 1, 512), MOST_PRODUCT // (n * vocab)))
         c = _product("", rows, vocab, n, fmt, cap=rng.choice([0.0, 0.0, 30.0]))
     else:
         dtype = rng.choice(["bf16", "f16", "f32"])
@@ -115,7 +115,8 @@ def draw(rng):
 DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 SIZE = {"bf16": 2, "f16": 2, "f32": 4}
 DEV = "cuda"
-FP4 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+GRIDS = {"fp4": (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0),
+         "fp6": tuple(i / 8 for i in range(16)) + tuple(i / 4 for i in range(8, 16)) + tuple(i / 2 for i in range(8, 16))}
 
 
 def _gen(seed):
@@ -233,10 +234,10 @@ def _blocks(x):
 def _rounded(x, fmt):
     """The values that x [rows, n] is held as, and the exponents of its blocks' scales."""
     b, e = _blocks(x)
-    e = (e - (2 if fmt == "fp4" else 8)).clamp(-127, 127)
+    e = (e - 2).clamp(-127, 127)
     t = _times2(b, -e)
-    low, bits, most = (0, 1, 6.0) if fmt == "fp4" else (-6, 3, 448.0)
-    step = (torch.frexp(t).exponent - 1).clamp(min=low) - bits
+    bits, most = (1, 6.0) if fmt == "fp4" else (3, 7.5)
+    step = (torch.frexp(t).exponent - 1).clamp(min=0) - bits
     t = _times2(torch.round(_times2(t, -step)), step).clamp(-most, most)
     return t, e
 
@@ -245,12 +246,18 @@ def _encode(x, fmt):
     """x in the layout of dlk_quantize_mx: bytes and scales."""
     t, e = _rounded(x, fmt)
     rows, blocks = t.shape[:2]
+    grid = torch.tensor(GRIDS[fmt], dtype=torch.float64, device=DEV)
+    code = torch.bucketize(t.abs(), grid) + len(grid) * (t < 0)
     if fmt == "fp4":
-        code = torch.bucketize(t.abs(), torch.tensor(FP4, dtype=torch.float64, device=DEV)) + 8 * (t < 0)
         code = code.view(rows, -1, 2)
         q = (code[..., 0] + 16 * code[..., 1]).to(torch.uint8)
     else:
-        q = t.float().to(torch.float8_e4m3fn).view(torch.uint8).reshape(rows, -1)
+        code = code.view(rows, -1, 4)                        # four values in three bytes, the first lowest
+        word = code[..., 0] + (code[..., 1] << 6) + (code[..., 2] << 12) + (code[..., 3] << 18)
+        held = torch.stack((word & 255, word >> 8 & 255, word >> 16), 2).to(torch.uint8).view(rows, -1)
+        q = torch.zeros((rows, (blocks * 24 + 15) // 16 * 16), dtype=torch.uint8, device=DEV)
+        q[:, :blocks * 24] = held
+        q = q[:, :blocks * 24]
     scale = torch.zeros((rows, (blocks + 15) // 16 * 16), dtype=torch.uint8, device=DEV)
     scale[:, :blocks] = (e + 127).squeeze(2)
     return q, scale[:, :blocks]
@@ -269,10 +276,12 @@ def _decode(q, scale):
     """Float32 values of rows of blocks."""
     rows, blocks = scale.shape
     if q.shape[1] == blocks * 16:
-        code = torch.stack((q & 15, q >> 4), dim=2).int()
-        v = torch.tensor(FP4 + tuple(-f for f in FP4), device=DEV)[code]
+        code, grid = torch.stack((q & 15, q >> 4), dim=2).int(), GRIDS["fp4"]
     else:
-        v = q.view(torch.float8_e4m3fn).float()
+        b = q.reshape(rows, -1, 3).int()
+        word = (b[..., 0] + (b[..., 1] << 8) + (b[..., 2] << 16)).unsqueeze(2)
+        code, grid = word >> torch.tensor((0, 6, 12, 18), device=DEV) & 63, GRIDS["fp6"]
+    v = torch.tensor(grid + tuple(-f for f in grid), device=DEV)[code]
     # (a scale's bits are a float's exponent)
     by = torch.where(scale == 0, 2.0 ** -127, (scale.int() << 23).view(torch.float32))
     return (v.reshape(rows, blocks, 32) * by.unsqueeze(2)).view(rows, blocks * 32)
@@ -397,14 +406,14 @@ def work(case):
         blocks = (case["n"] + 31) // 32
     if op == "quantise":
         n = rows * case["n"]
-        held = rows * blocks * (17 if case["fmt"] == "fp4" else 33)
+        held = rows * blocks * (17 if case["fmt"] == "fp4" else 25)
         # the values, the blocks, and what those stand for
         return {"bytes": 2 * n * SIZE[case["dtype"]] + 2 * held, "flops": 6 * n}
     if op == "embed":
         return {"bytes": rows * (blocks * 17 + 4 + case["n"] * SIZE[case["dtype"]]), "flops": rows * case["n"]}
     if op == "logits":
         V = case["vocab"]
-        x = rows * blocks * (17 if case["fmt"] == "fp4" else 33)
+        x = rows * blocks * (17 if case["fmt"] == "fp4" else 25)
         return {"bytes": x + V * blocks * 17 + 4 * rows * V, "flops": 2 * rows * V * case["n"]}
     V = case["vocab"]
     b = rows * V * SIZE[case["dtype"]] + rows * (8 * case["given"] + 16)
@@ -424,14 +433,11 @@ def _powers():
 
 def _grid(fmt):
     """The magnitudes of an element format."""
-    if fmt == "fp4":
-        exps, bits, low, codes = 2, 1, 0, 8
-    else:
-        exps, bits, low, codes = 4, 3, -6, 127
+    bits = 1 if fmt == "fp4" else 3
     v = []
-    for code in range(codes):
+    for code in range(4 << bits):
         ex, m = code >> bits, code & ((1 << bits) - 1)
-        v.append(m * 2.0 ** (low - bits) if ex == 0 else (1 + m / 2.0 ** bits) * 2.0 ** (ex - 1 + low))
+        v.append(m / 2.0 ** bits if ex == 0 else (1 + m / 2.0 ** bits) * 2.0 ** (ex - 1))
     return torch.tensor(v, dtype=torch.float64, device=DEV)
 
 
@@ -440,7 +446,7 @@ def _exact_quantise(case, s):
     grid, powers = _grid(case["fmt"]), _powers()
     x = s["x"]
     out = torch.empty(x.shape, dtype=torch.float64, device=DEV)
-    emax = math.floor(math.log2(grid[-1].item()))
+    emax = 2
     for r in range(0, x.shape[0], 4096):
         for i in range(0, x.shape[1], 32 * 16):
             part = x[r:r + 4096, i:i + 512].to(torch.float64)
@@ -457,11 +463,13 @@ def _exact_quantise(case, s):
 
 
 def _exact_rows(q, scale):
-    grid = _grid("fp4" if q.shape[1] == scale.shape[1] * 16 else "fp8")
-    if len(grid) == 8:
-        q = torch.cat((q.unsqueeze(2) % 16, q.unsqueeze(2) // 16), 2).flatten(1)
-    half = 8 if len(grid) == 8 else 128
-    v = grid[(q % half).long()] * (1.0 - 2.0 * (q >= half))
+    width = q.shape[1] * 8 // (scale.shape[1] * 32)          # bits of a value
+    grid = _grid("fp%d" % width)
+    bit = q.unsqueeze(2) >> torch.arange(8, device=DEV, dtype=torch.uint8) & 1
+    bit = bit.reshape(q.shape[0], -1, width).to(torch.float64)
+    code = (bit * torch.tensor([2.0 ** k for k in range(width)], dtype=torch.float64, device=DEV)).sum(2).long()
+    half = 2 ** (width - 1)
+    v = torch.where(code >= half, -1.0, 1.0) * grid[code % half]
     return v * _powers()[scale.long()].repeat_interleave(32, 1)
 
 
