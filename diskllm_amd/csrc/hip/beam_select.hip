@@ -35,6 +35,7 @@
  */
 #include "dlk_device.h"
 #include "beam_select.h"
+#include "top_list.h"
 #include "../../../include/diskllm_amd.h"
 
 namespace dlk {
@@ -43,11 +44,6 @@ constexpr int kBeamList = 512;         /* entries that a merge orders at once */
 constexpr int kBeamWaveList = 256;     /* and that a wave lists of a slice */
 constexpr int kBeamSaid = 128;         /* occurrences of a history's ids that a wave holds */
 constexpr int kBeamPacked = 512;       /* of a wave's 1,024 logits: so many allowed ones or fewer are packed */
-
-DLK_DEV void bpub64(uint64_t *a, uint64_t v) { __hip_atomic_store(a, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-DLK_DEV uint64_t bget64(const uint64_t *a) {
-    return __hip_atomic_load((uint64_t *)a, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
 
 /* a * b + c with c in scalar registers and its own destination (the compiler's choice adds
  * a move of c for each). */
@@ -83,25 +79,6 @@ DLK_DEV double exp_neg(double x) {
     return __hiloint2double(__double2hiint(y) + (__double2loint(t) << 20), __double2loint(y));
 }
 
-/* x where bit c of `bits` is set, else -inf (a bit field's sign, a bitwise choice). */
-DLK_DEV float allowed_or_ninf(float x, uint32_t bits, int c) {
-    const uint32_t m = (uint32_t)((int)(bits << (31 - c)) >> 31);
-    return u2f((f2u(x) & m) | (0xff800000u & ~m));
-}
-
-/* The larger of three (NaN: of the others): one instruction, where fmaxf makes one for each
- * value to quiet it. */
-DLK_DEV float max3(float a, float b, float c) {
-    float d;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-    return d;
-}
-
-/* An entry of a list: larger is better (the logit's ascending key, then the lower id). */
-DLK_DEV uint64_t entry_of(float l, int id) { return (uint64_t)~desc_key(l) << 32 | (uint32_t)~id; }
-DLK_DEV float entry_logit(uint64_t e) { return key_value(~(uint32_t)(e >> 32)); }
-DLK_DEV int entry_id(uint64_t e) { return (int)~(uint32_t)e; }
-
 /* Ascending key of a double (no NaN); zero below every one. */
 DLK_DEV uint64_t double_key(double d) {
     uint64_t u = d2u(d);
@@ -124,28 +101,6 @@ DLK_DEV float beam_penalised(const BeamParams &p, float x, int cnt) {
         }
     }
     return x;
-}
-
-/* A key that at least r of the lanes' keys reach (0: fewer than r lanes have one): the largest
- * for r = 1, else the largest of 20 leading bits (0.5 us where few waves run). */
-DLK_DEV uint32_t wave_rth(uint32_t a, int r) {
-    uint32_t K = 0;
-    if (r == 1) return wave_minmax_u32<false>(a);
-#pragma unroll 1
-    for (uint32_t bit = 0x80000000u; bit >= 0x1000u; bit >>= 1)
-        if ((int)__popcll(ballot(a >= (K | bit))) >= r) K |= bit;
-    return K;
-}
-
-/* Lane's place among the lanes of `who`, from `first` on. */
-DLK_DEV int place_in(uint64_t who, int first) {
-    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, (uint32_t)first));
-}
-
-/* LDS that only this wave writes and reads: its instructions go in order, the compiler has to keep it. */
-DLK_DEV void wave_order() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
 }
 
 /* Maximum over each row of 16 lanes (every lane gets its row's). */
@@ -202,24 +157,6 @@ DLK_DEV bool before(uint64_t ka, int ra, uint64_t ea, uint64_t kb, int rb, uint6
     if (ka != kb) return ka > kb;
     if (ra != rb) return ra < rb;
     return ea > eb;
-}
-
-/* How many of list[0 .. n) are above v, and how many equal to it. */
-DLK_DEV int rank_in(const uint64_t *list, int n, uint64_t v, int &equal) {
-    int above = 0;
-    equal = 0;
-    int c = 0;
-    for (; c + 4 <= n; c += 4) {
-        const ulonglong2 a = *(const ulonglong2 *)&list[c], b = *(const ulonglong2 *)&list[c + 2];
-        above += (a.x > v ? 1 : 0) + (a.y > v ? 1 : 0) + (b.x > v ? 1 : 0) + (b.y > v ? 1 : 0);
-        equal += (a.x == v ? 1 : 0) + (a.y == v ? 1 : 0) + (b.x == v ? 1 : 0) + (b.y == v ? 1 : 0);
-    }
-    for (; c < n; c++) {
-        const uint64_t a = list[c];
-        above += a > v ? 1 : 0;
-        equal += a == v ? 1 : 0;
-    }
-    return above;
 }
 
 /* What a row adds to its continuations, out of LDS once for many of them. */

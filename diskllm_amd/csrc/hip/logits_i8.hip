@@ -33,12 +33,10 @@
 
 #include <hip/hip_runtime.h>
 
-#include "dlk_device.h"
-#include "../../../include/diskllm_amd.h"
+#include "logits_tile.h"
 
 namespace dlk {
 
-typedef int i4 __attribute__((ext_vector_type(4)));
 typedef int i4_any __attribute__((ext_vector_type(4), aligned(1)));
 
 struct I8Params {
@@ -75,39 +73,6 @@ DLK_DEV i4 load16_to(const int8_t *p, int k, int n) {
     const uint64_t l1 = s < 8 ? (lo >> b) | (b ? hi << (64 - b) : 0) : s < 16 ? hi >> b : 0;
     const uint64_t h1 = s < 8 ? hi >> b : 0;
     return i4{(int)(uint32_t)l1, (int)(uint32_t)(l1 >> 32), (int)(uint32_t)h1, (int)(uint32_t)(h1 >> 32)};
-}
-
-/* Waits until at most N of the wave's loads are in flight and its LDS work is done. */
-template <int N>
-DLK_DEV void wait_loads() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (N >> 4) << 14);
-    asm volatile("" ::: "memory");
-}
-
-/* 16-byte chunk c of row r of a staged tile lies at chunk place(r, c): the lanes of a
- * fragment read (16 rows at one or two neighbouring chunks) then meet every bank once. */
-template <int BK>
-DLK_DEV int place(int r, int c) {
-    return BK == 64 ? c ^ ((0x78 >> (2 * ((r >> 2) & 3))) & 3) : BK == 128 ? c ^ (r & 7) : c ^ (r & 15);
-}
-
-/* cap * tanh(y / cap) in some 16 instructions (libm's bits, which dlk_softcap gives, take
- * 65: 240 us of the 512 x 262,144 product against 60).  t = |y| / cap: below 0.35 the
- * series of tanh(t) / t to t^10 (what is left out: 2e-9 of it), above (1 - e) / (1 + e)
- * with e = exp(-2t).  At 0.35, the worst place, e is off by 3.4 half-steps, which 2 e / (1
- * + e)^2 / tanh makes 4.5; with t's own two and those of 1 + e, its reciprocal and the
- * products some 10 half-steps of the result at most.  recip: 1 / cap, finite. */
-DLK_DEV float capped(float y, float cap, float recip) {
-    const float q = y * recip, t = fabsf(q), t2 = t * t;
-    float s = fmaf(t2, -1382.0f / 155925.0f, 62.0f / 2835.0f);
-    s = fmaf(t2, s, -17.0f / 315.0f);
-    s = fmaf(t2, s, 2.0f / 15.0f);
-    s = fmaf(t2, s, -1.0f / 3.0f);
-    s = fmaf(t * t2, s, t);
-    const float e = __builtin_amdgcn_exp2f(-2.88539008177792681f * t);
-    const float b = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
-    return copysignf(t < 0.35f ? s : b, q) * cap;
 }
 
 /* A wave's MF x NF fragments of sums as logits: rows m0 .., ids v0 ...  A fragment's lane
@@ -165,12 +130,6 @@ DLK_DEV void write_logits(const I8Params &p, const i4 (&acc)[MF][NF], int m0, in
     }
 }
 
-/* Loads 16 bytes a lane straight into LDS: lane i's to dst + 16 i (dst the same in all lanes). */
-DLK_DEV void load_to_lds(const int8_t *src, int8_t *dst) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
-                                     (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
-}
-
 /* Of a last, shorter step the chunks past n are copies of the last one (so that all lanes load):
  * this lane's chunk of x at k, once it is in LDS, gets zeros for what is past n.  What w has
  * there does not matter then. */
@@ -184,17 +143,6 @@ DLK_DEV void end_row(int8_t *chunk, int k, int n) {
         v[c] = b >= 4 ? v[c] : b <= 0 ? 0 : v[c] & ((1 << (8 * b)) - 1);
     }
     *(i4 *)chunk = v;
-}
-
-/* One tile's place: workgroups go to the XCDs in turn, so each XCD gets a run of tiles, the
- * tiles of x for one tile of w side by side: w comes from memory once. */
-template <int BM, int BN>
-DLK_DEV bool tile_of(const I8Params &p, int &m0, int &v0) {
-    const int mtiles = (p.rows + BM - 1) / BM, vtiles = (p.vocab + BN - 1) / BN;
-    const int tile = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
-    m0 = tile % mtiles * BM;
-    v0 = tile / mtiles * BN;
-    return tile < mtiles * vtiles;
 }
 
 /* The products of one staged step: x in xs, w in ws, BK bytes a row, chunks at place(). */
@@ -241,7 +189,7 @@ __global__ __launch_bounds__(WGM * WGN * 64, 2) void logits_i8_kernel(I8Params p
     __shared__ __align__(1024) int8_t lds[ST * STAGE];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
     int m0, v0;
-    if (!tile_of<BM, BN>(p, m0, v0)) return;
+    if (!tile_of<BM, BN>(p.rows, p.vocab, m0, v0)) return;
     const int8_t *src[NI];                         /* the row of this lane's chunk */
     int at[NI];                                    /* and its place in the row */
 #pragma unroll
@@ -299,7 +247,7 @@ __global__ __launch_bounds__(WGM * WGN * 64, BM == 32 ? 3 : 4) void logits_i8_an
     __shared__ __align__(1024) int8_t lds[2 * STAGE];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
     int m0, v0;
-    if (!tile_of<BM, BN>(p, m0, v0)) return;
+    if (!tile_of<BM, BN>(p.rows, p.vocab, m0, v0)) return;
     const int8_t *src[NI];
     int at[NI];
 #pragma unroll
@@ -356,7 +304,7 @@ __global__ __launch_bounds__(512, 2) void logits_i8_wide_kernel(I8Params p) {
     int8_t *const ldw = lds + 2 * XST;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
     int m0, v0;
-    if (!tile_of<BM, BN>(p, m0, v0)) return;
+    if (!tile_of<BM, BN>(p.rows, p.vocab, m0, v0)) return;
     const int8_t *sx[NX], *sw[NW];                 /* rows (a wave's loads have one row in eight: one place in all) */
     const int at = place<BK>(lane / 8, lane % 8) * 16;
 #pragma unroll
