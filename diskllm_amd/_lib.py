@@ -25,6 +25,8 @@ DLK_STATUS_UNSUPPORTED_ROW = 4
 DLK_STATUS_NOT_FINITE = 8
 F32, BF16, F16 = 0, 1, 2
 MAX_BEAMS = 64
+MX_FP4, MX_FP6 = 0, 1
+MAX_GIVEN = MAX_ALTERNATIVES = 64
 PATH_AUTO, PATH_ROW, PATH_FULL_EXACT, PATH_FULL_NO_WAIT = 0, 1, 2, 3
 
 OP_REPETITION, OP_FREQUENCY, OP_PRESENCE = 1, 2, 3
@@ -75,6 +77,27 @@ class BeamHistory(C.Structure):
                 ("out_off", C.c_void_p), ("out_ids", C.c_void_p)]
 
 
+class LogprobBatch(C.Structure):
+    """dlk_logprob_batch (include/diskllm_amd.h)."""
+    _fields_ = [("logits", C.c_void_p), ("dtype", C.c_int), ("ld", C.c_int64), ("mask", C.c_void_p),
+                ("mask_ld", C.c_int64), ("mask_row", C.c_void_p), ("tokens", C.c_void_p), ("out_logprobs", C.c_void_p),
+                ("out_stats", C.c_void_p), ("out_top_ids", C.c_void_p), ("out_top_logprobs", C.c_void_p),
+                ("status", C.c_void_p)]
+
+
+class LogprobParams(C.Structure):
+    """dlk_logprob_params (include/diskllm_amd.h)."""
+    _fields_ = [("n_given", C.c_int), ("n_top", C.c_int), ("temperature", C.c_float)]
+
+
+class LogprobGradBatch(C.Structure):
+    """dlk_logprob_grad_batch (include/diskllm_amd.h)."""
+    _fields_ = [("logits", C.c_void_p), ("dtype", C.c_int), ("ld", C.c_int64), ("mask", C.c_void_p),
+                ("mask_ld", C.c_int64), ("mask_row", C.c_void_p), ("tokens", C.c_void_p), ("stats", C.c_void_p),
+                ("grad_logprobs", C.c_void_p), ("grad_entropy", C.c_void_p), ("grad", C.c_void_p),
+                ("ld_grad", C.c_int64)]
+
+
 class SamplerConfig(C.Structure):
     """include/sampler.h:10-16."""
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int), ("top_p", C.c_float), ("min_p", C.c_float),
@@ -111,7 +134,8 @@ EXPORTS = [
     "dlk_seed_state", "dlk_sample", "dlk_sample_noalloc", "dlk_release_stream", "dlk_dfa_mask", "dlk_expf", "dlk_apply_penalties", "dlk_grammar_mode_of",
     "dlk_grammar_row_init", "dlk_grammar_row_feed", "dlk_grammar_mask", "dlk_grammar_advance", "dlk_sample_grammar",
     "dlk_vocab_csr_from_gguf", "dlk_csr_token_str", "dlk_softcap", "dlk_quantize_rows", "dlk_logits_i8",
-    "dlk_beam_select", "dlk_beam_reorder",
+    "dlk_beam_select", "dlk_beam_reorder", "dlk_quantize_mx", "dlk_dequantize_mx", "dlk_logits_mx",
+    "dlk_token_logprobs", "dlk_token_logprobs_grad",
     # include/sampler.h
     "sampler_create", "sampler_free", "sampler_apply_repetition_penalty", "sampler_apply_presence_penalty",
     "sampler_sample", "greedy_sample",
@@ -205,6 +229,21 @@ def lib() -> C.CDLL:
         L.dlk_beam_reorder.restype = C.c_int
         L.dlk_beam_reorder.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.POINTER(BeamState), C.c_int,
                                        C.POINTER(BeamHistory), C.c_void_p]
+        L.dlk_quantize_mx.restype = C.c_int
+        L.dlk_quantize_mx.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int64,
+                                      C.c_void_p, C.c_int64, C.c_void_p]
+        L.dlk_dequantize_mx.restype = C.c_int
+        L.dlk_dequantize_mx.argtypes = [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_int,
+                                        C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_void_p]
+        L.dlk_logits_mx.restype = C.c_int
+        L.dlk_logits_mx.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                    C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_int, C.c_float, C.c_void_p, C.c_int64,
+                                    C.c_void_p]
+        L.dlk_token_logprobs.restype = C.c_int
+        L.dlk_token_logprobs.argtypes = [C.POINTER(LogprobBatch), C.c_int, C.c_int, C.POINTER(LogprobParams), C.c_void_p]
+        L.dlk_token_logprobs_grad.restype = C.c_int
+        L.dlk_token_logprobs_grad.argtypes = [C.POINTER(LogprobGradBatch), C.c_int, C.c_int, C.POINTER(LogprobParams),
+                                              C.c_void_p]
         L.dlk_vocab_csr_from_gguf.restype = C.c_int
         L.dlk_vocab_csr_from_gguf.argtypes = [C.c_char_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int64,
                                               C.POINTER(C.c_int32), C.POINTER(C.c_int64)]

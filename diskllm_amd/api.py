@@ -442,3 +442,172 @@ def beam_reorder(parents: torch.Tensor, beams: int, n_out: int, states=(), histo
         k = len(states)
         arr = (_STATES.get(k) or _lib.BeamState * k)(*states) if k else None
         _call(dev, stream, "dlk_beam_reorder", _lib.lib().dlk_beam_reorder, at, groups, beams, n_out, arr, k, history)
+
+
+# ---- 4-bit logits and scores of tokens ---------------------------------------------
+
+_FORMATS = {"fp4": (_lib.MX_FP4, 16), "fp6": (_lib.MX_FP6, 24)}         # and a block's bytes
+_MX_OF = {16: _lib.MX_FP4, 24: _lib.MX_FP6}
+
+
+def _blocks_of(q: torch.Tensor, scale: torch.Tensor, dev: int, what: str):
+    """(rows, blocks, format, stride, scales' stride) of rows of microscaled blocks; the format by their widths."""
+    rows, width, ldq = _rows2d(q, dev, _U8, what)
+    s_rows, blocks, lds = _rows2d(scale, dev, _U8, what + "_scale")
+    fmt = _MX_OF.get(width // blocks) if blocks and width % blocks == 0 else None
+    if s_rows != rows or fmt is None:
+        raise ValueError(f"{what}: rows of 16 (fp4) or 24 (fp6) bytes for each scale are wanted")
+    return rows, blocks, fmt, ldq, lds
+
+
+def quantize_mx(x: torch.Tensor, fmt: str = "fp4", q: Optional[torch.Tensor] = None,
+                scale: Optional[torch.Tensor] = None, stream: Optional[int] = None):
+    """(q uint8 [rows, blocks * 16 or 24], scale uint8 [rows, blocks]) of x [rows, n] in float32, bfloat16 or float16:
+    blocks of 32 values in 4 bits (weights) or 6 (hidden states), a power of two each (dlk_quantize_mx).  What is made
+    here has the strides that logits_mx wants."""
+    dt = _DTYPES.get(x.dtype)
+    _want(dt is not None, "x: float32, bfloat16 or float16 is wanted")
+    _want(fmt in _FORMATS, "fmt: fp4 or fp6 is wanted")
+    kind, width = _FORMATS[fmt]
+    dev = x.get_device()
+    rows, n, ldx = _rows2d(x, dev, None, "x")
+    blocks = (n + 31) // 32
+    if q is None:
+        ldq = blocks * width
+        q = _empty((rows, ldq), _U8, x, dev, stream)
+    else:
+        q_rows, q_n, ldq = _rows2d(q, dev, _U8, "q")
+        _want(q_rows == rows and q_n == blocks * width, "q: [rows, blocks * 16 or 24] is wanted")
+    if scale is None:
+        lds = (blocks + 15) // 16 * 16
+        scale = _empty((rows, lds), _U8, x, dev, stream)
+        if lds != blocks:
+            scale = scale[:, :blocks]
+    else:
+        s_rows, s_n, lds = _rows2d(scale, dev, _U8, "scale")
+        _want(s_rows == rows and s_n == blocks, "scale: [rows, blocks] is wanted")
+    if rows:
+        _call(dev, stream, "dlk_quantize_mx", _lib.lib().dlk_quantize_mx, x.data_ptr(), dt, ldx, rows, n, kind,
+              q.data_ptr(), ldq, scale.data_ptr(), lds)
+    return q, scale
+
+
+def dequantize_mx(q: torch.Tensor, scale: torch.Tensor, n: Optional[int] = None, ids: Optional[torch.Tensor] = None,
+                  dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None,
+                  stream: Optional[int] = None) -> torch.Tensor:
+    """The first n values (all) of rows of blocks as [rows, n] of dtype; with ids int32 those rows of the table, zeros
+    for an id that it does not have: the embedding rows of tokens (dlk_dequantize_mx)."""
+    dev = q.get_device()
+    table, blocks, fmt, ldq, lds = _blocks_of(q, scale, dev, "q")
+    n = blocks * 32 if n is None else n
+    _want(blocks * 32 - 32 < n <= blocks * 32, "n: values of the last block are wanted")
+    rows, at = table, 0
+    if ids is not None:
+        rows = ids.numel()
+        _want(rows >> 31 == 0, _WIDE.format("dequantize_mx"))
+        at = _flat(ids, 0, dev, _I32, "ids")
+    if out is None:
+        _want(dtype in _DTYPES, "dtype: float32, bfloat16 or float16 is wanted")
+        ld = n
+        out = _empty((rows, n), dtype, q, dev, stream)
+    else:
+        _want(out.dtype in _DTYPES, "out: float32, bfloat16 or float16 is wanted")
+        o_rows, o_n, ld = _rows2d(out, dev, None, "out")
+        _want(o_rows == rows and o_n == n, "out: [rows, n] is wanted")
+    if rows:
+        _call(dev, stream, "dlk_dequantize_mx", _lib.lib().dlk_dequantize_mx, q.data_ptr(), ldq, scale.data_ptr(), lds,
+              table, at, rows, n, fmt, out.data_ptr(), _DTYPES[out.dtype], ld)
+    return out
+
+
+def logits_mx(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, softcap: float = 0.0,
+              out: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> torch.Tensor:
+    """Logits float32 [rows, vocab] of hidden states in microscaled blocks (4 or 6 bits) over 4-bit weights [vocab, ..],
+    soft-capped where softcap > 0 (dlk_logits_mx)."""
+    dev = x.get_device()
+    rows, blocks, fmt, ldx, ldxs = _blocks_of(x, x_scale, dev, "x")
+    V, w_blocks, w_fmt, ldw, ldws = _blocks_of(w, w_scale, dev, "w")
+    _want(w_fmt == _lib.MX_FP4 and w_blocks == blocks, "w: 4-bit rows of x's length are wanted")
+    _want(blocks <= 0x1ffffff, _WIDE.format("logits_mx"))
+    if out is None:
+        ld = (V + 63) // 64 * 64
+        out = _empty((rows, ld), _F32, x, dev, stream)
+        if ld != V:
+            out = out[:, :V]
+    else:
+        o_rows, o_n, ld = _rows2d(out, dev, _F32, "out")
+        _want(o_rows == rows and o_n == V, "out: [rows, vocab] is wanted")
+    if rows:
+        _call(dev, stream, "dlk_logits_mx", _lib.lib().dlk_logits_mx, x.data_ptr(), fmt, ldx, x_scale.data_ptr(), ldxs,
+              w.data_ptr(), ldw, w_scale.data_ptr(), ldws, rows, V, blocks * 32, softcap, out.data_ptr(), ld)
+    return out
+
+
+def _scored(logits: torch.Tensor, tokens: Optional[torch.Tensor], mask, mask_row):
+    """What the forward and the backward call of the scores have in common."""
+    dt = _DTYPES.get(logits.dtype)
+    _want(dt is not None, "logits: float32, bfloat16 or float16 is wanted")
+    dev = logits.get_device()
+    rows, V, ld = _rows2d(logits, dev, None, "logits")
+    given = at = 0
+    if tokens is not None:
+        _want(tokens.dim() in (1, 2) and tokens.shape[0] == rows, "tokens: [rows] or [rows, given] is wanted")
+        given = 1 if tokens.dim() == 1 else tokens.shape[1]
+        at = _flat(tokens, rows * given, dev, _I32, "tokens")
+    mk = mask_ld = 0
+    mr = 0 if mask_row is None else _flat(mask_row, rows, dev, _I32, "mask_row")
+    if mask is not None:
+        m_rows, words, mask_ld = _rows2d(mask, dev, _I32, "mask")
+        _want(words >= (V + 31) // 32 and (mr or m_rows >= rows), "mask: the words of every row are wanted")
+        mk = mask.data_ptr()
+    return dev, dt, rows, V, ld, given, at, mk, mask_ld, mr
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, top: int = 0,
+                   mask: Optional[torch.Tensor] = None, mask_row: Optional[torch.Tensor] = None,
+                   temperature: float = 1.0, out: Optional[dict] = None, status: Optional[torch.Tensor] = None,
+                   stream: Optional[int] = None) -> dict:
+    """Scores of tokens int32 [rows] or [rows, given] under logits [rows, vocab] in float32, bfloat16 or float16
+    (dlk_token_logprobs): logprobs (tokens' shape, or None without tokens), entropy [rows], stats [rows, 4] (for
+    token_logprobs_grad; entropy is its column 2), and top_ids, top_logprobs [rows, top] (None without)."""
+    dev, dt, rows, V, ld, given, at, mk, mask_ld, mr = _scored(logits, tokens, mask, mask_row)
+    if not 0 <= top <= 0x7fffffff:
+        raise ValueError(_WIDE.format("token_logprobs"))
+    if out is None:
+        stats = _empty((rows, 4), _F32, logits, dev, stream)
+        out = dict(logprobs=None if tokens is None else _empty(tokens.shape, _F32, logits, dev, stream), stats=stats,
+                   entropy=stats[:, 2], top_ids=_empty((rows, top), _I32, logits, dev, stream) if top else None,
+                   top_logprobs=_empty((rows, top), _F32, logits, dev, stream) if top else None)
+    lp = _flat(out["logprobs"], rows * given, dev, _F32, "logprobs") if given else 0
+    st = _flat(out["stats"], rows * 4, dev, _F32, "stats")
+    ti = _flat(out["top_ids"], rows * top, dev, _I32, "top_ids") if top else 0
+    tl = _flat(out["top_logprobs"], rows * top, dev, _F32, "top_logprobs") if top else 0
+    bits = 0 if status is None else _flat(status, 1, dev, _I32, "status")
+    if rows:
+        _call(dev, stream, "dlk_token_logprobs", _lib.lib().dlk_token_logprobs,
+              _lib.LogprobBatch(logits.data_ptr(), dt, ld, mk, mask_ld, mr, at, lp, st, ti, tl, bits), rows, V,
+              _lib.LogprobParams(given, top, temperature))
+    return out
+
+
+def token_logprobs_grad(logits: torch.Tensor, tokens: Optional[torch.Tensor], stats: torch.Tensor,
+                        grad_logprobs: Optional[torch.Tensor], *, grad_entropy: Optional[torch.Tensor] = None,
+                        mask: Optional[torch.Tensor] = None, mask_row: Optional[torch.Tensor] = None,
+                        temperature: float = 1.0, out: Optional[torch.Tensor] = None,
+                        stream: Optional[int] = None) -> torch.Tensor:
+    """The gradient of the logits, in their type, of token_logprobs' logprobs and entropy, given theirs
+    (dlk_token_logprobs_grad); stats as the forward call left them, out = logits: in place."""
+    dev, dt, rows, V, ld, given, at, mk, mask_ld, mr = _scored(logits, tokens, mask, mask_row)
+    st = _flat(stats, rows * 4, dev, _F32, "stats")
+    _want(given == 0 or grad_logprobs is not None, "grad_logprobs: a value for each token is wanted")
+    g = _flat(grad_logprobs, rows * given, dev, _F32, "grad_logprobs") if given else 0
+    h = 0 if grad_entropy is None else _flat(grad_entropy, rows, dev, _F32, "grad_entropy")
+    if out is None:
+        out = _empty((rows, V), logits.dtype, logits, dev, stream)
+    o_rows, o_n, ld_out = _rows2d(out, dev, logits.dtype, "out")
+    _want(o_rows == rows and o_n == V, "out: logits' shape is wanted")
+    if rows:
+        _call(dev, stream, "dlk_token_logprobs_grad", _lib.lib().dlk_token_logprobs_grad,
+              _lib.LogprobGradBatch(logits.data_ptr(), dt, ld, mk, mask_ld, mr, at, st, g, h, out.data_ptr(), ld_out),
+              rows, V, _lib.LogprobParams(given, 0, temperature))
+    return out

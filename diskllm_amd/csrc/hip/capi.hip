@@ -16,6 +16,7 @@
 #include "sampler_topk.h"
 #include "sampler_full.h"
 #include "beam_select.h"
+#include "token_logprobs.h"
 #include "tanhf_glibc.h"
 
 extern "C" int dlk_launch_row_kernel(const dlk::RowParams *p, int rows, size_t lds_bytes, hipStream_t stream);
@@ -30,6 +31,7 @@ extern "C" int dlk_launch_long_history_penalties(float *logits, int64_t ld, int 
 extern "C" int dlk_launch_long_history_fixup(int rows, const int32_t *too_long, const uint64_t *rng_saved,
                                              uint64_t *rng, int32_t *out_ids, uint32_t *status, hipStream_t stream);
 extern "C" int dlk_launch_beam_select(const dlk::BeamParams *p, int groups, hipStream_t stream);
+extern "C" int dlk_launch_token_logprobs(const dlk::LogprobParams *p, int dtype, int rows, hipStream_t stream);
 extern "C" int dlk_launch_prepare_rows(const float *src, int64_t ld, float *dst, int64_t dld, int rows, int vocab,
                                        const uint32_t *mask, int64_t mask_ld, const int32_t *mask_row, float cap,
                                        hipStream_t stream);
@@ -41,7 +43,7 @@ constexpr int kMaxTopKLds = 4096;          /* larger top-k: candidates in global
 constexpr int kHcapDirect = 1024;          /* longer histories: penalties applied to a scratch copy first */
 constexpr size_t kFullWorkspace = (size_t)512 << 20;      /* workspace per launch of the fused kernel */
 constexpr size_t kGlobalTopkBudget = (size_t)256 << 20;   /* workspace per launch of the large-k row kernel */
-constexpr size_t kBeamWorkspace = (size_t)64 << 20;       /* workspace per launch of the beam selection */
+constexpr size_t kBeamWorkspace = (size_t)64 << 20;       /* workspace per launch of the beam selection, of scoring */
 constexpr int kLsdWords = 256 + 16 * 256 + 16;            /* select_top_k_global's LDS words */
 
 size_t r16(size_t b) { return (b + 15) & ~(size_t)15; }
@@ -728,6 +730,56 @@ extern "C" int dlk_beam_select(const dlk_beam_batch *b, int groups, int vocab, c
         const int n = groups - p.g0 < step ? groups - p.g0 : step;
         if (dlk_launch_beam_select(&p, n, stream) != 0) return DLK_ERR_HIP;
         if (groups - p.g0 <= step) break;
+    }
+    return DLK_OK;
+}
+
+/* Tokens scored (token_logprobs.hip), the rows in as many launches as the workspace's bound
+ * asks for; rows of one workgroup each need none. */
+extern "C" int dlk_token_logprobs(const dlk_logprob_batch *b, int rows, int vocab, const dlk_logprob_params *prm,
+                                  hipStream_t stream) {
+    using namespace dlk;
+    if (!b || !prm || rows < 0 || vocab <= 0 || !b->logits || b->ld < vocab) return DLK_ERR_INVALID;
+    if (b->dtype != DLK_F32 && b->dtype != DLK_BF16 && b->dtype != DLK_F16) return DLK_ERR_INVALID;
+    if (prm->n_given < 0 || prm->n_top < 0) return DLK_ERR_INVALID;
+    if (prm->n_given > 0 && (!b->tokens || !b->out_logprobs)) return DLK_ERR_INVALID;
+    if (prm->n_top > 0 && (!b->out_top_ids || !b->out_top_logprobs)) return DLK_ERR_INVALID;
+    if (b->mask && b->mask_ld < (vocab + 31) / 32) return DLK_ERR_INVALID;
+    if (!(prm->temperature >= 1e-30f && prm->temperature < INFINITY)) return DLK_ERR_INVALID;
+    if (((uintptr_t)b->logits & (b->dtype == DLK_F32 ? 3 : 1)) != 0 || ((uintptr_t)b->out_stats & 3) != 0) return DLK_ERR_INVALID;
+    if (prm->n_given > DLK_MAX_GIVEN || prm->n_top > DLK_MAX_ALTERNATIVES) return DLK_ERR_UNSUPPORTED;
+    if (vocab > 0x7fffffff - (1 << 20)) return DLK_ERR_UNSUPPORTED;
+    if (rows == 0) return DLK_OK;
+    LogprobParams p;
+    memset(&p, 0, sizeof(p));
+    p.logits = b->logits; p.ld = b->ld; p.V = vocab;
+    p.mask = b->mask; p.mask_ld = b->mask_ld; p.mask_row = b->mask_row;
+    p.tokens = b->tokens; p.given = prm->n_given; p.n = prm->n_top;
+    p.logprobs = b->out_logprobs; p.stats = b->out_stats;
+    p.top_ids = b->out_top_ids; p.top_logprobs = b->out_top_logprobs;
+    p.status = b->status;
+    p.inv_t = 1.0 / (double)prm->temperature;
+    p.scale = (float)(1.4426950408889634 * p.inv_t);
+    const int batch = logprob_batch(b->dtype);
+    p.batches = (int)(((int64_t)vocab + batch - 1) / batch);
+    p.slices = logprob_slices(rows, p.batches);
+    const size_t per = (size_t)p.slices * (sizeof(LogprobSlot) + (size_t)p.n * 8);
+    /* (2^32 threads and over are no launch) */
+    int64_t most = 0xffffff / p.slices;
+    if (p.slices > 1 && most > (int64_t)(kBeamWorkspace / per)) most = (int64_t)(kBeamWorkspace / per);
+    const int step = most < rows ? (int)most : rows;
+    std::lock_guard<std::mutex> lock(g_mu);
+    if (p.slices > 1) {
+        WsView ws;
+        if (!workspace(stream, 0, (size_t)step, (size_t)step * per, ws)) return ws_status();
+        p.counters = ws.counters;
+        p.slots = (LogprobSlot *)ws.data;
+        p.cands = (uint64_t *)(ws.data + (size_t)step * p.slices * sizeof(LogprobSlot));
+    }
+    for (p.r0 = 0; p.r0 < rows; p.r0 += step) {
+        const int n = rows - p.r0 < step ? rows - p.r0 : step;
+        if (dlk_launch_token_logprobs(&p, b->dtype, n, stream) != 0) return DLK_ERR_HIP;
+        if (rows - p.r0 <= step) break;
     }
     return DLK_OK;
 }

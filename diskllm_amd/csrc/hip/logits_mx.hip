@@ -1,0 +1,285 @@
+/*
+ * logits_mx.hip -- an LM head in microscaled 4-bit floating point (dlk_logits_mx):
+ *
+ *   logits[r, v] = sum over blocks b of 2^(sx[r, b] + sw[v, b] - 254) * (x_r . w_v over the block's 32 values)
+ *
+ * v_mfma_scale_f32_16x16x128 takes four blocks of 16 rows of each side with their scales as
+ * they are stored: nothing is unpacked or multiplied by a scale elsewhere.  Products of 4-bit
+ * by 4- or 6-bit values are exact in it and its sums are in 32 bits (8-bit values, which it
+ * takes too, it adds eight at a time to 2^-14 of the largest: not offered).  A lane's k-th
+ * group of the instruction's four need not be the k-th block as long as both sides agree: of
+ * 16 blocks lane group g takes 4 g .. 4 g + 3 in turn, whose four scales are one word of the
+ * scales' row, picked by the instruction.  w is its first operand, as in logits_i8.hip.
+ */
+#include <math.h>
+
+#include <type_traits>
+
+#include "logits_tile.h"
+
+namespace dlk {
+
+typedef int i2 __attribute__((ext_vector_type(2)));
+typedef int i8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+struct MxParams {
+    const uint8_t *x, *w, *xs, *ws;
+    int64_t ldx, ldw, ldxs, ldws, ld;
+    float *logits;
+    int rows, vocab, blocks;
+    float cap, recip;
+};
+
+/* A wave's sums as logits (write_logits of logits_i8.hip without scales). */
+template <bool CAP, bool WIDE, int MF, int NF>
+DLK_DEV void write_sums(const MxParams &p, const f4 (&acc)[MF][NF], int m0, int v0, float *mine) {
+    const int lane = lane_id(), lr = lane & 15, lk = lane >> 4;
+    constexpr int LD = NF * 16 + 4, LPR = NF * 4, RPS = 64 / LPR;        /* lanes of a row, rows of a store */
+    auto store = [&](int r, int v, const float (&y)[4]) {
+        if (r >= p.rows) return;
+        float *out = p.logits + (int64_t)r * p.ld + v;
+        if (v + 3 < p.vocab) {
+            store4(out, make_float4(y[0], y[1], y[2], y[3]));
+        } else {
+#pragma unroll
+            for (int c = 0; c < 3; c++)
+                if (v + c < p.vocab) out[c] = y[c];
+        }
+    };
+#pragma unroll
+    for (int m = 0; m < MF; m++) {
+#pragma unroll
+        for (int f = 0; f < NF; f++) {
+            float y[4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) y[c] = CAP ? capped(acc[m][f][c], p.cap, p.recip) : acc[m][f][c];
+            if (WIDE) *(float4 *)&mine[lr * LD + f * 16 + lk * 4] = make_float4(y[0], y[1], y[2], y[3]);
+            else store(m0 + m * 16 + lr, v0 + f * 16 + lk * 4, y);
+        }
+        if (WIDE) {
+#pragma unroll
+            for (int i = 0; i < 16 / RPS; i++) {
+                const int r = i * RPS + lane / LPR, c = lane % LPR * 4;
+                const float4 q = *(const float4 *)&mine[r * LD + c];
+                const float y[4] = {q.x, q.y, q.z, q.w};
+                store(m0 + m * 16 + r, v0 + c, y);
+            }
+        }
+    }
+}
+
+/* One instruction: OP is the byte of the scale words, FMT the format of x. */
+template <int FMT, int OP>
+DLK_DEV f4 mx_mfma(i8 w, i8 x, f4 acc, int sw, int sx) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, acc, 4, FMT == DLK_MX_FP4 ? 4 : 2, OP, sw, OP, sx);
+}
+
+/* What a workgroup stages of each step of NB blocks: rows of w and x in 16-byte chunks at
+ * place() (an FP6 block's 24 bytes as its first and its last 16), then 16 bytes of scales a row
+ * (NB = 8: those of this step and its neighbour). */
+template <int FMT, int BM, int BN, int NB>
+struct MxStage {
+    static constexpr int CX = FMT == DLK_MX_FP4 ? 1 : 2;                 /* chunks of a block of x */
+    static constexpr int WROW = NB * 16, XROW = NB * CX * 16;
+    static constexpr int X = BN * WROW, SW = X + BM * XROW, SX = SW + BN * 16, END = SX + BM * 16;
+    static constexpr int CHUNKS = END / 16;
+};
+
+/* The products of one staged step.  LAST: the row may end in it (blocks behind its end count as zeros). */
+template <int FMT, int BM, int BN, int NB, bool LAST, int MF, int NF>
+DLK_DEV void multiply_mx(const int8_t *lds, int wm, int wn, int it, int blocks, f4 (&acc)[MF][NF]) {
+    typedef MxStage<FMT, BM, BN, NB> St;
+    constexpr int PER = NB / 4;                    /* blocks of a lane group */
+    const int lr = lane_id() & 15, g = lane_id() >> 4;
+    const int8_t *const w = lds + (wn + lr) * St::WROW, *const x = lds + St::X + (wm + lr) * St::XROW;
+    int sw[NF], sx[MF];
+    auto scales = [&](const int8_t *at) {
+        int v;
+        if (NB == 16) v = *(const int *)(at + g * 4);
+        else v = *(const uint16_t *)(at + (it & 1) * 8 + g * 2);
+        if (LAST) {
+            /* 1 in the place of those behind the row's end (255 among them would be NaN) */
+            const int left = min(max(blocks - (it * NB + g * PER), 0), PER);
+            const uint32_t keep = left >= 4 ? 0xffffffffu : (1u << (8 * left)) - 1;
+            v = (int)(((uint32_t)v & keep) | (0x7f7f7f7fu & ~keep));
+        }
+        return v;
+    };
+#pragma unroll
+    for (int f = 0; f < NF; f++) sw[f] = scales(lds + St::SW + (wn + f * 16 + lr) * 16);
+#pragma unroll
+    for (int m = 0; m < MF; m++) sx[m] = scales(lds + St::SX + (wm + m * 16 + lr) * 16);
+    auto step = [&](auto number) {
+        constexpr int s = decltype(number)::value;
+        i8 a[NF], b[MF];
+        const int c = g * PER + s;
+#pragma unroll
+        for (int f = 0; f < NF; f++) {
+            const i4 v = *(const i4 *)&w[f * 16 * St::WROW + place<St::WROW>(lr, c) * 16];
+            a[f] = i8{v.x, v.y, v.z, v.w, 0, 0, 0, 0};
+        }
+        const bool some = !LAST || it * NB + c < blocks;
+#pragma unroll
+        for (int m = 0; m < MF; m++) {
+            const int8_t *row = &x[m * 16 * St::XROW];
+            if (FMT == DLK_MX_FP4) {
+                const i4 v = *(const i4 *)&row[place<St::XROW>(lr, c) * 16];
+                b[m] = some ? i8{v.x, v.y, v.z, v.w, 0, 0, 0, 0} : i8{0, 0, 0, 0, 0, 0, 0, 0};
+            } else {
+                const i4 v = *(const i4 *)&row[place<St::XROW>(lr, 2 * c) * 16];
+                const i2 u = *(const i2 *)&row[place<St::XROW>(lr, 2 * c + 1) * 16 + 8];
+                b[m] = some ? i8{v.x, v.y, v.z, v.w, u.x, u.y, 0, 0} : i8{0, 0, 0, 0, 0, 0, 0, 0};
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MF; m++)
+#pragma unroll
+            for (int f = 0; f < NF; f++) acc[m][f] = mx_mfma<FMT, s>(a[f], b[m], acc[m][f], sw[f], sx[m]);
+    };
+    step(std::integral_constant<int, 0>());
+    step(std::integral_constant<int, 1>());
+    if constexpr (PER == 4) {
+        step(std::integral_constant<int, 2>());
+        step(std::integral_constant<int, 3>());
+    }
+}
+
+/* BM rows of x and BN of w per workgroup, WGM x WGN waves, steps of NB blocks loaded straight
+ * into LDS, ST stages in a ring: step it + ST - 1 is asked for while step it is multiplied, one
+ * barrier a step. */
+template <int FMT, int BM, int BN, int WGM, int WGN, int NB, int ST, bool CAP>
+__global__ __launch_bounds__(WGM * WGN * 64, 2) void logits_mx_kernel(MxParams p) {
+    typedef MxStage<FMT, BM, BN, NB> St;
+    constexpr int W = WGM * WGN, WM = BM / WGM, WN = BN / WGN, MF = WM / 16, NF = WN / 16;
+    constexpr int NI = (St::CHUNKS + 64 * W - 1) / (64 * W);             /* loads of a wave per stage */
+    constexpr int STAGE = NI * W * 1024;
+    __shared__ __align__(1024) int8_t lds[ST * STAGE];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
+    int m0, v0;
+    if (!tile_of<BM, BN>(p.rows, p.vocab, m0, v0)) return;
+    const int steps = (p.blocks + NB - 1) / NB, whole = p.blocks / NB;
+    /* this lane's chunk of load j: at src + min(it * per + first, last) * size */
+    const uint8_t *src[NI];
+    int first[NI], size[NI];
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+        const int c = min(((j * W + wave) * 64 + lane), St::CHUNKS - 1) * 16;
+        if (c < St::X) {
+            const int r = c / St::WROW, k = place<St::WROW>(r, c % St::WROW / 16);
+            src[j] = p.w + (int64_t)min(v0 + r, p.vocab - 1) * p.ldw;
+            first[j] = k;
+            size[j] = 16;
+        } else if (c < St::SW) {
+            const int r = (c - St::X) / St::XROW, k = place<St::XROW>(r, (c - St::X) % St::XROW / 16);
+            src[j] = p.x + (int64_t)min(m0 + r, p.rows - 1) * p.ldx + (St::CX == 2 ? k % 2 * 8 : 0);
+            first[j] = k / St::CX;
+            size[j] = St::CX == 2 ? 24 : 16;
+        } else {
+            const bool of_w = c < St::SX;
+            const int r = (c - (of_w ? St::SW : St::SX)) / 16;
+            src[j] = of_w ? p.ws + (int64_t)min(v0 + r, p.vocab - 1) * p.ldws : p.xs + (int64_t)min(m0 + r, p.rows - 1) * p.ldxs;
+            first[j] = 0;
+            size[j] = 1;                           /* (a byte a block) */
+        }
+    }
+    auto fetch = [&](int it, int slot) {
+#pragma unroll
+        for (int j = 0; j < NI; j++) {
+            const int b = it * NB + first[j];
+            const int at = size[j] == 1 ? b & ~15 : min(b, p.blocks - 1) * size[j];
+            load_to_lds((const int8_t *)src[j] + at, &lds[slot * STAGE + (j * W + wave) * 1024]);
+        }
+    };
+    const int wm = wave % WGM * WM, wn = wave / WGM * WN;
+    f4 acc[MF][NF];
+#pragma unroll
+    for (int m = 0; m < MF; m++)
+#pragma unroll
+        for (int f = 0; f < NF; f++) acc[m][f] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < ST - 1; s++)
+        if (s < steps) fetch(s, s);
+    int slot = 0;
+    for (int it = 0; it < whole; it++) {
+        if (it + ST - 2 < steps) wait_loads<NI *(ST - 2)>();
+        else wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        /* the slot that step it - 1 has left */
+        if (it + ST - 1 < steps) fetch(it + ST - 1, slot == 0 ? ST - 1 : slot - 1);
+        multiply_mx<FMT, BM, BN, NB, false>(&lds[slot * STAGE], wm, wn, it, p.blocks, acc);
+        slot = slot == ST - 1 ? 0 : slot + 1;
+    }
+    if (whole < steps) {                           /* a last, shorter step */
+        wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        multiply_mx<FMT, BM, BN, NB, true>(&lds[slot * STAGE], wm, wn, whole, p.blocks, acc);
+    }
+    constexpr bool WIDE = NF >= 4;
+    static_assert(!WIDE || W * 16 * (WN + 4) * 4 <= ST * STAGE, "room for the output");
+    if (WIDE) __syncthreads();
+    write_sums<CAP, WIDE>(p, acc, m0 + wm, v0 + wn, (float *)lds + (WIDE ? wave * 16 * (WN + 4) : 0));
+}
+
+template <int FMT, int BM, int BN, int WGM, int WGN, int NB, int ST>
+int launch_mx(const MxParams &p, hipStream_t stream) {
+    const int64_t tiles = (((int64_t)p.vocab + BN - 1) / BN) * (((int64_t)p.rows + BM - 1) / BM);
+    const int threads = WGM * WGN * 64;
+    if ((tiles + 7) / 8 * 8 * threads > 0xffffffffLL) return DLK_ERR_UNSUPPORTED;      /* (no launch) */
+    const dim3 grid((unsigned)((tiles + 7) / 8 * 8));
+    if (p.cap > 0.0f)
+        hipLaunchKernelGGL((logits_mx_kernel<FMT, BM, BN, WGM, WGN, NB, ST, true>), grid, dim3(threads), 0, stream, p);
+    else
+        hipLaunchKernelGGL((logits_mx_kernel<FMT, BM, BN, WGM, WGN, NB, ST, false>), grid, dim3(threads), 0, stream, p);
+    return hipGetLastError() == hipSuccess ? DLK_OK : DLK_ERR_HIP;
+}
+
+template <int FMT>
+int launch_mx_tiles(const MxParams &p, hipStream_t stream) {
+    if (p.rows <= 16) return launch_mx<FMT, 16, 64, 1, 4, 16, 3>(p, stream);
+    if (p.rows <= 32) return launch_mx<FMT, 32, 64, 2, 2, 16, 3>(p, stream);
+    if (p.rows <= 64) return launch_mx<FMT, 64, 64, 2, 2, 16, 2>(p, stream);
+    if (p.rows <= 128) return launch_mx<FMT, 128, 128, 2, 2, 8, 2>(p, stream);
+    if (FMT == DLK_MX_FP4 && p.rows > 384) return launch_mx<DLK_MX_FP4, 256, 256, 2, 4, 8, 2>(p, stream);
+    return launch_mx<FMT, 128, 256, 2, 4, 8, 2>(p, stream);
+}
+
+}  // namespace dlk
+
+extern "C" int dlk_logits_mx(const uint8_t *x, int x_format, int64_t ldx, const uint8_t *x_scale, int64_t ldxs,
+                             const uint8_t *w, int64_t ldw, const uint8_t *w_scale, int64_t ldws, int rows, int vocab,
+                             int n, float softcap, float *logits, int64_t ld, hipStream_t stream) {
+    using namespace dlk;
+    if (!x || !x_scale || !w || !w_scale || !logits || rows < 0 || vocab <= 0 || n <= 0) return DLK_ERR_INVALID;
+    if (x_format != DLK_MX_FP4 && x_format != DLK_MX_FP6) return DLK_ERR_INVALID;
+    const int64_t blocks = ((int64_t)n + 31) / 32, scales = (blocks + 15) / 16 * 16;
+    const int64_t bytes = blocks * (x_format == DLK_MX_FP4 ? 16 : 24);
+    /* (the stride of a single row says nothing) */
+    if ((rows > 1 && (ldx < bytes || ldxs < scales)) || (vocab > 1 && (ldw < blocks * 16 || ldws < scales)) || ld < vocab)
+        return DLK_ERR_INVALID;
+    if (!(fabsf(softcap) < INFINITY)) return DLK_ERR_INVALID;
+    if ((((uintptr_t)x | (uint64_t)(rows > 1 ? ldx : 0)) & (x_format == DLK_MX_FP4 ? 15 : 7)) != 0) return DLK_ERR_INVALID;
+    if ((((uintptr_t)w | (uintptr_t)x_scale | (uintptr_t)w_scale | (uint64_t)(rows > 1 ? ldxs : 0) |
+          (uint64_t)(vocab > 1 ? ldw | ldws : 0)) & 15) != 0 || ((uintptr_t)logits & 3) != 0)
+        return DLK_ERR_INVALID;
+    /* int indices of a row's bytes */
+    if (n > 0x3fffffff || vocab > 0x7fffffff - 65536 || rows > 0x7fffffff - 65536) return DLK_ERR_UNSUPPORTED;
+    if (rows == 0) return DLK_OK;
+    /* a cap below 2^-128 has no reciprocal among the floats: the product without it, then the cap by exact quotients */
+    if (softcap > 0.0f && 1.0f / softcap == INFINITY) {
+        int rc = dlk_logits_mx(x, x_format, ldx, x_scale, ldxs, w, ldw, w_scale, ldws, rows, vocab, n, 0.0f, logits, ld, stream);
+        for (int64_t r = 0; rc == DLK_OK && r < rows; r += 65535)
+            rc = dlk_softcap(logits + r * ld, ld, (int)(rows - r < 65535 ? rows - r : 65535), vocab, softcap, stream);
+        return rc;
+    }
+    MxParams p;
+    p.x = x; p.w = w; p.xs = x_scale; p.ws = w_scale;
+    p.ldx = ldx; p.ldw = ldw; p.ldxs = ldxs; p.ldws = ldws; p.ld = ld;
+    p.logits = logits;
+    p.rows = rows; p.vocab = vocab; p.blocks = (int)blocks;
+    p.cap = softcap > 0.0f ? softcap : 0.0f;
+    p.recip = p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
+    return x_format == DLK_MX_FP4 ? launch_mx_tiles<DLK_MX_FP4>(p, stream) : launch_mx_tiles<DLK_MX_FP6>(p, stream);
+}

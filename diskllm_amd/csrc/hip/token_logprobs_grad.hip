@@ -1,0 +1,153 @@
+/*
+ * token_logprobs_grad.hip -- the logits' gradient of the given tokens' log-probabilities and
+ * of the entropy (dlk_token_logprobs_grad):
+ *
+ *   dl_v = (1 / T) * (sum_j g_j [v = token_j] - p_v * (sum_j g_j + h * (log p_v + entropy)))
+ *
+ * with p_v = 2^((l_v - max) * log2(e) / T) / z of the statistics that the forward call left, so
+ * that a row is read once and no workgroup waits for another.  Bound by memory: 256 threads,
+ * 16-byte groups, a wave's 64 groups side by side, of which it knows by one ballot of the
+ * tokens (a lane each) whether any lies there.
+ */
+#include "logit_row.h"
+#include "../../../include/diskllm_amd.h"
+
+namespace dlk {
+
+constexpr int kGradThreads = 256;
+
+struct GradParams {
+    const void *logits;
+    int64_t ld;
+    const uint32_t *mask;
+    int64_t mask_ld;
+    const int32_t *mask_row;
+    const int32_t *tokens;
+    const float *stats, *g, *h;
+    void *grad;
+    int64_t ld_grad;
+    int V, given, pieces;
+    float scale, inv_t;  /* log2(e) / T, 1 / T */
+    int64_t r0;
+};
+
+/* Row blockIdx.x / pieces, piece blockIdx.x % pieces: four groups a thread. */
+template <int DT, bool ENTROPY>
+__global__ __launch_bounds__(kGradThreads) void token_logprobs_grad_kernel(GradParams p) {
+    typedef LogitRow<DT> In;
+    constexpr int T = kGradThreads, GR = 4, G = In::G, B = T * GR * G;
+    const int t = threadIdx.x, lane = lane_id();
+    const int64_t row = p.r0 + blockIdx.x / p.pieces;
+    const int b0 = (int)(blockIdx.x % p.pieces) * B;
+    const typename In::T *lg = (const typename In::T *)p.logits + row * p.ld;
+    typename In::T *out = (typename In::T *)p.grad + row * p.ld_grad;
+    const uint32_t *mw = p.mask ? p.mask + (int64_t)(p.mask_row ? p.mask_row[row] : row) * p.mask_ld : nullptr;
+    const int s1 = p.V;
+    typename In::Raw raw[GR];
+    auto place = [&](int j) { return b0 + (j * T + t) * G; };
+#pragma unroll
+    for (int j = 0; j < GR; j++)
+        if (place(j) + G <= s1) raw[j] = *(const typename In::Raw *)(lg + place(j));
+    const float top = p.stats[row * 4], z = p.stats[row * 4 + 1], entropy = p.stats[row * 4 + 2];
+    /* a token a lane (every wave holds them all); one that counts for nothing is -1 */
+    int32_t token = -1;
+    float g = 0.0f;
+    if (lane < p.given) {
+        token = p.tokens[row * p.given + lane];
+        if (token < 0 || token >= p.V || !mask_allows(mw, token)) token = -1;
+        if (token >= 0) g = p.g[row * p.given + lane];
+    }
+    float h = 0.0f;
+    if (ENTROPY) h = p.h[row];
+    float total = 0.0f;
+#pragma unroll 1
+    for (int j = 0; j < p.given; j++) total += shfl(g, j);
+    /* no allowed id, or nothing to differentiate (whatever the logits hold): zeros */
+    const bool none = top == -INFINITY || (ballot(g != 0.0f) == 0 && h == 0.0f);
+    const float inv_z = 1.0f / z;
+    const float per = p.inv_t * inv_z;
+    const float by = ENTROPY ? (total + h * (entropy - logf(z))) * per : total * per;
+    const float by_t = ENTROPY ? h * 0.693147180559945309f * per : 0.0f;
+#pragma unroll
+    for (int j = 0; j < GR; j++) {
+        const int i = place(j);
+        float x[G], y[G];
+        if (i + G <= s1) {
+            In::unpack(raw[j], x);
+        } else {
+#pragma unroll
+            for (int c = 0; c < G; c++) x[c] = i + c < s1 ? In::one(lg + i + c) : -INFINITY;
+        }
+        uint32_t bits = 0xffffffffu;
+        if (mw) bits = mw[min(i, s1 - 1) >> 5] >> (i & 31);
+#pragma unroll
+        for (int c = 0; c < G; c++) {
+            const float d = (x[c] - top) * p.scale, e = __builtin_amdgcn_exp2f(d);
+            y[c] = ENTROPY ? -e * fmaf(by_t, fmaxf(d, -200.0f), by) : -e * by;
+            if (mw) y[c] = (bits >> c & 1) != 0 ? y[c] : 0.0f;
+            y[c] = none || x[c] == -INFINITY ? 0.0f : y[c];
+        }
+        /* the wave's 64 groups lie side by side: the tokens among them, in their order */
+        const int w0 = b0 + (j * T + (t & ~63)) * G;
+        for (uint64_t who = ballot(token >= w0 && token - w0 < 64 * G); who != 0; who &= who - 1) {
+            const int k = __builtin_ctzll(who);
+            const int at = shfl(token, k) - i;
+            const float add = shfl(g, k) * p.inv_t;
+#pragma unroll
+            for (int c = 0; c < G; c++) y[c] += at == c && !none ? add : 0.0f;
+        }
+        if (i + G <= s1) {
+            *(typename In::Raw *)(out + i) = In::pack(y);
+        } else {
+#pragma unroll
+            for (int c = 0; c < G; c++)
+                if (i + c < s1) In::put(out + i + c, y[c]);
+        }
+    }
+}
+
+template <int DT>
+int launch_grad(const GradParams &p, int64_t blocks, hipStream_t stream) {
+    if (p.h)
+        hipLaunchKernelGGL((token_logprobs_grad_kernel<DT, true>), dim3((unsigned)blocks), dim3(kGradThreads), 0, stream, p);
+    else
+        hipLaunchKernelGGL((token_logprobs_grad_kernel<DT, false>), dim3((unsigned)blocks), dim3(kGradThreads), 0, stream, p);
+    return hipGetLastError() == hipSuccess ? DLK_OK : DLK_ERR_HIP;
+}
+
+}  // namespace dlk
+
+extern "C" int dlk_token_logprobs_grad(const dlk_logprob_grad_batch *b, int rows, int vocab,
+                                       const dlk_logprob_params *prm, hipStream_t stream) {
+    using namespace dlk;
+    if (!b || !prm || rows < 0 || vocab <= 0 || !b->logits || !b->stats || !b->grad) return DLK_ERR_INVALID;
+    if (b->ld < vocab || b->ld_grad < vocab) return DLK_ERR_INVALID;
+    if (b->dtype != DLK_F32 && b->dtype != DLK_BF16 && b->dtype != DLK_F16) return DLK_ERR_INVALID;
+    if (prm->n_given < 0 || (prm->n_given > 0 && (!b->tokens || !b->grad_logprobs))) return DLK_ERR_INVALID;
+    if (b->mask && b->mask_ld < (vocab + 31) / 32) return DLK_ERR_INVALID;
+    if (!(prm->temperature >= 1e-30f && prm->temperature < INFINITY)) return DLK_ERR_INVALID;
+    const uintptr_t align = b->dtype == DLK_F32 ? 3 : 1;
+    if ((((uintptr_t)b->logits | (uintptr_t)b->grad) & align) != 0) return DLK_ERR_INVALID;
+    /* over the logits: place by place only */
+    if (b->grad == b->logits && rows > 1 && b->ld_grad != b->ld) return DLK_ERR_INVALID;
+    if (prm->n_given > DLK_MAX_GIVEN || vocab > 0x7fffffff - (1 << 20)) return DLK_ERR_UNSUPPORTED;
+    if (rows == 0) return DLK_OK;
+    GradParams p;
+    p.logits = b->logits; p.ld = b->ld; p.mask = b->mask; p.mask_ld = b->mask_ld; p.mask_row = b->mask_row;
+    p.tokens = b->tokens; p.stats = b->stats; p.g = b->grad_logprobs; p.h = b->grad_entropy;
+    p.grad = b->grad; p.ld_grad = b->ld_grad; p.V = vocab; p.given = prm->n_given;
+    p.inv_t = 1.0f / prm->temperature;
+    p.scale = (float)(1.4426950408889634 / (double)prm->temperature);
+    const int batch = kGradThreads * 4 * (b->dtype == DLK_F32 ? 4 : 8);
+    p.pieces = (int)(((int64_t)vocab + batch - 1) / batch);
+    /* (2^32 threads and over are no launch) */
+    const int64_t most = 0xffffffLL / p.pieces;
+    for (p.r0 = 0; p.r0 < rows; p.r0 += most) {
+        const int64_t blocks = (rows - p.r0 < most ? rows - p.r0 : most) * p.pieces;
+        const int rc = b->dtype == DLK_F32 ? launch_grad<DLK_F32>(p, blocks, stream)
+                     : b->dtype == DLK_BF16 ? launch_grad<DLK_BF16>(p, blocks, stream)
+                                            : launch_grad<DLK_F16>(p, blocks, stream);
+        if (rc != DLK_OK) return rc;
+    }
+    return DLK_OK;
+}

@@ -282,6 +282,115 @@ int dlk_logits_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8
                   const float *w_scale, int rows, int vocab, int n, float softcap, float *logits, int64_t ld,
                   hipStream_t stream);
 
+/* ---- logits from 4-bit weights ---------------------------------------------------
+ * The same head with its weights in microscaled 4-bit floating point: half the bytes of
+ * the 8-bit one, which a decode step is bound by.  A row of n values is ceil(n / 32) blocks
+ * of 32; block b's value i is an element times 2^(scale[b] - 127).  Elements: DLK_MX_FP4, 16
+ * bytes a block, value 2 k in the low and 2 k + 1 in the high half of byte k, each a sign and
+ * one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (E2M1); DLK_MX_FP6, 24 bytes a block, value i in the 6 bits
+ * from 6 i on (the first byte's lowest bit is bit 0), each a sign and one of 0, 0.125 .. 2, 2.25 .. 4,
+ * 4.5 .. 7.5 (E2M3): for hidden states, which 4 bits are few for.  Scale 255: NaN.  No counterpart
+ * in the reference. */
+#define DLK_MX_FP4 0
+#define DLK_MX_FP6 1
+
+/* Blocks of each row of x [rows, n] (DLK_F32, DLK_BF16 or DLK_F16; strides in elements).  A
+ * block's scale is 2^(floor(log2(max |x|)) - 2), at least 2^-127; its elements are x over that to the nearest, halves to the even code, decided exactly, and
+ * at most the largest element.  A block of zeros: scale 2^-127 and zeros; one that holds
+ * NaN or infinity: scale 255 and zeros.  The last block of a row is filled with zeros.  q
+ * takes ceil(n / 32) * 16 (FP6: 24) bytes a row at q + r * ldq, 8-byte aligned (ldq too); scale
+ * ceil(n / 32) bytes a row at scale + r * ld_scale, of any alignment.  x needs its elements'
+ * alignment; no overlaps. */
+int dlk_quantize_mx(const void *x, int dtype, int64_t ldx, int rows, int n, int format, uint8_t *q, int64_t ldq,
+                    uint8_t *scale, int64_t ld_scale, hipStream_t stream);
+
+/* The values of rows of blocks, n of each, in `dtype` (rounded to the nearest, halves to even, where
+ * it does not hold them): out[r * ld + i] of row ids[r] of the table q, or of row r where ids is
+ * NULL: with ids the embedding rows of tokens from a tied table.  An id outside [0,
+ * table_rows) gives zeros (rows <= table_rows without ids).  Alignment as above; of out its
+ * elements'. */
+int dlk_dequantize_mx(const uint8_t *q, int64_t ldq, const uint8_t *scale, int64_t ld_scale, int table_rows,
+                      const int32_t *ids, int rows, int n, int format, void *out, int dtype, int64_t ld,
+                      hipStream_t stream);
+
+/* logits[r * ld + v] = sum over the ceil(n / 32) blocks of x's row r (x_format) and w's row v
+ * (FP4) of their values' products; softcap as in dlk_logits_i8.  The products of a block are
+ * exact, sums are in 32 bits: off by at most 2^-22 of the sum of the products' sizes for each
+ * 128 values.  A block with scale 255 makes its row's logits NaN.  x, w and the scales: 16-byte aligned
+ * (x in FP6: 8), strides too (the bytes of a row of scales up to the next multiple of 16 are read; what
+ * stands there does not matter).  Entries past vocab in a row of logits are left as they are; logits may not overlap
+ * the inputs. */
+int dlk_logits_mx(const uint8_t *x, int x_format, int64_t ldx, const uint8_t *x_scale, int64_t ldxs, const uint8_t *w,
+                  int64_t ldw, const uint8_t *w_scale, int64_t ldws, int rows, int vocab, int n, float softcap,
+                  float *logits, int64_t ld, hipStream_t stream);
+
+/* ---- scores of tokens ----------------------------------------------------------------
+ * What a model's logits say of tokens that are known: the log-probabilities that a
+ * request asks for beside its sampled tokens, of a prompt's tokens, or of a batch in
+ * training, with their gradient.  No counterpart in the reference. */
+
+#define DLK_MAX_GIVEN 64                /* given tokens of a row */
+#define DLK_MAX_ALTERNATIVES 64         /* alternatives of a row */
+
+typedef struct {
+    const void *logits;       /* [rows, ld] of dtype, read only */
+    int dtype;                /* DLK_F32, DLK_BF16 or DLK_F16 */
+    int64_t ld;               /* row stride in elements (>= vocab) */
+    const uint32_t *mask;     /* packed allow-masks as in dlk_batch, or NULL */
+    int64_t mask_ld;
+    const int32_t *mask_row;
+    const int32_t *tokens;    /* [rows, n_given]; outside [0, vocab): no token */
+    float *out_logprobs;      /* [rows, n_given] their log-probabilities; 0 where there is no token */
+    float *out_stats;         /* [rows, 4] or NULL: largest allowed logit, sum of exp((l - largest) / T),
+                                 entropy, log of the sum of exp(l / T) */
+    int32_t *out_top_ids;     /* [rows, n_top] the largest allowed logits' ids, largest first, of equal ones the lower
+                                 id; -1 where a row has no more */
+    float *out_top_logprobs;  /* [rows, n_top] their log-probabilities; -inf likewise */
+    uint32_t *status;         /* one word of DLK_STATUS_* bits, OR-ed, or NULL */
+} dlk_logprob_batch;
+
+typedef struct {
+    int n_given;              /* tokens of each row, at most DLK_MAX_GIVEN; 0 = none */
+    int n_top;                /* alternatives of each row, at most DLK_MAX_ALTERNATIVES; 0 = none */
+    float temperature;        /* T: finite, at least 1e-30 */
+} dlk_logprob_params;
+
+/* log p_v = l_v / T - log(sum_u exp(l_u / T)) over the ids that the mask allows (-inf for
+ * the others); the entropy -sum p log p.  The logits are read once.  A row without an allowed logit
+ * above -inf: log-probabilities -inf, statistics -inf, 0, 0 and -inf, no alternatives.  A
+ * row whose allowed logits hold NaN or +inf: NaN (ids -1), and DLK_STATUS_NOT_FINITE; what stands in
+ * places that are not allowed does not matter.  Exponentials and sums of up to 32 terms in 32 bits, the rest in
+ * 64: log-probabilities are off by their own rounding and 1.5e-5 at most at up to 262,144 logits a row (some
+ * 2e-7 as measured).  Takes workspace as dlk_sample does where rows are few (dlk_release_stream; one call on the stream before capturing it, else
+ * DLK_ERR_HIP).  Outputs may not overlap inputs. */
+int dlk_token_logprobs(const dlk_logprob_batch *batch, int rows, int vocab, const dlk_logprob_params *params,
+                       hipStream_t stream);
+
+typedef struct {
+    const void *logits;       /* these as in the forward call */
+    int dtype;
+    int64_t ld;
+    const uint32_t *mask;
+    int64_t mask_ld;
+    const int32_t *mask_row;
+    const int32_t *tokens;
+    const float *stats;       /* [rows, 4] as dlk_token_logprobs has left them */
+    const float *grad_logprobs;  /* [rows, n_given] */
+    const float *grad_entropy;   /* [rows], or NULL: 0 */
+    void *grad;               /* [rows, ld_grad] of dtype: written; may be the logits themselves (ld_grad == ld) */
+    int64_t ld_grad;
+} dlk_logprob_grad_batch;
+
+/* The logits' gradient of sum_j grad_logprobs[r, j] * logprob[r, j] + grad_entropy[r] * entropy[r]:
+ *   grad_v = (1 / T) * (sum_j g_j [v = token_j] - p_v * (sum_j g_j + h * (log p_v + entropy)))
+ * in 32 bits, rounded once to dtype; 0 for ids that are not allowed.  The same token
+ * may be given several times.  Places without a token, or whose token the mask does not allow, count for
+ * nothing.  A row in which nothing is to be differentiated (every g that counts and h are 0, or
+ * no logit is allowed): zeros, whatever its logits hold; else a row whose statistics are
+ * NaN gets NaN for its allowed ids.  n_top does not matter.  No workspace. */
+int dlk_token_logprobs_grad(const dlk_logprob_grad_batch *batch, int rows, int vocab, const dlk_logprob_params *params,
+                            hipStream_t stream);
+
 /* ---- beam search ----------------------------------------------------------------
  * The deterministic counterpart of dlk_sample: the best continuations of each group
  * (request) of `beams` rows over the vocabulary, and the beams' states following
