@@ -568,20 +568,30 @@ def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
                    temperature: float = 1.0, out: Optional[dict] = None, status: Optional[torch.Tensor] = None,
                    stream: Optional[int] = None) -> dict:
     """Scores of tokens int32 [rows] or [rows, given] under logits [rows, vocab] in float32, bfloat16 or float16
-    (dlk_token_logprobs): logprobs (tokens' shape, or None without tokens), entropy [rows], stats [rows, 4] (for
-    token_logprobs_grad; entropy is its column 2), and top_ids, top_logprobs [rows, top] (None without)."""
+    (dlk_token_logprobs): logprobs (tokens' shape, or None without tokens), stats [rows, 4] (largest logit, sum, entropy,
+    log-sum; for token_logprobs_grad too), and top_ids, top_logprobs [rows, top] (None without)."""
     dev, dt, rows, V, ld, given, at, mk, mask_ld, mr = _scored(logits, tokens, mask, mask_row)
     if not 0 <= top <= 0x7fffffff:
         raise ValueError(_WIDE.format("token_logprobs"))
+    lp = ti = tl = 0
     if out is None:
-        stats = _empty((rows, 4), _F32, logits, dev, stream)
-        out = dict(logprobs=None if tokens is None else _empty(tokens.shape, _F32, logits, dev, stream), stats=stats,
-                   entropy=stats[:, 2], top_ids=_empty((rows, top), _I32, logits, dev, stream) if top else None,
-                   top_logprobs=_empty((rows, top), _F32, logits, dev, stream) if top else None)
-    lp = _flat(out["logprobs"], rows * given, dev, _F32, "logprobs") if given else 0
-    st = _flat(out["stats"], rows * 4, dev, _F32, "stats")
-    ti = _flat(out["top_ids"], rows * top, dev, _I32, "top_ids") if top else 0
-    tl = _flat(out["top_logprobs"], rows * top, dev, _F32, "top_logprobs") if top else 0
+        out = dict(logprobs=None, stats=_empty((rows, 4), _F32, logits, dev, stream), top_ids=None, top_logprobs=None)
+        st = out["stats"].data_ptr()
+        if tokens is not None:
+            made = out["logprobs"] = _empty(tokens.shape, _F32, logits, dev, stream)
+            lp = made.data_ptr()
+        if top:
+            made = out["top_ids"] = _empty((rows, top), _I32, logits, dev, stream)
+            ti = made.data_ptr()
+            made = out["top_logprobs"] = _empty((rows, top), _F32, logits, dev, stream)
+            tl = made.data_ptr()
+    else:
+        st = _flat(out["stats"], rows * 4, dev, _F32, "stats")
+        if given:
+            lp = _flat(out["logprobs"], rows * given, dev, _F32, "logprobs")
+        if top:
+            ti = _flat(out["top_ids"], rows * top, dev, _I32, "top_ids")
+            tl = _flat(out["top_logprobs"], rows * top, dev, _F32, "top_logprobs")
     bits = 0 if status is None else _flat(status, 1, dev, _I32, "status")
     if rows:
         _call(dev, stream, "dlk_token_logprobs", _lib.lib().dlk_token_logprobs,

@@ -763,7 +763,8 @@ extern "C" int dlk_token_logprobs(const dlk_logprob_batch *b, int rows, int voca
     const int batch = logprob_batch(b->dtype);
     p.batches = (int)(((int64_t)vocab + batch - 1) / batch);
     p.slices = logprob_slices(rows, p.batches);
-    const size_t per = (size_t)p.slices * (sizeof(LogprobSlot) + (size_t)p.n * 8);
+    p.cap = p.n > 0 ? std::min(p.n + 12, DLK_MAX_ALTERNATIVES) : 0;
+    const size_t per = (size_t)p.slices * (sizeof(LogprobSlot) + (size_t)p.cap * 8);
     /* (2^32 threads and over are no launch) */
     int64_t most = 0xffffff / p.slices;
     if (p.slices > 1 && most > (int64_t)(kBeamWorkspace / per)) most = (int64_t)(kBeamWorkspace / per);

@@ -14,7 +14,9 @@ constexpr int kLogprobMaxSlices = 64;                            /* of a row (a 
 constexpr int kLogprobEntries = kLogprobThreads * 16;            /* entries that a join takes */
 
 /* Logits of a batch: four 16-byte loads a thread. */
-inline int logprob_batch(int dtype) { return dtype == 0 ? kLogprobThreads * 16 : kLogprobThreads * 32; }
+inline int logprob_batch(int dtype) { return kLogprobThreads * (dtype == 0 ? 16 : 32); }
+
+constexpr int kLogprobRecords = 64;                              /* of each thread's maxima in a slice */
 
 /* What a workgroup says of its slice of a row. */
 struct LogprobSlot {
@@ -34,6 +36,7 @@ struct LogprobParams {
     float *top_logprobs;
     uint32_t *status;
     int V, given, n;     /* n: alternatives */
+    int cap;             /* entries that a slice may list for the row's last workgroup */
     float scale;         /* log2(e) / T */
     double inv_t;
     int r0;              /* first row of the launch */
@@ -41,13 +44,21 @@ struct LogprobParams {
     int batches;         /* of a row, shared out to them */
     uint32_t *counters;  /* [rows] zero between launches; none where slices == 1 */
     LogprobSlot *slots;  /* [rows][slices] */
-    uint64_t *cands;     /* [rows][slices][n] */
+    uint64_t *cands;     /* [rows][slices][cap] */
 };
 
-/* Workgroups for each row: some 800 in all (three a CU), as the beam selection's slices. */
+/* Workgroups for each row: some 384 in all, two at least up to 256 rows (of more than four rows two thirds of the
+ * batches at most); past that one.  What each one adds, its list and the row's joining, is a chain of some 5 us
+ * that others of its CU run beside (us by workgroups a row, float32 with 5 alternatives):
+ *   1 x 32,000      1: 10.9, 2: 12.0, 4: 12.2, 8: 10.8
+ *   8 x 151,936     4: 16.0, 8: 13.8, 18: 12.5, 25: 12.1, 37: 13.7
+ *   64 x 151,936    1: 28.7, 2: 21.7, 4: 18.0, 8: 18.2, 13: 19.7, 37: 35.8
+ *   128 x 50,257    1: 16.0, 2: 15.5, 4: 16.8, 9: 21.1
+ *   256 x 151,936   1: 48.9, 2: 42.7, 4: 42.5, 8: 47.6
+ *   300 x 50,257    1: 20.4, 2: 22.7, 4: 29.9 */
 inline int logprob_slices(int64_t rows, int batches) {
-    int64_t s = (800 + rows / 2) / rows;
-    if (s < 1) s = 1;
+    int64_t s = rows > 256 ? 1 : (384 + rows / 2) / rows;
+    if (rows > 4 && s > (batches * 2 + 2) / 3) s = (batches * 2 + 2) / 3;
     if (s > kLogprobMaxSlices) s = kLogprobMaxSlices;
     return (int)(s < batches ? s : batches);
 }

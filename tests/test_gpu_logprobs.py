@@ -88,7 +88,7 @@ def check(logits, tokens, top=0, allow=None, T=1.0, words=None, mask_row=None, *
     H, lse = stats[:, 2], stats[:, 3]
     near(got["stats"][:, 0], stats[:, 0], 0)
     near(got["stats"][:, 1], stats[:, 1], (d + U) * stats[:, 1])
-    near(got["entropy"], H, d * (2 * math.log(max(V, 2)) + 2) + U * H)
+    near(got["stats"][:, 2], H, d * (2 * math.log(max(V, 2)) + 2) + U * H)
     near(got["stats"][:, 3], lse, d + U * lse.abs())
     if top:
         assert torch.equal(got["top_ids"].cpu().long(), ids)
@@ -218,7 +218,7 @@ def test_same_result_each_time(cuda):
     for _ in range(20):
         again = api.token_logprobs(lg, tokens, top=50)
         for k, v in first.items():
-            assert torch.equal(v, again[k])
+            assert torch.equal(v, again[k]), k
 
 
 def test_offsets_past_32_bits(cuda):
