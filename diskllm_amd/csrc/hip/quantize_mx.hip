@@ -78,7 +78,7 @@ template <int DT, int FMT>
 __global__ __launch_bounds__(kMxThreads) void quantize_mx_kernel(const typename LogitRow<DT>::T *__restrict__ x,
                                                                  int64_t ldx, int rows, int n, uint32_t per,
                                                                  uint8_t *__restrict__ q, int64_t ldq,
-                                                                 uint8_t *__restrict__ scale, int64_t lds) {
+                                                                 uint8_t *__restrict__ scale, int64_t lds, bool past) {
     typedef LogitRow<DT> In;
     const int lane = lane_id();
     const uint64_t first = ((uint64_t)blockIdx.x * (kMxThreads / 64) + __builtin_amdgcn_readfirstlane(wave_id())) * 64 * kMxSpans;
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(kMxThreads) void quantize_mx_kernel(const typename 
         const int64_t block = unit[s] >> 2;
         const int part = (int)(unit[s] & 3);
         if (FMT == DLK_MX_FP4) {
-            *(uint32_t *)(q + row[s] * ldq + block * 16 + part * 4) = w0;
+            store_past((uint32_t *)(q + row[s] * ldq + block * 16 + part * 4), w0, past);
         } else {
             /* three of a block's four threads store eight bytes each */
             const uint32_t n0 = quad<kQuadNext>(w0), n1 = quad<kQuadNext>(w1);
@@ -152,19 +152,32 @@ __global__ __launch_bounds__(kMxThreads) void quantize_mx_kernel(const typename 
 
 typedef uint32_t u1_any __attribute__((aligned(2)));
 
-/* Eight values of a group: w0 (and w1: the last 16 of 48 bits) times the scale of byte e. */
-template <int FMT>
-DLK_DEV void mx_values(uint32_t w0, uint32_t w1, uint32_t e, float (&v)[8]) {
+/* The bits of group `unit` of G values of a row at p. */
+template <int FMT, int G>
+DLK_DEV uint64_t mx_bits(const uint8_t *p, uint32_t unit) {
+    if (FMT == DLK_MX_FP4) {
+        p += (uint64_t)unit * (G / 2);
+        return G == 8 ? *(const uint32_t *)p : *(const uint16_t *)p;
+    }
+    p += (uint64_t)unit * (G / 4 * 3);
+    if (G == 8) return *(const u1_any *)p | (uint64_t) * (const uint16_t *)(p + 4) << 32;
+    return (uint32_t)p[0] | (uint32_t)p[1] << 8 | (uint32_t)p[2] << 16;
+}
+
+/* A group's values: its bits times the scale of byte e. */
+template <int FMT, int G>
+DLK_DEV void mx_values(uint64_t w, uint32_t e, float (&v)[G]) {
     const float by = u2f(e == 0 ? 0x400000u : e == 255 ? 0x7fc00000u : e << 23);
     if (FMT == DLK_MX_FP4) {
-        const f2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w0, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w0, 1.0f, 1);
-        const f2_t c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w0, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w0, 1.0f, 3);
+        const f2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4((uint32_t)w, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4((uint32_t)w, 1.0f, 1);
         v[0] = a.x * by; v[1] = a.y * by; v[2] = b.x * by; v[3] = b.y * by;
-        v[4] = c.x * by; v[5] = c.y * by; v[6] = d.x * by; v[7] = d.y * by;
+        if constexpr (G == 8) {
+            const f2_t c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4((uint32_t)w, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4((uint32_t)w, 1.0f, 3);
+            v[4] = c.x * by; v[5] = c.y * by; v[6] = d.x * by; v[7] = d.y * by;
+        }
     } else {
-        const uint64_t w = (uint64_t)w1 << 32 | w0;
 #pragma unroll
-        for (int c = 0; c < 8; c++) {
+        for (int c = 0; c < G; c++) {
             const uint32_t k = (uint32_t)(w >> (6 * c));
             /* the code's five bits as a float's last of the exponent and first of the mantissa: 2^-126 of the element */
             const float m = u2f((k & 31) << 20 | (k & 32) << 26);
@@ -173,17 +186,20 @@ DLK_DEV void mx_values(uint32_t w0, uint32_t w1, uint32_t e, float (&v)[8]) {
     }
 }
 
+/* 16 bytes of the output a thread and span, so that a wave's store is 1 KB in one piece. */
 template <int DT, int FMT>
 __global__ __launch_bounds__(kMxThreads) void dequantize_mx_kernel(const uint8_t *__restrict__ q, int64_t ldq,
                                                                    const uint8_t *__restrict__ scale, int64_t lds,
                                                                    int table_rows, const int32_t *__restrict__ ids,
                                                                    int rows, int n, uint32_t per,
-                                                                   typename LogitRow<DT>::T *__restrict__ out, int64_t ld) {
+                                                                   typename LogitRow<DT>::T *__restrict__ out, int64_t ld, bool past) {
     typedef LogitRow<DT> Out;
+    constexpr int G = Out::G;
     const int lane = lane_id();
     const uint64_t first = ((uint64_t)blockIdx.x * (kMxThreads / 64) + __builtin_amdgcn_readfirstlane(wave_id())) * 64 * kMxSpans;
     int64_t row[kMxSpans];
-    uint32_t unit[kMxSpans], w0[kMxSpans], w1[kMxSpans], e[kMxSpans];
+    uint32_t unit[kMxSpans], e[kMxSpans];
+    uint64_t w[kMxSpans];
     bool none[kMxSpans];
 #pragma unroll
     for (int s = 0; s < kMxSpans; s++) {
@@ -192,31 +208,23 @@ __global__ __launch_bounds__(kMxThreads) void dequantize_mx_kernel(const uint8_t
         int64_t from = ids ? (int64_t)ids[r] : r;
         none[s] = from < 0 || from >= table_rows;
         from = none[s] ? 0 : from;
-        const uint8_t *p = q + from * ldq;
-        if (FMT == DLK_MX_FP4) {
-            w0[s] = *(const uint32_t *)(p + (int64_t)unit[s] * 4);
-            w1[s] = 0;
-        } else {
-            w0[s] = *(const u1_any *)(p + (int64_t)unit[s] * 6);
-            w1[s] = *(const uint16_t *)(p + (int64_t)unit[s] * 6 + 4);
-        }
-        e[s] = scale[from * lds + (unit[s] >> 2)];
+        w[s] = mx_bits<FMT, G>(q + from * ldq, unit[s]);
+        e[s] = scale[from * lds + unit[s] / (32 / G)];
     }
 #pragma unroll
     for (int s = 0; s < kMxSpans; s++) {
         if (row[s] >= rows) continue;
-        float v[8];
-        mx_values<FMT>(w0[s], w1[s], e[s], v);
+        float v[G];
+        mx_values<FMT, G>(w[s], e[s], v);
 #pragma unroll
-        for (int c = 0; c < 8; c++) v[c] = none[s] ? 0.0f : v[c];
-        const int i = (int)unit[s] * 8;
+        for (int c = 0; c < G; c++) v[c] = none[s] ? 0.0f : v[c];
+        const int i = (int)unit[s] * G;
         typename Out::T *o = out + row[s] * ld + i;
-        if (i + 8 <= n) {
-#pragma unroll
-            for (int k = 0; k < 8 / Out::G; k++) *(typename Out::Raw *)(o + k * Out::G) = Out::pack(v + k * Out::G);
+        if (i + G <= n) {
+            store_past((typename Out::Raw *)o, Out::pack(v), past);
         } else {
 #pragma unroll
-            for (int c = 0; c < 8; c++)
+            for (int c = 0; c < G; c++)
                 if (i + c < n) Out::put(o + c, v[c]);
         }
     }
@@ -235,12 +243,13 @@ int launch_quantize_mx(const void *x, int64_t ldx, int rows, int n, int format, 
     const uint32_t per = (uint32_t)(((int64_t)n + 31) / 32 * 4);
     const unsigned blocks = mx_blocks(rows, per);
     if (blocks == 0) return DLK_ERR_UNSUPPORTED;
+    const bool past = (int64_t)rows * n >= 64 << 20 && whole_lines(q, ldq);
     if (format == DLK_MX_FP4)
         hipLaunchKernelGGL((quantize_mx_kernel<DT, DLK_MX_FP4>), dim3(blocks), dim3(kMxThreads), 0, stream, (P)x, ldx,
-                           rows, n, per, q, ldq, scale, lds);
+                           rows, n, per, q, ldq, scale, lds, past);
     else
         hipLaunchKernelGGL((quantize_mx_kernel<DT, DLK_MX_FP6>), dim3(blocks), dim3(kMxThreads), 0, stream, (P)x, ldx,
-                           rows, n, per, q, ldq, scale, lds);
+                           rows, n, per, q, ldq, scale, lds, past);
     return hipGetLastError() == hipSuccess ? DLK_OK : DLK_ERR_HIP;
 }
 
@@ -248,15 +257,19 @@ template <int DT>
 int launch_dequantize_mx(const uint8_t *q, int64_t ldq, const uint8_t *scale, int64_t lds, int table_rows,
                          const int32_t *ids, int rows, int n, int format, void *out, int64_t ld, hipStream_t stream) {
     typedef typename LogitRow<DT>::T *P;
-    const uint32_t per = (uint32_t)(((int64_t)n + 7) / 8);
+    constexpr int G = LogitRow<DT>::G;
+    /* (more than the L2 caches hold) */
+    const int64_t size = DT == DLK_F32 ? 4 : 2;
+    const bool past = rows * size * n >= 32 << 20 && whole_lines(out, ld * size);
+    const uint32_t per = (uint32_t)(((int64_t)n + G - 1) / G);
     const unsigned blocks = mx_blocks(rows, per);
     if (blocks == 0) return DLK_ERR_UNSUPPORTED;
     if (format == DLK_MX_FP4)
         hipLaunchKernelGGL((dequantize_mx_kernel<DT, DLK_MX_FP4>), dim3(blocks), dim3(kMxThreads), 0, stream, q, ldq,
-                           scale, lds, table_rows, ids, rows, n, per, (P)out, ld);
+                           scale, lds, table_rows, ids, rows, n, per, (P)out, ld, past);
     else
         hipLaunchKernelGGL((dequantize_mx_kernel<DT, DLK_MX_FP6>), dim3(blocks), dim3(kMxThreads), 0, stream, q, ldq,
-                           scale, lds, table_rows, ids, rows, n, per, (P)out, ld);
+                           scale, lds, table_rows, ids, rows, n, per, (P)out, ld, past);
     return hipGetLastError() == hipSuccess ? DLK_OK : DLK_ERR_HIP;
 }
 

@@ -28,6 +28,7 @@ struct GradParams {
     int64_t ld_grad;
     int V, given, pieces;
     float scale, inv_t;  /* log2(e) / T, 1 / T */
+    bool past;           /* stores go past the caches */
     int64_t r0;
 };
 
@@ -97,7 +98,7 @@ __global__ __launch_bounds__(kGradThreads) void token_logprobs_grad_kernel(GradP
             for (int c = 0; c < G; c++) y[c] += at == c && !none ? add : 0.0f;
         }
         if (i + G <= s1) {
-            *(typename In::Raw *)(out + i) = In::pack(y);
+            store_past((typename In::Raw *)(out + i), In::pack(y), p.past);
         } else {
 #pragma unroll
             for (int c = 0; c < G; c++)
@@ -138,6 +139,9 @@ extern "C" int dlk_token_logprobs_grad(const dlk_logprob_grad_batch *b, int rows
     p.grad = b->grad; p.ld_grad = b->ld_grad; p.V = vocab; p.given = prm->n_given;
     p.inv_t = 1.0f / prm->temperature;
     p.scale = (float)(1.4426950408889634 / (double)prm->temperature);
+    /* (64 x 151,936 bf16, 19 MB: 9.5 us past the caches, 10.9 through them; 48 x 50,257 float32, 10 MB: 7.9 both) */
+    const int64_t size = b->dtype == DLK_F32 ? 4 : 2;
+    p.past = rows * size * vocab >= 16 << 20 && whole_lines(b->grad, b->ld_grad * size);
     const int batch = kGradThreads * 4 * (b->dtype == DLK_F32 ? 4 : 8);
     p.pieces = (int)(((int64_t)vocab + batch - 1) / batch);
     /* (2^32 threads and over are no launch) */
