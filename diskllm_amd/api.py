@@ -486,9 +486,11 @@ def quantize_mx(x: torch.Tensor, fmt: str = "fp4", q: Optional[torch.Tensor] = N
     else:
         s_rows, s_n, lds = _rows2d(scale, dev, _U8, "scale")
         _want(s_rows == rows and s_n == blocks, "scale: [rows, blocks] is wanted")
+    at = q.data_ptr()
+    _want((at | ldq) & 7 == 0, "q: rows at multiples of 8 bytes are wanted")
     if rows:
-        _call(dev, stream, "dlk_quantize_mx", _lib.lib().dlk_quantize_mx, x.data_ptr(), dt, ldx, rows, n, kind,
-              q.data_ptr(), ldq, scale.data_ptr(), lds)
+        _call(dev, stream, "dlk_quantize_mx", _lib.lib().dlk_quantize_mx, x.data_ptr(), dt, ldx, rows, n, kind, at, ldq,
+              scale.data_ptr(), lds)
     return q, scale
 
 
@@ -501,6 +503,7 @@ def dequantize_mx(q: torch.Tensor, scale: torch.Tensor, n: Optional[int] = None,
     table, blocks, fmt, ldq, lds = _blocks_of(q, scale, dev, "q")
     n = blocks * 32 if n is None else n
     _want(blocks * 32 - 32 < n <= blocks * 32, "n: values of the last block are wanted")
+    _want((q.data_ptr() | ldq) & 7 == 0, "q: rows at multiples of 8 bytes are wanted")
     rows, at = table, 0
     if ids is not None:
         rows = ids.numel()
@@ -529,6 +532,14 @@ def logits_mx(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     V, w_blocks, w_fmt, ldw, ldws = _blocks_of(w, w_scale, dev, "w")
     _want(w_fmt == _lib.MX_FP4 and w_blocks == blocks, "w: 4-bit rows of x's length are wanted")
     _want(blocks <= 0x1ffffff, _WIDE.format("logits_mx"))
+    at, xs, wp, ws = x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr()
+    if rows > 1:                               # (the strides of a single row say nothing)
+        if (ldx & (15 if fmt == _lib.MX_FP4 else 7)) | (ldxs & 15):
+            raise ValueError("x, x_scale: rows at multiples of 16 bytes (6-bit x: 8) are wanted, as quantize_mx makes them")
+    if V > 1 and (ldw | ldws) & 15:
+        raise ValueError("w, w_scale: rows at multiples of 16 bytes are wanted, as quantize_mx makes them")
+    _want(at & (15 if fmt == _lib.MX_FP4 else 7) == 0 and (xs | wp | ws) & 15 == 0,
+          "tensors at multiples of 16 bytes (6-bit x: 8) are wanted")
     if out is None:
         ld = (V + 63) // 64 * 64
         out = _empty((rows, ld), _F32, x, dev, stream)
@@ -538,8 +549,7 @@ def logits_mx(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
         o_rows, o_n, ld = _rows2d(out, dev, _F32, "out")
         _want(o_rows == rows and o_n == V, "out: [rows, vocab] is wanted")
     if rows:
-        _call(dev, stream, "dlk_logits_mx", _lib.lib().dlk_logits_mx, x.data_ptr(), fmt, ldx, x_scale.data_ptr(), ldxs,
-              w.data_ptr(), ldw, w_scale.data_ptr(), ldws, rows, V, blocks * 32, softcap, out.data_ptr(), ld)
+        _call(dev, stream, "dlk_logits_mx", _lib.lib().dlk_logits_mx, at, fmt, ldx, xs, ldxs, wp, ldw, ws, ldws, rows, V, blocks * 32, softcap, out.data_ptr(), ld)
     return out
 
 

@@ -187,6 +187,7 @@ def check_product(torch, x, xs, w, ws, fmt, softcap=0.0, out=None):
 @pytest.mark.parametrize("rows,vocab,n", [
     (1, 1, 1), (1, 64, 32), (2, 65, 33), (16, 63, 511), (17, 129, 512), (15, 200, 513), (32, 1000, 2047), (33, 257, 96),
     (64, 300, 1024), (65, 100, 1000), (128, 259, 4096), (129, 511, 256), (200, 256, 257), (385, 513, 640), (513, 300, 40),
+    (256, 256, 256), (256, 300, 32), (257, 255, 512), (500, 1000, 288), (512, 257, 4128), (1000, 256, 33), (640, 520, 513),
     (1, 5000, 8192), (3, 70, 31)])
 def test_product(cuda, fmt, rows, vocab, n):
     import torch
@@ -214,6 +215,20 @@ def test_product_strided(cuda, fmt, rows):
     room = torch.full((rows, vocab + 7), 5.0, device="cuda")
     check_product(torch, X[:, 16:16 + x.shape[1]], xs, W[:, 32:32 + w.shape[1]], ws, fmt, out=room[:, 3:3 + vocab])
     assert (room[:, :3] == 5).all() and (room[:, 3 + vocab:] == 5).all()
+
+
+def test_product_of_many_rows_is_each_rows_own(cuda):
+    """Tiles that lie over one another compute the same bits: a row's logits do not depend on where it stands among 256
+    or more, nor an id's among the others, and every call gives the same."""
+    import torch
+    from diskllm_amd import api
+    x, xs, w, ws = inputs(torch, 700, 601, 520, "fp4")
+    all_rows = check_product(torch, x, xs, w, ws, "fp4")
+    for _ in range(5):
+        assert torch.equal(api.logits_mx(x, xs, w, ws), all_rows)
+    for a, b in ((0, 256), (444, 700), (17, 500)):
+        assert torch.equal(api.logits_mx(x[a:b], xs[a:b], w, ws), all_rows[a:b])
+    assert torch.equal(api.logits_mx(x, xs, w[89:], ws[89:]), all_rows[:, 89:])
 
 
 def test_product_fp6_rows_of_odd_blocks(cuda):

@@ -134,6 +134,20 @@ def test_masked(cuda, dtype, rows, V, T):
     assert status.item() == 0
 
 
+def test_long_rows(cuda):
+    """More batches than a workgroup keeps records of."""
+    lg, tokens, _ = some(1, 17_000_001, "f32", 2)
+    lg[0, ::1000] = lg[0].amax() + 1                             # ties at the top, far apart
+    check(lg, tokens, 40)
+    lg, tokens, _ = some(258, 270_001, "bf16", 1, spread=1.0)
+    lg[7, 3::50_000] = 9.0
+    check(lg[:8], tokens[:8], 5)
+    import diskllm_amd.api as api
+    few, all_rows = api.token_logprobs(lg[:8], tokens[:8], top=5), api.token_logprobs(lg, tokens, top=5)
+    assert torch.equal(few["top_ids"], all_rows["top_ids"][:8])
+    near(all_rows["logprobs"][:8], few["logprobs"].double().cpu(), 2 * delta(270_001, torch.bfloat16))
+
+
 def test_mask_rows_shared(cuda):
     """mask_row names the mask of each row."""
     lg, tokens, g = some(6, 5000, "f32", 1)

@@ -155,6 +155,11 @@ def f32(*shape):
     lambda: api.logits_mx(u8(2, 32), u8(2, 2), u8(9, 48), u8(9, 3)),
     lambda: api.logits_mx(u8(2, 32), u8(2, 2), u8(9, 32), u8(9, 2), out=f32(2, 8)),
     lambda: api.logits_mx(u8(2, 32).char(), u8(2, 2), u8(9, 32), u8(9, 2)),
+    lambda: api.logits_mx(u8(2, 48)[:, :32], u8(2, 16)[:, :2], u8(9, 32), u8(9, 2)),              # packed scales
+    lambda: api.logits_mx(u8(2, 40)[:, :32], u8(2, 16)[:, :2], u8(9, 32), u8(9, 16)[:, :2]),
+    lambda: api.logits_mx(u8(2, 32), u8(2, 16)[:, :2], u8(9 * 32 + 8)[8:].view(9, 32), u8(9, 16)[:, :2]),
+    lambda: api.quantize_mx(f32(4, 64), q=u8(4, 36)[:, :32]),
+    lambda: api.dequantize_mx(u8(4, 36)[:, :32], u8(4, 2)),
     lambda: api.token_logprobs(f32(2, 9)),                                         # not on a GPU
     lambda: api.token_logprobs(f32(2, 9).double()),
     lambda: api.token_logprobs(f32(2, 9), torch.zeros(2, dtype=torch.int64)),
@@ -179,3 +184,57 @@ def f32(*shape):
 def test_python(fn):
     with pytest.raises(ValueError):
         fn()
+
+
+@pytest.fixture
+def on_no_device(monkeypatch):
+    """CPU or meta tensors taken for the GPU's, calls recorded and not made; returns what was called."""
+    calls = []
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    monkeypatch.setattr(api, "_call", lambda dev, stream, what, fn, *args: calls.append((what, stream, args)))
+    return calls
+
+
+def test_counts_past_32_bits(on_no_device):
+    """What ctypes would cut to its low 32 bits is refused."""
+    big = 1 << 32
+    meta = lambda *shape, **kw: torch.empty(shape, device="meta", **kw)
+    for bad in (lambda: api.quantize_mx(meta(big + 1, 32)), lambda: api.quantize_mx(meta(1, big + 32)),
+                lambda: api.dequantize_mx(u8(4, 32), u8(4, 2), ids=meta(big + 1, dtype=torch.int32)),
+                lambda: api.logits_mx(meta(big + 1, 16, dtype=torch.uint8), meta(big + 1, 1, dtype=torch.uint8),
+                                      u8(9, 16), u8(9, 1)),
+                lambda: api.token_logprobs(meta(big + 1, 9)), lambda: api.token_logprobs(meta(1, big + 9)),
+                lambda: api.token_logprobs(f32(2, 9), top=big + 1)):
+        with pytest.raises(ValueError):
+            bad()
+    assert on_no_device == []
+
+
+@pytest.mark.parametrize("current,stream,made_on", [(111, 222, 222), (111, 0, 0), (111, 111, None), (111, None, None)])
+def test_outputs_are_made_on_the_calls_stream(on_no_device, monkeypatch, current, stream, made_on):
+    """Outputs that a call makes come from the memory of the stream that writes them."""
+    import contextlib
+    now, made = [None], []
+
+    @contextlib.contextmanager
+    def on(s):
+        before, now[0] = now[0], s
+        yield
+        now[0] = before
+    empty = torch.empty
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda at, device=None: at)
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: current, raising=False)
+    # (16-byte aligned, as the allocator's)
+    aligned = torch.zeros(1 << 16, dtype=torch.uint8)
+    aligned = aligned[-aligned.data_ptr() % 64:]
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: made.append(now[0]) or empty(*a, **kw))
+    q, s = aligned[:64].view(2, 32), aligned[64:96].view(2, 16)[:, :2]
+    api.quantize_mx(f32(4, 64), q=aligned[:128].view(4, 32), stream=stream)                         # the scales
+    api.dequantize_mx(q, s, stream=stream)
+    api.logits_mx(q, s, q, s, stream=stream)
+    api.token_logprobs(f32(2, 9), i32(2), top=3, stream=stream)                                   # four
+    api.token_logprobs_grad(f32(2, 9), i32(2), f32(2, 4), f32(2), stream=stream)
+    assert [s for _, s, _ in on_no_device] == [stream] * 5
+    assert made == [made_on] * 8 and now == [None]
