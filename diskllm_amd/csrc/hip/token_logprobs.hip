@@ -386,9 +386,12 @@ __global__ __launch_bounds__(kLogprobThreads, 4) void token_logprobs_kernel(Logp
 #pragma unroll
                     for (int c = 0; c < G; c++) x[j][c] = -INFINITY;
             }
+            /* (equal to the bound's logit, of ids above the bound's: none of them; where all logits are equal that is all) */
+            const bool equal_too = ((bound >> 32 << 32) | (uint32_t)~place(b0, 0)) >= bound;
+            const float from_here = equal_too ? least : key_value(~((uint32_t)(bound >> 32) + 1));
             uint32_t at_least = 0;                           /* bit j * G + c */
 #pragma unroll
-            for (int q = 0; q < E; q++) at_least |= x[q / G][q % G] >= least && x[q / G][q % G] > -INFINITY ? 1u << q : 0u;
+            for (int q = 0; q < E; q++) at_least |= x[q / G][q % G] >= from_here && x[q / G][q % G] > -INFINITY ? 1u << q : 0u;
 #pragma unroll 1
             while (ballot(at_least != 0) != 0) {
                 const int k = at_least != 0 ? __builtin_ctz(at_least) : 0;
