@@ -5,7 +5,7 @@ Layout:
   csrc/host/  C11 drop-in implementations of include/sampler.h and include/grammar.h
   _lib.py     ctypes binding of the built libdiskllm_amd.so
   api.py      Python host side of the batched path (torch only for device memory/streams), and
-              tensor functions of the 8-bit LM head and the beam step
+              tensor functions of the 8-bit and 4-bit LM heads, the beam step and the scores of tokens
   workloads.py the synthetic configurations C1-C5
 """
 from ._lib import build, lib  # noqa: F401

@@ -10,6 +10,13 @@
  * group of the instruction's four need not be the k-th block as long as both sides agree: of
  * 16 blocks lane group g takes 4 g .. 4 g + 3 in turn, whose four scales are one word of the
  * scales' row, picked by the instruction.  w is its first operand, as in logits_i8.hip.
+ *
+ * Bounds.  Few rows: w's bytes, as there (16 x 151,936 x 4,096 in 66 us with 6-bit hidden states, 5.1 TB/s; a large
+ * copy: 4.9).  Many: the products and what feeds them, 512 x 262,144 x 4,096 in 380 us, 390-412 with the cap, of which
+ * some 80 write 537 MB after each workgroup's loop; between n = 4,096 and 8,192 3.56 PFLOP/s (a library product of
+ * 16,384^3 in this format, written in 16 bits: 3.32 in all).  The loop has the matrix cores busy for 40% of its cycles
+ * at a clock that falls to some 1.8 GHz; its LDS reads met none of the same bank once chunks lay as mx_spot() has them,
+ * which changed nothing, nor did more stages of half the length.
  */
 #include <math.h>
 
@@ -433,6 +440,15 @@ int launch_mx_wide(const MxParams &p, hipStream_t stream) {
 
 template <int FMT>
 int launch_mx_tiles(const MxParams &p, hipStream_t stream) {
+    /* Tiles by the rows (us at 151,936 ids of n = 4,096, hidden states of 4 and of 6 bits):
+     *   16 rows     64 ids, 16 blocks a step, 2 stages 68, 70; 3 stages 69, 80; 128 ids, 8 blocks, 3 stages 71, 72
+     *   32          128 ids, 8 blocks, 3 stages 78, 84; 64 ids, 16 blocks, 2 stages 78-83, 82; 256 ids 91, 99
+     *   64          64 ids, 16 blocks, 2 stages 88, 126; 128 ids, 8 blocks, 3 stages 89, 95; 256 ids 93, 98
+     *   128         128 x 128 111, 134; 128 x 256 117, 125
+     *   200         256 x 256 142, -; 128 x 256 160, 186; 128 x 128 154, 247
+     *   300         128 x 128 198, 331; 256 x 256 210, -; 128 x 256 220, 257
+     *   512         256 x 256 by quarters 229; at once 234, -; 128 x 256 314, 368; 128 x 128 286, 480
+     * (two stages of 256 rows in 6 bits do not fit LDS) */
     if (p.rows <= 16) return launch_mx<FMT, 16, 64, 1, 4, 16, 2>(p, stream);
     if (p.rows <= 32) return launch_mx<FMT, 32, 128, 1, 4, 8, 3>(p, stream);
     if (FMT == DLK_MX_FP6) {

@@ -12,6 +12,9 @@
  *
  * Bound by memory: eight values a thread (16-byte loads of 16-bit types), four threads a
  * block, a wave's 64 groups side by side over the ends of rows, four such spans a wave.
+ * 100,001 x 4,090 bfloat16 to 4 bits 198-226 us, 4.6-5.3 TB/s (a large copy: 4.9), and back 176,
+ * 5.8; 8,192 rows of a table of 151,936 x 4,096 by id as float32 23.7, 6.4; one row of 4,096 3.4
+ * and 3.1, a launch and a round trip.  Eight spans a wave, or two, were no faster.
  */
 #include "logit_row.h"
 

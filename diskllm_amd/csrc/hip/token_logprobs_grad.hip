@@ -7,7 +7,9 @@
  * with p_v = 2^((l_v - max) * log2(e) / T) / z of the statistics that the forward call left, so
  * that a row is read once and no workgroup waits for another.  Bound by memory: 256 threads,
  * 16-byte groups, a wave's 64 groups side by side, of which it knows by one ballot of the
- * tokens (a lane each) whether any lies there.
+ * tokens (a lane each) whether any lies there.  2,048 x 151,936 bfloat16 216 us, 5.75 TB/s read
+ * and written (a large copy: 4.9); 48 x 50,257 float32 6.5-7.2, its statistics and tokens a round
+ * trip before the first product.
  */
 #include "logit_row.h"
 #include "../../../include/diskllm_amd.h"
