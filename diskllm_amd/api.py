@@ -623,9 +623,10 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: Optional[torch.Tensor], st
     g = _flat(grad_logprobs, rows * given, dev, _F32, "grad_logprobs") if given else 0
     h = 0 if grad_entropy is None else _flat(grad_entropy, rows, dev, _F32, "grad_entropy")
     if out is None:
-        out = _empty((rows, V), logits.dtype, logits, dev, stream)
-    o_rows, o_n, ld_out = _rows2d(out, dev, logits.dtype, "out")
-    _want(o_rows == rows and o_n == V, "out: logits' shape is wanted")
+        out, ld_out = _empty((rows, V), logits.dtype, logits, dev, stream), V
+    else:
+        o_rows, o_n, ld_out = _rows2d(out, dev, logits.dtype, "out")
+        _want(o_rows == rows and o_n == V, "out: logits' shape is wanted")
     if rows:
         _call(dev, stream, "dlk_token_logprobs_grad", _lib.lib().dlk_token_logprobs_grad,
               _lib.LogprobGradBatch(logits.data_ptr(), dt, ld, mk, mask_ld, mr, at, st, g, h, out.data_ptr(), ld_out),

@@ -444,16 +444,17 @@ int launch_mx_tiles(const MxParams &p, hipStream_t stream) {
      *   16 rows     64 ids, 16 blocks a step, 2 stages 68, 70; 3 stages 69, 80; 128 ids, 8 blocks, 3 stages 71, 72
      *   32          128 ids, 8 blocks, 3 stages 78, 84; 64 ids, 16 blocks, 2 stages 78-83, 82; 256 ids 91, 99
      *   64          64 ids, 16 blocks, 2 stages 88, 126; 128 ids, 8 blocks, 3 stages 89, 95; 256 ids 93, 98
-     *   128         128 x 128 111, 134; 128 x 256 117, 125
-     *   200         256 x 256 142, -; 128 x 256 160, 186; 128 x 128 154, 247
-     *   300         128 x 128 198, 331; 256 x 256 210, -; 128 x 256 220, 257
-     *   512         256 x 256 by quarters 229; at once 234, -; 128 x 256 314, 368; 128 x 128 286, 480
-     * (two stages of 256 rows in 6 bits do not fit LDS) */
+     *   128         128 x 128 111, 134; 128 x 256 117, 117
+     *   200         256 x 256 142, -; 128 x 256 160, 172; 128 x 128 154, 237
+     *   300         128 x 128 198, 332; 256 x 256 210, -; 128 x 256 220, 241
+     *   512         256 x 256 by quarters 229; at once 234, -; 128 x 256 314, 354; 128 x 128 286, 458
+     * (128 x 256 in 6 bits with a wave's 32 rows of 128 ids; 64 of 64: 120, 178, 252, 399;
+     * two stages of 256 rows in 6 bits do not fit LDS) */
     if (p.rows <= 16) return launch_mx<FMT, 16, 64, 1, 4, 16, 2>(p, stream);
     if (p.rows <= 32) return launch_mx<FMT, 32, 128, 1, 4, 8, 3>(p, stream);
     if (FMT == DLK_MX_FP6) {
         if (p.rows <= 64) return launch_mx<DLK_MX_FP6, 64, 128, 2, 2, 8, 3>(p, stream);
-        return launch_mx<DLK_MX_FP6, 128, 256, 2, 4, 8, 2>(p, stream);
+        return launch_mx<DLK_MX_FP6, 128, 256, 4, 2, 8, 2>(p, stream);
     }
     if (p.rows <= 64) return launch_mx<DLK_MX_FP4, 64, 64, 2, 2, 16, 2>(p, stream);
     if (p.rows <= 128) return launch_mx<DLK_MX_FP4, 128, 128, 2, 2, 8, 2>(p, stream);
