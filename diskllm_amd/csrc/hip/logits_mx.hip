@@ -448,8 +448,9 @@ int launch_mx_tiles(const MxParams &p, hipStream_t stream) {
      *   200         256 x 256 142, -; 128 x 256 160, 172; 128 x 128 154, 237
      *   300         128 x 128 198, 332; 256 x 256 210, -; 128 x 256 220, 241
      *   512         256 x 256 by quarters 229; at once 234, -; 128 x 256 314, 354; 128 x 128 286, 458
-     * (128 x 256 in 6 bits with a wave's 32 rows of 128 ids; 64 of 64: 120, 178, 252, 399;
-     * two stages of 256 rows in 6 bits do not fit LDS) */
+     * (128 x 256 in 6 bits: a wave has 32 rows of 128 ids; with 64 of 64 120, 178, 252, 399.  256 x 256 at once: 64
+     * rows of 128 ids; with 128 of 64 as long, and 200 x 50,257 x 1,024 24.2 for 22.5.  Two stages of 256 rows in 6
+     * bits do not fit LDS) */
     if (p.rows <= 16) return launch_mx<FMT, 16, 64, 1, 4, 16, 2>(p, stream);
     if (p.rows <= 32) return launch_mx<FMT, 32, 128, 1, 4, 8, 3>(p, stream);
     if (FMT == DLK_MX_FP6) {
@@ -458,7 +459,7 @@ int launch_mx_tiles(const MxParams &p, hipStream_t stream) {
     }
     if (p.rows <= 64) return launch_mx<DLK_MX_FP4, 64, 64, 2, 2, 16, 2>(p, stream);
     if (p.rows <= 128) return launch_mx<DLK_MX_FP4, 128, 128, 2, 2, 8, 2>(p, stream);
-    if (p.rows < 256) return launch_mx<DLK_MX_FP4, 256, 256, 2, 4, 8, 2>(p, stream);
+    if (p.rows < 256) return launch_mx<DLK_MX_FP4, 256, 256, 4, 2, 8, 2>(p, stream);
     /* past that tiles of 256 rows where they leave little empty (and a lane's offsets in a tile fit 32 bits) */
     const int64_t by128 = ((int64_t)p.rows + 127) / 128 * 128, by256 = ((int64_t)p.rows + 255) / 256 * 256;
     const bool near = ((p.ldx | p.ldw | p.ldxs | p.ldws) >> 22) == 0;
