@@ -295,12 +295,12 @@ int dlk_logits_i8(const int8_t *x, int64_t ldx, const float *x_scale, const int8
 #define DLK_MX_FP6 1
 
 /* Blocks of each row of x [rows, n] (DLK_F32, DLK_BF16 or DLK_F16; strides in elements).  A
- * block's scale is 2^(floor(log2(max |x|)) - 2), at least 2^-127; its elements are x over that to the nearest, halves to the even code, decided exactly, and
- * at most the largest element.  A block of zeros: scale 2^-127 and zeros; one that holds
- * NaN or infinity: scale 255 and zeros.  The last block of a row is filled with zeros.  q
- * takes ceil(n / 32) * 16 (FP6: 24) bytes a row at q + r * ldq, 8-byte aligned (ldq too); scale
- * ceil(n / 32) bytes a row at scale + r * ld_scale, of any alignment.  x needs its elements'
- * alignment; no overlaps. */
+ * block's scale is 2^(floor(log2(max |x|)) - 2), at least 2^-127; its elements are x over that
+ * to the nearest, halves to the even code, decided exactly, and at most the largest element.
+ * A block of zeros: scale 2^-127 and zeros; one that holds NaN or infinity: scale 255 and
+ * zeros.  The last block of a row is filled with zeros.  q takes ceil(n / 32) * 16 (FP6: 24)
+ * bytes a row at q + r * ldq, 8-byte aligned (ldq too); scale ceil(n / 32) bytes a row at
+ * scale + r * ld_scale, of any alignment.  x needs its elements' alignment; no overlaps. */
 int dlk_quantize_mx(const void *x, int dtype, int64_t ldx, int rows, int n, int format, uint8_t *q, int64_t ldq,
                     uint8_t *scale, int64_t ld_scale, hipStream_t stream);
 
@@ -315,11 +315,11 @@ int dlk_dequantize_mx(const uint8_t *q, int64_t ldq, const uint8_t *scale, int64
 
 /* logits[r * ld + v] = sum over the ceil(n / 32) blocks of x's row r (x_format) and w's row v
  * (FP4) of their values' products; softcap as in dlk_logits_i8.  The products of a block are
- * exact, sums are in 32 bits: off by at most 2^-22 of the sum of the products' sizes for each
- * 128 values.  A block with scale 255 makes its row's logits NaN.  x, w and the scales: 16-byte aligned
- * (x in FP6: 8), strides too (the bytes of a row of scales up to the next multiple of 16 are read; what
- * stands there does not matter).  Entries past vocab in a row of logits are left as they are; logits may not overlap
- * the inputs. */
+ * exact, sums are in 32 bits: off by at most 2^-20 of the sum of the products' sizes for each
+ * 512 values or part of them (four sums).  A block with scale 255 makes its row's logits NaN.
+ * x, w and the scales: 16-byte aligned (x in FP6: 8), strides too (the bytes of a row of
+ * scales up to the next multiple of 16 are read; what stands there does not matter).  Entries
+ * past vocab in a row of logits are left as they are; logits may not overlap the inputs. */
 int dlk_logits_mx(const uint8_t *x, int x_format, int64_t ldx, const uint8_t *x_scale, int64_t ldxs, const uint8_t *w,
                   int64_t ldw, const uint8_t *w_scale, int64_t ldws, int rows, int vocab, int n, float softcap,
                   float *logits, int64_t ld, hipStream_t stream);
@@ -359,9 +359,10 @@ typedef struct {
  * the others); the entropy -sum p log p.  The logits are read once.  A row without an allowed logit
  * above -inf: log-probabilities -inf, statistics -inf, 0, 0 and -inf, no alternatives.  A
  * row whose allowed logits hold NaN or +inf: NaN (ids -1), and DLK_STATUS_NOT_FINITE; what stands in
- * places that are not allowed does not matter.  Exponentials and sums of up to 32 terms in 32 bits, the rest in
- * 64: log-probabilities are off by their own rounding and 1.5e-5 at most at up to 262,144 logits a row (some
- * 2e-7 as measured).  Takes workspace as dlk_sample does where rows are few (dlk_release_stream; one call on the stream before capturing it, else
+ * places that are not allowed does not matter.  Exponentials and sums of up to 32 terms in
+ * 32 bits, the rest in 64: log-probabilities are off by their own rounding and 1.5e-5 at most
+ * at up to 262,144 logits a row (some 2e-7 as measured).  Takes workspace as dlk_sample does
+ * where rows are few (dlk_release_stream; one call on the stream before capturing it, else
  * DLK_ERR_HIP).  Outputs may not overlap inputs. */
 int dlk_token_logprobs(const dlk_logprob_batch *batch, int rows, int vocab, const dlk_logprob_params *params,
                        hipStream_t stream);

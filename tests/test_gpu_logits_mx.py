@@ -217,6 +217,28 @@ def test_product_strided(cuda, fmt, rows):
     assert (room[:, :3] == 5).all() and (room[:, 3 + vocab:] == 5).all()
 
 
+@pytest.mark.parametrize("rows,vocab,n", [(500, 301, 300), (256, 258, 1056), (300, 259, 600)])
+@pytest.mark.parametrize("far", [False, True])
+def test_product_of_many_rows_strided(cuda, rows, vocab, n, far):
+    """Rows of hidden states, weights and scales apart (weights by 4 MB: past the offsets of one tile), logits in a
+    larger matrix, at a place of its own in a row."""
+    import torch
+    x, xs, w, ws = inputs(torch, rows, vocab, n, "fp4")
+    blocks = xs.shape[1]
+    X = torch.full((rows, x.shape[1] + 32), 255, dtype=torch.uint8, device="cuda")
+    X[:, 16:16 + x.shape[1]] = x
+    W = torch.full((vocab, 1 << 22 if far else w.shape[1] + 48), 255, dtype=torch.uint8, device="cuda")
+    W[:, 32:32 + w.shape[1]] = w
+    XS = torch.full((rows, (blocks + 15) // 16 * 16 + 16), 255, dtype=torch.uint8, device="cuda")
+    XS[:, 16:16 + blocks] = xs
+    WS = torch.full((vocab, (blocks + 15) // 16 * 16 + 32), 255, dtype=torch.uint8, device="cuda")
+    WS[:, 16:16 + blocks] = ws
+    room = torch.full((rows + 1, vocab + 7), 5.0, device="cuda")
+    check_product(torch, X[:, 16:16 + x.shape[1]], XS[:, 16:16 + blocks], W[:, 32:32 + w.shape[1]], WS[:, 16:16 + blocks],
+                  "fp4", out=room[:rows, 3:3 + vocab])
+    assert (room[:rows, :3] == 5).all() and (room[:rows, 3 + vocab:] == 5).all() and (room[rows] == 5).all()
+
+
 def test_product_of_many_rows_is_each_rows_own(cuda):
     """Tiles that lie over one another compute the same bits: a row's logits do not depend on where it stands among 256
     or more, nor an id's among the others, and every call gives the same."""
