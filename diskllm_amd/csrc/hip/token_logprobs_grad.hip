@@ -4,12 +4,15 @@
  *
  *   dl_v = (1 / T) * (sum_j g_j [v = token_j] - p_v * (sum_j g_j + h * (log p_v + entropy)))
  *
- * with p_v = 2^((l_v - max) * log2(e) / T) / z of the statistics that the forward call left, so
- * that a row is read once and no workgroup waits for another.  Bound by memory: 256 threads,
- * 16-byte groups, a wave's 64 groups side by side, of which it knows by one ballot of the
- * tokens (a lane each) whether any lies there.  2,048 x 151,936 bfloat16 216 us, 5.75 TB/s read
- * and written (a large copy: 4.9); 48 x 50,257 float32 6.5-7.2, its statistics and tokens a round
- * trip before the first product.
+ * over the given tokens whose own logit is above -inf (-inf is a mask as the bits are), with
+ * p_v = 2^((l_v - max) * log2(e) / T) / z of the statistics that the forward call left, so that a
+ * row is read once and no workgroup waits for another.  Bound by memory: 256 threads, 16-byte
+ * groups, a wave's 64 groups side by side, of which it knows by one ballot of the tokens (a lane
+ * each) whether any lies there.  2,048 x 151,936 bfloat16 215 us, 5.8 TB/s read and written (a
+ * large copy: 4.9); 48 x 50,257 float32 5.9 within a graph, its statistics and tokens, and then the tokens' logits,
+ * a round trip each before the first product.  Over the logits the tokens' groups are a launch of their
+ * own (48 x 50,257 with four tokens a row 9.6, 2,048 x 151,936 bfloat16 250; in one launch, which could
+ * take a stored gradient for a token's logit, 6.5 and 245).
  */
 #include "logit_row.h"
 #include "../../../include/diskllm_amd.h"
@@ -34,12 +37,68 @@ struct GradParams {
     int64_t r0;
 };
 
-/* Row blockIdx.x / pieces, piece blockIdx.x % pieces: four groups a thread. */
+/* Lane k's v, k the same in all lanes. */
+DLK_DEV int32_t of_lane(int32_t v, int k) { return __builtin_amdgcn_readlane(v, k); }
+DLK_DEV float of_lane(float v, int k) { return u2f((uint32_t)__builtin_amdgcn_readlane((int)f2u(v), k)); }
+
+/* What a row's workgroups all know of it. */
+struct GradRow {
+    int32_t held, token;     /* this lane's given token: that the mask allows, that counts (its logit above -inf); else -1 */
+    float g;                 /* its weight, 0 where it does not count */
+    float top, by, by_t;     /* p's weight is by + by_t * (the logit's exponent of 2) */
+    bool none;               /* no allowed id, or nothing to differentiate (whatever the logits hold): zeros */
+};
+
 template <int DT, bool ENTROPY>
+DLK_DEV GradRow grad_row(const GradParams &p, int64_t row, const typename LogitRow<DT>::T *lg, const uint32_t *mw) {
+    GradRow r;
+    const int lane = lane_id();
+    const float z = p.stats[row * 4 + 1], entropy = p.stats[row * 4 + 2];
+    r.top = p.stats[row * 4];
+    r.token = -1;
+    r.g = 0.0f;
+    if (lane < p.given) {
+        r.token = p.tokens[row * p.given + lane];
+        r.g = p.g[row * p.given + lane];
+    }
+    if (r.token < 0 || r.token >= p.V || !mask_allows(mw, r.token)) r.token = -1;
+    r.held = r.token;
+    if (r.token >= 0 && LogitRow<DT>::one(lg + r.token) == -INFINITY) r.token = -1;
+    if (r.token < 0) r.g = 0.0f;
+    float h = 0.0f;
+    if (ENTROPY) h = p.h[row];
+    float total = 0.0f;
+#pragma unroll 1
+    for (int j = 0; j < p.given; j++) total += of_lane(r.g, j);
+    r.none = r.top == -INFINITY || (ballot(r.g != 0.0f) == 0 && h == 0.0f);
+    const float per = p.inv_t * (1.0f / z);
+    r.by = ENTROPY ? (total + h * (entropy - logf(z))) * per : total * per;
+    r.by_t = ENTROPY ? h * 0.693147180559945309f * per : 0.0f;
+    return r;
+}
+
+/* -p_v * its weight for the group of logits x at i. */
+template <int DT, bool ENTROPY>
+DLK_DEV void grad_group(const GradParams &p, const GradRow &r, const uint32_t *mw, int i, const float (&x)[LogitRow<DT>::G],
+                        float (&y)[LogitRow<DT>::G]) {
+    uint32_t bits = 0xffffffffu;
+    if (mw) bits = mw[min(i, p.V - 1) >> 5] >> (i & 31);
+#pragma unroll
+    for (int c = 0; c < LogitRow<DT>::G; c++) {
+        const float d = (x[c] - r.top) * p.scale, e = __builtin_amdgcn_exp2f(d);
+        y[c] = ENTROPY ? -e * fmaf(r.by_t, fmaxf(d, -200.0f), r.by) : -e * r.by;
+        if (mw) y[c] = (bits >> c & 1) != 0 ? y[c] : 0.0f;
+        y[c] = r.none || x[c] == -INFINITY ? 0.0f : y[c];
+    }
+}
+
+/* Row blockIdx.x / pieces, piece blockIdx.x % pieces: four groups a thread.  OVER: the gradient goes over the logits;
+ * every workgroup of a row reads its tokens' logits, so their groups are left to the kernel below. */
+template <int DT, bool ENTROPY, bool OVER>
 __global__ __launch_bounds__(kGradThreads) void token_logprobs_grad_kernel(GradParams p) {
     typedef LogitRow<DT> In;
     constexpr int T = kGradThreads, GR = 4, G = In::G, B = T * GR * G;
-    const int t = threadIdx.x, lane = lane_id();
+    const int t = threadIdx.x;
     const int64_t row = p.r0 + blockIdx.x / p.pieces;
     const int b0 = (int)(blockIdx.x % p.pieces) * B;
     const typename In::T *lg = (const typename In::T *)p.logits + row * p.ld;
@@ -51,26 +110,7 @@ __global__ __launch_bounds__(kGradThreads) void token_logprobs_grad_kernel(GradP
 #pragma unroll
     for (int j = 0; j < GR; j++)
         if (place(j) + G <= s1) raw[j] = *(const typename In::Raw *)(lg + place(j));
-    const float top = p.stats[row * 4], z = p.stats[row * 4 + 1], entropy = p.stats[row * 4 + 2];
-    /* a token a lane (every wave holds them all); one that counts for nothing is -1 */
-    int32_t token = -1;
-    float g = 0.0f;
-    if (lane < p.given) {
-        token = p.tokens[row * p.given + lane];
-        if (token < 0 || token >= p.V || !mask_allows(mw, token)) token = -1;
-        if (token >= 0) g = p.g[row * p.given + lane];
-    }
-    float h = 0.0f;
-    if (ENTROPY) h = p.h[row];
-    float total = 0.0f;
-#pragma unroll 1
-    for (int j = 0; j < p.given; j++) total += shfl(g, j);
-    /* no allowed id, or nothing to differentiate (whatever the logits hold): zeros */
-    const bool none = top == -INFINITY || (ballot(g != 0.0f) == 0 && h == 0.0f);
-    const float inv_z = 1.0f / z;
-    const float per = p.inv_t * inv_z;
-    const float by = ENTROPY ? (total + h * (entropy - logf(z))) * per : total * per;
-    const float by_t = ENTROPY ? h * 0.693147180559945309f * per : 0.0f;
+    const GradRow r = grad_row<DT, ENTROPY>(p, row, lg, mw);
 #pragma unroll
     for (int j = 0; j < GR; j++) {
         const int i = place(j);
@@ -81,24 +121,23 @@ __global__ __launch_bounds__(kGradThreads) void token_logprobs_grad_kernel(GradP
 #pragma unroll
             for (int c = 0; c < G; c++) x[c] = i + c < s1 ? In::one(lg + i + c) : -INFINITY;
         }
-        uint32_t bits = 0xffffffffu;
-        if (mw) bits = mw[min(i, s1 - 1) >> 5] >> (i & 31);
-#pragma unroll
-        for (int c = 0; c < G; c++) {
-            const float d = (x[c] - top) * p.scale, e = __builtin_amdgcn_exp2f(d);
-            y[c] = ENTROPY ? -e * fmaf(by_t, fmaxf(d, -200.0f), by) : -e * by;
-            if (mw) y[c] = (bits >> c & 1) != 0 ? y[c] : 0.0f;
-            y[c] = none || x[c] == -INFINITY ? 0.0f : y[c];
-        }
+        grad_group<DT, ENTROPY>(p, r, mw, i, x, y);
         /* the wave's 64 groups lie side by side: the tokens among them, in their order */
         const int w0 = b0 + (j * T + (t & ~63)) * G;
-        for (uint64_t who = ballot(token >= w0 && token - w0 < 64 * G); who != 0; who &= who - 1) {
+        bool mine = true;
+        const int32_t of = OVER ? r.held : r.token;
+        for (uint64_t who = ballot(of >= w0 && of - w0 < 64 * G); who != 0; who &= who - 1) {
             const int k = __builtin_ctzll(who);
-            const int at = shfl(token, k) - i;
-            const float add = shfl(g, k) * p.inv_t;
+            const int at = shfl(of, k) - i;
+            if (OVER) {
+                mine &= at < 0 || at >= G;
+            } else {
+                const float add = shfl(r.g, k) * p.inv_t;
 #pragma unroll
-            for (int c = 0; c < G; c++) y[c] += at == c && !none ? add : 0.0f;
+                for (int c = 0; c < G; c++) y[c] += at == c && !r.none ? add : 0.0f;
+            }
         }
+        if (OVER && !mine) continue;
         if (i + G <= s1) {
             store_past((typename In::Raw *)(out + i), In::pack(y), p.past);
         } else {
@@ -109,13 +148,56 @@ __global__ __launch_bounds__(kGradThreads) void token_logprobs_grad_kernel(GradP
     }
 }
 
-template <int DT>
-int launch_grad(const GradParams &p, int64_t blocks, hipStream_t stream) {
-    if (p.h)
-        hipLaunchKernelGGL((token_logprobs_grad_kernel<DT, true>), dim3((unsigned)blocks), dim3(kGradThreads), 0, stream, p);
-    else
-        hipLaunchKernelGGL((token_logprobs_grad_kernel<DT, false>), dim3((unsigned)blocks), dim3(kGradThreads), 0, stream, p);
+/* The tokens' groups of a gradient over its logits, a wave a row and a lane a token: a wave has read all of its row's
+ * before it stores one. */
+template <int DT, bool ENTROPY>
+__global__ __launch_bounds__(kGradThreads) void token_logprobs_grad_tokens_kernel(GradParams p, int rows) {
+    typedef LogitRow<DT> In;
+    constexpr int G = In::G;
+    const int lane = lane_id(), n = (int)blockIdx.x * (kGradThreads / 64) + wave_id();
+    if (n >= rows) return;
+    const int64_t row = p.r0 + n;
+    typename In::T *lg = (typename In::T *)p.grad + row * p.ld_grad;
+    const uint32_t *mw = p.mask ? p.mask + (int64_t)(p.mask_row ? p.mask_row[row] : row) * p.mask_ld : nullptr;
+    const GradRow r = grad_row<DT, ENTROPY>(p, row, lg, mw);
+    const int i = max(r.held, 0) / G * G;
+    float x[G], y[G];
+#pragma unroll
+    for (int c = 0; c < G; c++) x[c] = i + c < p.V ? In::one(lg + i + c) : -INFINITY;
+    grad_group<DT, ENTROPY>(p, r, mw, i, x, y);
+    bool mine = r.held >= 0;                       /* no earlier lane has this group */
+#pragma unroll 1
+    for (int k = 0; k < p.given; k++) {
+        const int at = of_lane(r.token, k) - i, first = of_lane(r.held, k);
+        const float add = of_lane(r.g, k) * p.inv_t;
+        mine &= k >= lane || first < i || first >= i + G;
+#pragma unroll
+        for (int c = 0; c < G; c++) y[c] += at == c && !r.none ? add : 0.0f;
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    if (!mine) return;
+#pragma unroll
+    for (int c = 0; c < G; c++)
+        if (i + c < p.V) In::put(lg + i + c, y[c]);
+}
+
+template <int DT, bool ENTROPY>
+int launch_grad_kernels(const GradParams &p, int64_t rows, hipStream_t stream) {
+    const dim3 pieces((unsigned)(rows * p.pieces)), threads(kGradThreads);
+    constexpr int waves = kGradThreads / 64;
+    if (p.grad != p.logits || p.given == 0) {
+        hipLaunchKernelGGL((token_logprobs_grad_kernel<DT, ENTROPY, false>), pieces, threads, 0, stream, p);
+    } else {
+        hipLaunchKernelGGL((token_logprobs_grad_kernel<DT, ENTROPY, true>), pieces, threads, 0, stream, p);
+        hipLaunchKernelGGL((token_logprobs_grad_tokens_kernel<DT, ENTROPY>), dim3((unsigned)((rows + waves - 1) / waves)),
+                           threads, 0, stream, p, (int)rows);
+    }
     return hipGetLastError() == hipSuccess ? DLK_OK : DLK_ERR_HIP;
+}
+
+template <int DT>
+int launch_grad(const GradParams &p, int64_t rows, hipStream_t stream) {
+    return p.h ? launch_grad_kernels<DT, true>(p, rows, stream) : launch_grad_kernels<DT, false>(p, rows, stream);
 }
 
 }  // namespace dlk
@@ -149,10 +231,10 @@ extern "C" int dlk_token_logprobs_grad(const dlk_logprob_grad_batch *b, int rows
     /* (2^32 threads and over are no launch) */
     const int64_t most = 0xffffffLL / p.pieces;
     for (p.r0 = 0; p.r0 < rows; p.r0 += most) {
-        const int64_t blocks = (rows - p.r0 < most ? rows - p.r0 : most) * p.pieces;
-        const int rc = b->dtype == DLK_F32 ? launch_grad<DLK_F32>(p, blocks, stream)
-                     : b->dtype == DLK_BF16 ? launch_grad<DLK_BF16>(p, blocks, stream)
-                                            : launch_grad<DLK_F16>(p, blocks, stream);
+        const int64_t n = rows - p.r0 < most ? rows - p.r0 : most;
+        const int rc = b->dtype == DLK_F32 ? launch_grad<DLK_F32>(p, n, stream)
+                     : b->dtype == DLK_BF16 ? launch_grad<DLK_BF16>(p, n, stream)
+                                            : launch_grad<DLK_F16>(p, n, stream);
         if (rc != DLK_OK) return rc;
     }
     return DLK_OK;

@@ -384,11 +384,12 @@ typedef struct {
 
 /* The logits' gradient of sum_j grad_logprobs[r, j] * logprob[r, j] + grad_entropy[r] * entropy[r]:
  *   grad_v = (1 / T) * (sum_j g_j [v = token_j] - p_v * (sum_j g_j + h * (log p_v + entropy)))
- * in 32 bits, rounded once to dtype; 0 for ids that are not allowed.  The same token
- * may be given several times.  Places without a token, or whose token the mask does not allow, count for
- * nothing.  A row in which nothing is to be differentiated (every g that counts and h are 0, or
- * no logit is allowed): zeros, whatever its logits hold; else a row whose statistics are
- * NaN gets NaN for its allowed ids.  n_top does not matter.  No workspace. */
+ * in 32 bits, rounded once to dtype; 0 for ids that are not allowed or whose logit is -inf.  The same
+ * token may be given several times.  Places without a token, or whose token the mask does not allow or
+ * whose logit is -inf, count for nothing.  A row in which nothing is to be differentiated (every g that
+ * counts and h are 0, or no logit is allowed): zeros, whatever its logits hold; else a row whose statistics
+ * are NaN gets NaN for its allowed ids, but for those whose logit is -inf.  n_top does not matter.  No
+ * workspace. */
 int dlk_token_logprobs_grad(const dlk_logprob_grad_batch *batch, int rows, int vocab, const dlk_logprob_params *params,
                             hipStream_t stream);
 

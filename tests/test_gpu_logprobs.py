@@ -384,6 +384,114 @@ def test_gradient_against_differences(cuda):
         assert ((got[:, v] - want).abs() <= off[:, v] + U * want.abs() + 12 / 0.8 ** 3 * step ** 2 + 1e-10).all()
 
 
+def minus_infinity(rows, V, dtype, given, seed):
+    """Logits of which a third are -inf, tokens among them (the first of each row is one, the last row's all are), two the
+    same where there are more than two; where they are finite."""
+    lg, tokens, gen = some(rows, V, dtype, given, seed=seed, pad=V % 2)
+    dead = torch.rand((rows, V), device="cuda", generator=gen) < 0.3
+    if given > 2:
+        tokens[:, 2] = tokens[:, 0]
+    dead.scatter_(1, tokens[:, 1:].long(), False)
+    dead.scatter_(1, tokens[:, :1].long(), True)
+    dead[-1].scatter_(0, tokens[-1].long(), True)
+    lg[dead] = -math.inf
+    return lg, tokens, ~dead, gen
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,V,given,entropy", [
+    (1, 2, 1, True), (3, 100, 64, True), (2, 4097, 2, False), (5, 9001, 3, True), (3, 50257, 64, False), (300, 777, 1, True),
+    (2, 151936, 64, True)])
+def test_gradient_of_minus_infinity(cuda, dtype, rows, V, given, entropy):
+    """-inf in the logits is a mask: tokens there count for nothing and ids there get zeros, as the same rows masked by
+    bits to the bit; over the logits themselves too, whose tokens other workgroups' stores could reach first."""
+    from diskllm_amd import api
+    lg, tokens, live, gen = minus_infinity(rows, V, dtype, given, V + given)
+    g = torch.randn((rows, given), device="cuda", generator=gen)
+    h = torch.randn(rows, device="cuda", generator=gen) if entropy else None
+    st = api.token_logprobs(lg, tokens)["stats"]
+    got = api.token_logprobs_grad(lg, tokens, st, g, grad_entropy=h)
+    want, off = plain_grad(lg, tokens, g, h, live)               # (the mask in the place of -inf)
+    tiny = torch.finfo(lg.dtype).smallest_normal * torch.finfo(lg.dtype).eps
+    near(got, want, off + HALF[lg.dtype] * (want.abs() + off) + tiny)
+    assert (got[~live] == 0).all()
+    bits = api.token_logprobs_grad(lg, tokens, st, g, grad_entropy=h, mask=allow_words(live))
+    assert torch.equal(got, bits)
+    for _ in range(3):
+        over = torch.empty_strided(lg.shape, lg.stride(), dtype=lg.dtype, device="cuda").copy_(lg)
+        assert api.token_logprobs_grad(over, tokens, st, g, grad_entropy=h, out=over) is over
+        assert torch.equal(over, got)
+
+
+def test_gradient_of_minus_infinity_and_nan(cuda):
+    """A row whose statistics are NaN: NaN, but zeros where its logits are -inf, and everywhere if all that is to be
+    differentiated lies there."""
+    from diskllm_amd import api
+    lg, _, _ = some(3, 9000, "f32", 1)
+    lg[:, ::3] = -math.inf
+    lg[1:, 7] = math.nan
+    tokens = torch.tensor([[3, 5000], [3, 5000], [3, 8001]], dtype=torch.int32, device="cuda")
+    g = torch.ones((3, 2), device="cuda")
+    st = api.token_logprobs(lg, tokens)["stats"]
+    out = api.token_logprobs_grad(lg, tokens, st, g)
+    assert (out[:, ::3] == 0).all() and not out[0].isnan().any() and (out[2] == 0).all()
+    rest = torch.ones(9000, dtype=torch.bool, device="cuda")
+    rest[::3] = False
+    assert out[1, rest].isnan().all()
+    api.token_logprobs_grad(lg, tokens, st, g, out=lg)
+    assert torch.equal(lg.nan_to_num(nan=7.0), out.nan_to_num(nan=7.0))
+
+
+def test_gradient_of_minus_infinity_against_differences(cuda):
+    """Central differences at the finite logits of the 64-bit value over the tokens that have one (their own error as in
+    test_gradient_against_differences)."""
+    from diskllm_amd import api
+    lg, tokens, live, gen = minus_infinity(2, 40, "f32", 3, 4)
+    g = torch.rand((2, 3), device="cuda", generator=gen)
+    h = torch.rand(2, device="cuda", generator=gen)
+    st = api.token_logprobs(lg, tokens, temperature=0.8)["stats"]
+    got = api.token_logprobs_grad(lg, tokens, st, g, grad_entropy=h, temperature=0.8).double().cpu()
+    step = 1e-4
+
+    def value(x):
+        lp, stats, _, _, _ = plain(x, tokens, 0, None, 0.8)
+        return torch.where(lp > -math.inf, lp * g.double().cpu(), 0.0).sum(1) + stats[:, 2] * h.double().cpu()
+    _, off = plain_grad(lg, tokens, g, h, live, 0.8)
+    for v in range(40):
+        up, down = lg.double().clone(), lg.double().clone()
+        up[:, v] += step
+        down[:, v] -= step
+        want = (value(up) - value(down)) / (2 * step)
+        assert ((got[:, v] - want).abs() <= off[:, v] + U * want.abs() + 3 * 12 / 0.8 ** 3 * step ** 2 + 1e-10).all()
+
+
+def test_gradient_in_place_graph(cuda):
+    """In place and captured: replays over new logits, eager calls between them."""
+    from diskllm_amd import api
+    rows, V, given = 4, 30001, 5
+    src, tokens, _, gen = minus_infinity(rows, V, "f32", given, 9)
+    g, h = torch.randn((rows, given), device="cuda", generator=gen), torch.randn(rows, device="cuda", generator=gen)
+    over = torch.empty_like(src)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = api.token_logprobs(src, tokens)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            over.copy_(src)
+            api.token_logprobs(over, tokens, out=out)
+            api.token_logprobs_grad(over, tokens, out["stats"], g, grad_entropy=h, out=over)
+        for k in range(4):
+            src.copy_(torch.where(src > -math.inf, src + 0.25 * k, src).roll(17 * k, 1))
+            graph.replay()
+            st = api.token_logprobs(src, tokens)["stats"]
+            want = api.token_logprobs_grad(src, tokens, st, g, grad_entropy=h)
+            side.synchronize()
+            assert torch.equal(over, want)
+    side.synchronize()
+
+
 # ---- streams, graphs, the path as a whole ------------------------------------------
 
 def test_graph(cuda):
