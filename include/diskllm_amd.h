@@ -360,8 +360,8 @@ typedef struct {
  * above -inf: log-probabilities -inf, statistics -inf, 0, 0 and -inf, no alternatives.  A
  * row whose allowed logits hold NaN or +inf: NaN (ids -1), and DLK_STATUS_NOT_FINITE; what stands in
  * places that are not allowed does not matter.  Exponentials and sums of up to 32 terms in
- * 32 bits, the rest in 64: log-probabilities are off by their own rounding and 1.5e-5 at most
- * at up to 262,144 logits a row (some 2e-7 as measured).  Takes workspace as dlk_sample does
+ * 32 bits, the rest in 64: at up to 262,144 logits a row log-probabilities are off by their own rounding and
+ * 2.2e-5 at most (logits of 16 bits: 1.4e-5; some 2e-7 as measured).  Takes workspace as dlk_sample does
  * where rows are few (dlk_release_stream; one call on the stream before capturing it, else
  * DLK_ERR_HIP).  Outputs may not overlap inputs. */
 int dlk_token_logprobs(const dlk_logprob_batch *batch, int rows, int vocab, const dlk_logprob_params *params,

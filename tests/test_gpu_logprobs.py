@@ -1,5 +1,7 @@
 """dlk_token_logprobs and dlk_token_logprobs_grad against plain forms in 64 bits."""
 import math
+import os
+import re
 
 import pytest
 import torch
@@ -146,6 +148,23 @@ def test_long_rows(cuda):
     few, all_rows = api.token_logprobs(lg[:8], tokens[:8], top=5), api.token_logprobs(lg, tokens, top=5)
     assert torch.equal(few["top_ids"], all_rows["top_ids"][:8])
     near(all_rows["logprobs"][:8], few["logprobs"].double().cpu(), 2 * delta(270_001, torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype,what", [("f32", r"rounding and\s+\*?\s*(\S+) at most"), ("bf16", r"16 bits: ([^;\s]+);"),
+                                        ("f16", r"16 bits: ([^;\s]+);")])
+def test_the_header_s_bound(cuda, dtype, what):
+    """What the header says of 262,144 logits a row is what delta() derives, and holds where every batch's maximum is above
+    all before it, so that each one lowers the sums."""
+    from diskllm_amd import api
+    header = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "diskllm_amd.h")
+    said = float(re.search(what, open(header).read()).group(1))
+    V = 262144
+    assert 0.9 * said <= delta(V, DTYPES[dtype]) <= said
+    lg, tokens, _ = some(300, V, dtype, 3, seed=8, spread=1.0)
+    lg += (torch.arange(V, device="cuda") * (24.0 / V)).to(lg.dtype)
+    got = api.token_logprobs(lg, tokens)["logprobs"][::50]
+    want = plain(lg[::50], tokens[::50], 0)[0]
+    near(got, want, said + U * want.abs())
 
 
 def test_mask_rows_shared(cuda):
