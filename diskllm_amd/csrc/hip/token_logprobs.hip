@@ -364,11 +364,12 @@ __global__ __launch_bounds__(kLogprobThreads, 4) void token_logprobs_kernel(Logp
         uint64_t bound = (uint64_t)bound_key << 32;
         float least = bound_key != 0 ? key_value(~bound_key) : -INFINITY;
         /* each thread's own records that hold entries, in order, so that of equal logits the lower ids are there first:
-         * a round of loads for as many threads as have one left, one or two rounds in all */
+         * a round of loads for as many threads as have one left, one or two rounds in all.  (0x7f is -inf's, 0x80 the
+         * lowest float's: where there is no bound, records without an allowed logit are still none) */
+        const uint32_t reaches = max(bound_key >> 16, 0x80u);
         uint64_t records = 0;
 #pragma unroll 4
-        for (int r = 0; r * group < count; r++)
-            records |= (uint64_t)(best_of[r * T] >= (uint32_t)(bound_key >> 16)) << r;
+        for (int r = 0; r * group < count; r++) records |= (uint64_t)(best_of[r * T] >= reaches) << r;
         if (bad) records = 0;
         int of_record = 0;
 #pragma unroll 1

@@ -356,7 +356,8 @@ typedef struct {
 } dlk_logprob_params;
 
 /* log p_v = l_v / T - log(sum_u exp(l_u / T)) over the ids that the mask allows (-inf for
- * the others); the entropy -sum p log p.  The logits are read once.  A row without an allowed logit
+ * the others); the entropy -sum p log p.  The logits are read once, with alternatives those near them
+ * again (where too many are equal, all).  A row without an allowed logit
  * above -inf: log-probabilities -inf, statistics -inf, 0, 0 and -inf, no alternatives.  A
  * row whose allowed logits hold NaN or +inf: NaN (ids -1), and DLK_STATUS_NOT_FINITE; what stands in
  * places that are not allowed does not matter.  Exponentials and sums of up to 32 terms in

@@ -167,6 +167,52 @@ def test_the_header_s_bound(cuda, dtype, what):
     near(got, want, said + U * want.abs())
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,V", [(3, 40_000), (300, 9_000), (2, 600_001)])
+@pytest.mark.parametrize("bits", [True, False])
+def test_fewer_allowed_than_alternatives(cuda, dtype, rows, V, bits):
+    """Rows that allow nothing, the type's lowest value alone, or a few ids, masked by bits or by -inf."""
+    lg, tokens, g = some(rows, V, dtype, 2, seed=V + rows)
+    allow = torch.zeros((rows, V), dtype=torch.bool, device="cuda")
+    lowest = torch.tensor([0, V // 2, V - 1], device="cuda")
+    allow[1, lowest] = True
+    lg[1, lowest] = torch.finfo(DTYPES[dtype]).min
+    if rows > 2:
+        allow[2:].scatter_(1, torch.randint(0, V, (rows - 2, 9), device="cuda", generator=g), True)
+        allow[2:].scatter_(1, tokens[2:, :1].long(), True)
+    if not bits:
+        lg[~allow] = -math.inf
+    check(lg, tokens, 20, allow if bits else None)
+
+
+@pytest.mark.parametrize("dtype,V", [("f32", 270_001), ("f32", 800_003), ("bf16", 530_001), ("f16", 1_100_000)])
+def test_long_rows_of_one_workgroup(cuda, dtype, V):
+    """Rows of more batches than a workgroup keeps records of, one workgroup each: many alternatives, ties, few allowed
+    ids, none."""
+    from diskllm_amd import api
+    rows, top = 257, 40
+    lg, tokens, g = some(rows, V, dtype, 2, seed=V, spread=1.0)
+    lg[3, 5::V // 90] = 11.0                                     # more of the same than there are alternatives
+    lg[4] = 0.5
+    lg[5, :V - 70] = -math.inf
+    lg[6] = -math.inf
+    lg[7, :] = -math.inf
+    lg[7, V - 1] = 2.0
+    lg[8] = torch.finfo(DTYPES[dtype]).min
+    at = [0, 3, 4, 5, 6, 7, 8, rows - 1]
+    allow = torch.rand((2, V), device="cuda", generator=g) < 0.5
+    of = torch.arange(rows, device="cuda", dtype=torch.int32) % 2
+    d = delta(V, DTYPES[dtype])
+    for mask in (None, allow_words(allow)):
+        got = api.token_logprobs(lg, tokens, top=top, mask=mask, mask_row=of)
+        lp, stats, ids, tl, _ = plain(lg[at], tokens[at], top, None if mask is None else allow[of[at].long()])
+        assert torch.equal(got["top_ids"][at].cpu().long(), ids)
+        near(got["top_logprobs"][at], tl, d + U * tl.abs())
+        near(got["logprobs"][at], lp, d + U * lp.abs())
+        near(got["stats"][at, 1], stats[:, 1], (d + U) * stats[:, 1])
+        near(got["stats"][at, 2], stats[:, 2], d * (2 * math.log(V) + 2) + U * stats[:, 2])
+
+
 def test_mask_rows_shared(cuda):
     """mask_row names the mask of each row."""
     lg, tokens, g = some(6, 5000, "f32", 1)
