@@ -498,7 +498,8 @@ def dequantize_mx(q: torch.Tensor, scale: torch.Tensor, n: Optional[int] = None,
                   dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None,
                   stream: Optional[int] = None) -> torch.Tensor:
     """The first n values (all) of rows of blocks as [rows, n] of dtype; with ids int32 those rows of the table, zeros
-    for an id that it does not have: the embedding rows of tokens (dlk_dequantize_mx)."""
+    for an id that it does not have: the embedding rows of tokens (dlk_dequantize_mx).  A table without rows has none to
+    give: ids of one are refused."""
     dev = q.get_device()
     table, blocks, fmt, ldq, lds = _blocks_of(q, scale, dev, "q")
     n = blocks * 32 if n is None else n
@@ -509,6 +510,7 @@ def dequantize_mx(q: torch.Tensor, scale: torch.Tensor, n: Optional[int] = None,
         rows = ids.numel()
         _want(rows >> 31 == 0, _WIDE.format("dequantize_mx"))
         at = _flat(ids, 0, dev, _I32, "ids")
+        _want(table > 0 or rows == 0, "q: a table with rows is wanted")
     if out is None:
         _want(dtype in _DTYPES, "dtype: float32, bfloat16 or float16 is wanted")
         ld = n

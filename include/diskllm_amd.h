@@ -307,8 +307,8 @@ int dlk_quantize_mx(const void *x, int dtype, int64_t ldx, int rows, int n, int 
 /* The values of rows of blocks, n of each, in `dtype` (rounded to the nearest, halves to even, where
  * it does not hold them): out[r * ld + i] of row ids[r] of the table q, or of row r where ids is
  * NULL: with ids the embedding rows of tokens from a tied table.  An id outside [0,
- * table_rows) gives zeros (rows <= table_rows without ids).  Alignment as above; of out its
- * elements'. */
+ * table_rows) gives zeros; rows <= table_rows without ids, and a table without rows is refused
+ * (DLK_ERR_INVALID) where rows > 0, with ids too.  Alignment as above; of out its elements'. */
 int dlk_dequantize_mx(const uint8_t *q, int64_t ldq, const uint8_t *scale, int64_t ld_scale, int table_rows,
                       const int32_t *ids, int rows, int n, int format, void *out, int dtype, int64_t ld,
                       hipStream_t stream);

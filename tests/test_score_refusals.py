@@ -210,6 +210,14 @@ def test_counts_past_32_bits(on_no_device):
     assert on_no_device == []
 
 
+def test_table_without_rows(on_no_device):
+    """Has no row to give zeros for: refused with ids as in C, nothing to do without any."""
+    with pytest.raises(ValueError):
+        api.dequantize_mx(u8(0, 32), u8(0, 2), ids=i32(3))
+    assert api.dequantize_mx(u8(0, 32), u8(0, 2), ids=i32(0)).shape == api.dequantize_mx(u8(0, 32), u8(0, 2)).shape == (0, 64)
+    assert on_no_device == []
+
+
 @pytest.mark.parametrize("current,stream,made_on", [(111, 222, 222), (111, 0, 0), (111, 111, None), (111, None, None)])
 def test_outputs_are_made_on_the_calls_stream(on_no_device, monkeypatch, current, stream, made_on):
     """Outputs that a call makes come from the memory of the stream that writes them."""
