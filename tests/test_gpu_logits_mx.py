@@ -105,6 +105,19 @@ def test_quantize_special_blocks(cuda, fmt):
 
 
 @pytest.mark.parametrize("fmt", ["fp4", "fp6"])
+@pytest.mark.parametrize("top", [-126, -120, -60, -10, -3, 0, 3, 30, 100, 127])
+def test_quantize_every_bfloat16(cuda, fmt, top):
+    """Every bfloat16 up to a block's largest, whose exponent is `top`."""
+    import torch
+    v = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    v = v[v.isfinite()]
+    v = v[v.double().abs() < 2.0 ** (top + 1)]
+    v = torch.cat((v, v.new_zeros(-len(v) % 31))).view(-1, 31)
+    x = torch.cat((torch.full((len(v), 1), 2.0 ** top, dtype=torch.bfloat16), v), 1)
+    check_quantized(torch, x.cuda(), fmt)
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp6"])
 def test_quantize_into_strided(cuda, fmt):
     """Into rows of other strides; what lies between the rows is left."""
     import torch
@@ -275,6 +288,40 @@ def test_nan_blocks_stay_in_their_rows(cuda, rows, n):
     bad[1] = True
     bad[:, 299] = True
     assert torch.equal(got.isnan(), bad)
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp6"])
+@pytest.mark.parametrize("rows", [1, 16, 32, 64, 100, 200, 300, 500])
+@pytest.mark.parametrize("n", [200, 1024])
+@pytest.mark.parametrize("cap", [0.5, 30.0, 1e-39])
+def test_product_capped_of_every_tile(cuda, fmt, rows, n, cap):
+    """The cap in both formats at rows of every tile, rows of whole and of part steps."""
+    import torch
+    check_product(torch, *inputs(torch, rows, 301, n, fmt, seed=rows, spread=0), fmt, softcap=cap)
+
+
+@pytest.mark.parametrize("fmt", ["fp4", "fp6"])
+@pytest.mark.parametrize("rows", [2, 16, 32, 64, 100, 200, 300, 500])
+@pytest.mark.parametrize("n", [96, 1024, 1500])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+def test_nan_blocks_of_every_tile(cuda, fmt, rows, n, cap):
+    """A scale of 255 in a row's last block, in one of hidden states in the middle and in one of weights; behind a row's end
+    it is none."""
+    import torch
+    from diskllm_amd import api
+    vocab = 300
+    x, xs, w, ws = inputs(torch, rows, vocab, n, fmt)
+    xs[rows - 1, 1] = 255
+    ws[7, -1] = 255
+    ws[299, 0] = 255
+    got = api.logits_mx(x, xs, w, ws, softcap=cap)
+    bad = torch.zeros((rows, vocab), dtype=torch.bool, device="cuda")
+    bad[rows - 1] = True
+    bad[:, [7, 299]] = True
+    assert torch.equal(got.isnan(), bad)
+    xs[0, -1] = 255
+    bad[0] = True
+    assert torch.equal(api.logits_mx(x, xs, w, ws, softcap=cap).isnan(), bad)
 
 
 def test_far_scales(cuda):
