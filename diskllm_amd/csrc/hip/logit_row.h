@@ -55,18 +55,19 @@ struct LogitRow<DLK_F32> {
  * goes to memory twice (100,001 rows of 4,090 bfloat16: 208 us past them, 183 through). */
 inline bool whole_lines(const void *p, int64_t ld) { return (((uintptr_t)p | (uintptr_t)ld) & 127) == 0; }
 
-/* Stores v, past the caches where `past`: what the next call would not find there anyway, as
- * large outputs, is written at the memory's rate (8,192 x 4,096 float32 dequantised: 44 us
+/* Stores v at p of ALIGN bytes' alignment, past the caches where `past`: what the next call would not find
+ * there anyway, as large outputs, is written at the memory's rate (8,192 x 4,096 float32 dequantised: 44 us
  * through the caches, 23.5 past them). */
-template <class V>
-DLK_DEV void store_past(V *p, V v, bool past) {
+template <int ALIGN, class V>
+DLK_DEV void store_past(void *p, V v, bool past) {
+    typedef V Any __attribute__((aligned(ALIGN)));
     if (past) {
         /* (apart from the other store, or the compiler makes one plain store of the two) */
         asm volatile("" ::: "memory");
-        __builtin_nontemporal_store(v, p);
+        __builtin_nontemporal_store(v, (Any *)p);
         asm volatile("" ::: "memory");
     } else {
-        *p = v;
+        *(Any *)p = v;
     }
 }
 

@@ -49,7 +49,7 @@ DLK_DEV void write_sums(const MxParams &p, const f4 (&acc)[MF][NF], int m0, int 
         if (r >= p.rows) return;
         float *out = p.logits + (int64_t)r * p.ld + v;
         if (v + 3 < p.vocab) {
-            store_past((f4_any *)out, f4_any{y[0], y[1], y[2], y[3]}, p.past);
+            store_past<4>(out, f4{y[0], y[1], y[2], y[3]}, p.past);
         } else {
 #pragma unroll
             for (int c = 0; c < 3; c++)

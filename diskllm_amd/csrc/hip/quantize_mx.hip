@@ -140,7 +140,7 @@ __global__ __launch_bounds__(kMxThreads) void quantize_mx_kernel(const typename 
         const int64_t block = unit[s] >> 2;
         const int part = (int)(unit[s] & 3);
         if (FMT == DLK_MX_FP4) {
-            store_past((uint32_t *)(q + row[s] * ldq + block * 16 + part * 4), w0, past);
+            store_past<4>(q + row[s] * ldq + block * 16 + part * 4, w0, past);
         } else {
             /* three of a block's four threads store eight bytes each */
             const uint32_t n0 = quad<kQuadNext>(w0), n1 = quad<kQuadNext>(w1);
@@ -224,7 +224,7 @@ __global__ __launch_bounds__(kMxThreads) void dequantize_mx_kernel(const uint8_t
         const int i = (int)unit[s] * G;
         typename Out::T *o = out + row[s] * ld + i;
         if (i + G <= n) {
-            store_past((typename Out::Raw *)o, Out::pack(v), past);
+            store_past<sizeof(*o)>(o, Out::pack(v), past);
         } else {
 #pragma unroll
             for (int c = 0; c < G; c++)

@@ -139,7 +139,7 @@ __global__ __launch_bounds__(kGradThreads) void token_logprobs_grad_kernel(GradP
         }
         if (OVER && !mine) continue;
         if (i + G <= s1) {
-            store_past((typename In::Raw *)(out + i), In::pack(y), p.past);
+            store_past<sizeof(*out)>(out + i, In::pack(y), p.past);
         } else {
 #pragma unroll
             for (int c = 0; c < G; c++)
