@@ -79,6 +79,14 @@ DLK_DEV double exp_neg(double x) {
     return __hiloint2double(__double2hiint(y) + (__double2loint(t) << 20), __double2loint(y));
 }
 
+/* The larger of three (NaN: of the others): one instruction, where fmaxf makes one for each
+ * value to quiet it. */
+DLK_DEV float max3(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+
 /* Ascending key of a double (no NaN); zero below every one. */
 DLK_DEV uint64_t double_key(double d) {
     uint64_t u = d2u(d);
@@ -101,6 +109,17 @@ DLK_DEV float beam_penalised(const BeamParams &p, float x, int cnt) {
         }
     }
     return x;
+}
+
+/* A key that at least r of the lanes' keys reach (0: fewer than r lanes have one): the largest
+ * for r = 1, else the largest of 20 leading bits (0.5 us where few waves run). */
+DLK_DEV uint32_t wave_rth(uint32_t a, int r) {
+    uint32_t K = 0;
+    if (r == 1) return wave_minmax_u32<false>(a);
+#pragma unroll 1
+    for (uint32_t bit = 0x80000000u; bit >= 0x1000u; bit >>= 1)
+        if ((int)__popcll(ballot(a >= (K | bit))) >= r) K |= bit;
+    return K;
 }
 
 /* Maximum over each row of 16 lanes (every lane gets its row's). */
@@ -157,6 +176,24 @@ DLK_DEV bool before(uint64_t ka, int ra, uint64_t ea, uint64_t kb, int rb, uint6
     if (ka != kb) return ka > kb;
     if (ra != rb) return ra < rb;
     return ea > eb;
+}
+
+/* How many of list[0 .. n) are above v, and how many equal to it. */
+DLK_DEV int rank_in(const uint64_t *list, int n, uint64_t v, int &equal) {
+    int above = 0;
+    equal = 0;
+    int c = 0;
+    for (; c + 4 <= n; c += 4) {
+        const ulonglong2 a = *(const ulonglong2 *)&list[c], b = *(const ulonglong2 *)&list[c + 2];
+        above += (a.x > v ? 1 : 0) + (a.y > v ? 1 : 0) + (b.x > v ? 1 : 0) + (b.y > v ? 1 : 0);
+        equal += (a.x == v ? 1 : 0) + (a.y == v ? 1 : 0) + (b.x == v ? 1 : 0) + (b.y == v ? 1 : 0);
+    }
+    for (; c < n; c++) {
+        const uint64_t a = list[c];
+        above += a > v ? 1 : 0;
+        equal += a == v ? 1 : 0;
+    }
+    return above;
 }
 
 /* What a row adds to its continuations, out of LDS once for many of them. */

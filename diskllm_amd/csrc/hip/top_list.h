@@ -20,29 +20,10 @@ DLK_DEV float allowed_or_ninf(float x, uint32_t bits, int c) {
     return u2f((f2u(x) & m) | (0xff800000u & ~m));
 }
 
-/* The larger of three (NaN: of the others): one instruction, where fmaxf makes one for each
- * value to quiet it. */
-DLK_DEV float max3(float a, float b, float c) {
-    float d;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-    return d;
-}
-
 /* An entry of a list: larger is better (the logit's ascending key, then the lower id). */
 DLK_DEV uint64_t entry_of(float l, int id) { return (uint64_t)~desc_key(l) << 32 | (uint32_t)~id; }
 DLK_DEV float entry_logit(uint64_t e) { return key_value(~(uint32_t)(e >> 32)); }
 DLK_DEV int entry_id(uint64_t e) { return (int)~(uint32_t)e; }
-
-/* A key that at least r of the lanes' keys reach (0: fewer than r lanes have one): the largest
- * for r = 1, else the largest of 20 leading bits (0.5 us where few waves run). */
-DLK_DEV uint32_t wave_rth(uint32_t a, int r) {
-    uint32_t K = 0;
-    if (r == 1) return wave_minmax_u32<false>(a);
-#pragma unroll 1
-    for (uint32_t bit = 0x80000000u; bit >= 0x1000u; bit >>= 1)
-        if ((int)__popcll(ballot(a >= (K | bit))) >= r) K |= bit;
-    return K;
-}
 
 /* Lane's place among the lanes of `who`, from `first` on. */
 DLK_DEV int place_in(uint64_t who, int first) {
@@ -53,24 +34,6 @@ DLK_DEV int place_in(uint64_t who, int first) {
 DLK_DEV void wave_order() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
-}
-
-/* How many of list[0 .. n) are above v, and how many equal to it. */
-DLK_DEV int rank_in(const uint64_t *list, int n, uint64_t v, int &equal) {
-    int above = 0;
-    equal = 0;
-    int c = 0;
-    for (; c + 4 <= n; c += 4) {
-        const ulonglong2 a = *(const ulonglong2 *)&list[c], b = *(const ulonglong2 *)&list[c + 2];
-        above += (a.x > v ? 1 : 0) + (a.y > v ? 1 : 0) + (b.x > v ? 1 : 0) + (b.y > v ? 1 : 0);
-        equal += (a.x == v ? 1 : 0) + (a.y == v ? 1 : 0) + (b.x == v ? 1 : 0) + (b.y == v ? 1 : 0);
-    }
-    for (; c < n; c++) {
-        const uint64_t a = list[c];
-        above += a > v ? 1 : 0;
-        equal += a == v ? 1 : 0;
-    }
-    return above;
 }
 
 }  // namespace dlk
