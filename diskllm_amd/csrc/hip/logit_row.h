@@ -51,6 +51,14 @@ struct LogitRow<DLK_F32> {
     DLK_DEV static void put(T *p, float v) { *p = v; }
 };
 
+/* Eight values at p. */
+template <int DT>
+DLK_DEV void load8(const typename LogitRow<DT>::T *p, float (&v)[8]) {
+    typedef LogitRow<DT> In;
+#pragma unroll
+    for (int k = 0; k < 8 / In::G; k++) In::unpack(*(const typename In::Raw *)(p + k * In::G), v + k * In::G);
+}
+
 /* Whether rows at p, ld bytes apart, begin with cache lines: past the caches a line that two waves write
  * goes to memory twice (100,001 rows of 4,090 bfloat16: 208 us past them, 183 through). */
 inline bool whole_lines(const void *p, int64_t ld) { return (((uintptr_t)p | (uintptr_t)ld) & 127) == 0; }

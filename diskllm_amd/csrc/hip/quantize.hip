@@ -19,41 +19,14 @@
  */
 #include <hip/hip_runtime.h>
 
-#include "dlk_device.h"
-#include "../../../include/diskllm_amd.h"
+#include "logit_row.h"
 
 namespace dlk {
 
 constexpr int kQuantThreads = 256;
 constexpr int kQuantKeep = 4;             /* groups of eight that a thread keeps in registers */
 
-typedef float f8_any __attribute__((ext_vector_type(8), aligned(4)));
-typedef uint16_t h8_any __attribute__((ext_vector_type(8), aligned(2)));
 typedef uint32_t u2_any __attribute__((ext_vector_type(2), aligned(1)));
-
-template <int DT>
-struct QuantIn {
-    typedef uint16_t T;
-    DLK_DEV static float one(const uint16_t *p) {
-        return DT == DLK_BF16 ? u2f((uint32_t)*p << 16) : (float)__builtin_bit_cast(_Float16, *p);
-    }
-    DLK_DEV static void eight(const uint16_t *p, float (&v)[8]) {
-        const h8_any h = *(const h8_any *)p;
-#pragma unroll
-        for (int c = 0; c < 8; c++)
-            v[c] = DT == DLK_BF16 ? u2f((uint32_t)h[c] << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h[c]);
-    }
-};
-template <>
-struct QuantIn<DLK_F32> {
-    typedef float T;
-    DLK_DEV static float one(const float *p) { return *p; }
-    DLK_DEV static void eight(const float *p, float (&v)[8]) {
-        const f8_any x = *(const f8_any *)p;
-#pragma unroll
-        for (int c = 0; c < 8; c++) v[c] = x[c];
-    }
-};
 
 /* x / scale to the nearest integer, halves to even, within +-127.  inv: the rounded
  * 1 / scale, 0 where that would leave the range of a float (scale below 1e-30: the
@@ -73,11 +46,11 @@ DLK_DEV int quantized(float x, float scale, float inv) {
 
 /* TPR threads to a row. */
 template <int DT, int TPR>
-__global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const typename QuantIn<DT>::T *__restrict__ x,
+__global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const typename LogitRow<DT>::T *__restrict__ x,
                                                                  int64_t ldx, int rows, int n,
                                                                  int8_t *__restrict__ q, int64_t ldq,
                                                                  float *__restrict__ scale) {
-    typedef QuantIn<DT> In;
+    typedef LogitRow<DT> In;
     __shared__ uint32_t part[kQuantThreads / 64];
     const int t = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * (kQuantThreads / TPR) + threadIdx.x / TPR;
@@ -90,7 +63,7 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const typename 
     for (int j = 0; j < kQuantKeep; j++) {
         const int i = (t + j * TPR) * 8;
         if (i + 8 <= n) {
-            In::eight(xr + i, v[j]);
+            load8<DT>(xr + i, v[j]);
         } else {
 #pragma unroll
             for (int c = 0; c < 8; c++) v[j][c] = i + c < n ? In::one(xr + i + c) : 0.0f;
@@ -140,7 +113,7 @@ __global__ __launch_bounds__(kQuantThreads) void quantize_kernel(const typename 
 template <int DT>
 int launch_quantize(const void *x, int64_t ldx, int rows, int n, int8_t *q, int64_t ldq, float *scale,
                     hipStream_t stream) {
-    typedef const typename QuantIn<DT>::T *P;
+    typedef const typename LogitRow<DT>::T *P;
     /* short rows: a wave each */
     if (n <= 1024)
         hipLaunchKernelGGL((quantize_kernel<DT, 64>), dim3((unsigned)((rows + 3) / 4)), dim3(kQuantThreads), 0, stream,

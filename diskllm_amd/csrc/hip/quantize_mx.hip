@@ -36,13 +36,6 @@ DLK_DEV void mx_place(uint64_t first, uint32_t per, int lane, int64_t &row, uint
     unit = u;
 }
 
-template <int DT>
-DLK_DEV void load8(const typename LogitRow<DT>::T *p, float (&v)[8]) {
-    typedef LogitRow<DT> In;
-#pragma unroll
-    for (int k = 0; k < 8 / In::G; k++) In::unpack(*(const typename In::Raw *)(p + k * In::G), v + k * In::G);
-}
-
 /* The larger of a and |b|, |c|; NaN where one is NaN. */
 DLK_DEV float maximum_abs(float a, float b, float c) {
     float d;
