@@ -43,7 +43,7 @@ constexpr int kMaxTopKLds = 4096;          /* larger top-k: candidates in global
 constexpr int kHcapDirect = 1024;          /* longer histories: penalties applied to a scratch copy first */
 constexpr size_t kFullWorkspace = (size_t)512 << 20;      /* workspace per launch of the fused kernel */
 constexpr size_t kGlobalTopkBudget = (size_t)256 << 20;   /* workspace per launch of the large-k row kernel */
-constexpr size_t kBeamWorkspace = (size_t)64 << 20;       /* workspace per launch of the beam selection, of scoring */
+constexpr size_t kBeamWorkspace = (size_t)64 << 20;       /* workspace per launch of the beam selection */
 constexpr int kLsdWords = 256 + 16 * 256 + 16;            /* select_top_k_global's LDS words */
 
 size_t r16(size_t b) { return (b + 15) & ~(size_t)15; }
@@ -734,8 +734,8 @@ extern "C" int dlk_beam_select(const dlk_beam_batch *b, int groups, int vocab, c
     return DLK_OK;
 }
 
-/* Tokens scored (token_logprobs.hip), the rows in as many launches as the workspace's bound
- * asks for; rows of one workgroup each need none. */
+/* Tokens scored (token_logprobs.hip).  Rows of one workgroup each need no workspace; those of several are 256 at most
+ * (logprob_slices()), a launch and 270 KB at most. */
 extern "C" int dlk_token_logprobs(const dlk_logprob_batch *b, int rows, int vocab, const dlk_logprob_params *prm,
                                   hipStream_t stream) {
     using namespace dlk;
@@ -765,17 +765,14 @@ extern "C" int dlk_token_logprobs(const dlk_logprob_batch *b, int rows, int voca
     p.slices = logprob_slices(rows, p.batches);
     p.cap = p.n > 0 ? std::min(p.n + 12, DLK_MAX_ALTERNATIVES) : 0;
     const size_t per = (size_t)p.slices * (sizeof(LogprobSlot) + (size_t)p.cap * 8);
-    /* (2^32 threads and over are no launch) */
-    int64_t most = 0xffffff / p.slices;
-    if (p.slices > 1 && most > (int64_t)(kBeamWorkspace / per)) most = (int64_t)(kBeamWorkspace / per);
-    const int step = most < rows ? (int)most : rows;
+    const int step = std::min(rows, 0xffffff / p.slices);    /* (2^32 threads and over are no launch) */
     std::lock_guard<std::mutex> lock(g_mu);
     if (p.slices > 1) {
         WsView ws;
-        if (!workspace(stream, 0, (size_t)step, (size_t)step * per, ws)) return ws_status();
+        if (!workspace(stream, 0, (size_t)rows, (size_t)rows * per, ws)) return ws_status();
         p.counters = ws.counters;
         p.slots = (LogprobSlot *)ws.data;
-        p.cands = (uint64_t *)(ws.data + (size_t)step * p.slices * sizeof(LogprobSlot));
+        p.cands = (uint64_t *)(ws.data + (size_t)rows * p.slices * sizeof(LogprobSlot));
     }
     for (p.r0 = 0; p.r0 < rows; p.r0 += step) {
         const int n = rows - p.r0 < step ? rows - p.r0 : step;
