@@ -557,6 +557,33 @@ def test_gradient_in_place_graph(cuda):
     side.synchronize()
 
 
+def test_more_rows_than_a_launch(cuda):
+    """2^24 rows and more, a workgroup each."""
+    from diskllm_amd import api
+    rows, V = (1 << 24) + 70_001, 3
+    g = torch.Generator("cuda").manual_seed(2)
+    lg = torch.randn((rows, V), device="cuda", generator=g)
+    tokens = torch.randint(0, V, (rows,), device="cuda", generator=g, dtype=torch.int32)
+    got = api.token_logprobs(lg, tokens, top=1)
+    w = torch.ones((rows, 1), device="cuda")
+    grad = api.token_logprobs_grad(lg, tokens, got["stats"], w)
+    d = delta(V, torch.float32)
+    for a in range(0, rows, 1 << 22):
+        s = slice(a, min(a + (1 << 22), rows))
+        lp = torch.log_softmax(lg[s].double(), 1)
+        want = lp.gather(1, tokens[s, None].long())[:, 0]
+        assert ((got["logprobs"][s].double() - want).abs() <= d + U * want.abs()).all()
+        first = torch.where(lg[s] == lg[s].amax(1, keepdim=True), torch.arange(V, device="cuda"), V).amin(1)
+        assert torch.equal(got["top_ids"][s, 0].long(), first)
+        p = lp.exp()
+        want = torch.nn.functional.one_hot(tokens[s].long(), V) - p
+        # (as plain_grad's, of one token of weight 1, and half a step of the result)
+        off = p * (U * (4 * (math.log(V) - lp) + 80) + 3 * d) + U * 70
+        assert ((grad[s].double() - want).abs() <= off + U * want.abs()).all()
+    api.token_logprobs_grad(lg, tokens, got["stats"], w, out=lg)
+    assert torch.equal(lg, grad)
+
+
 # ---- streams, graphs, the path as a whole ------------------------------------------
 
 def test_graph(cuda):
