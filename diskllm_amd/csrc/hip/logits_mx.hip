@@ -12,11 +12,12 @@
  * scales' row, picked by the instruction.  w is its first operand, as in logits_i8.hip.
  *
  * Bounds.  Few rows: w's bytes, as there (16 x 151,936 x 4,096 in 66 us with 6-bit hidden states, 5.1 TB/s; a large
- * copy: 4.9).  Many: the products and what feeds them, 512 x 262,144 x 4,096 in 380 us, 390-412 with the cap, of which
- * some 80 write 537 MB after each workgroup's loop; between n = 4,096 and 8,192 3.56 PFLOP/s (a library product of
- * 16,384^3 in this format, written in 16 bits: 3.32 in all).  The loop has the matrix cores busy for 40% of its cycles
- * at a clock that falls to some 1.8 GHz; its LDS reads met none of the same bank once chunks lay as mx_spot() has them,
- * which changed nothing, nor did more stages of half the length.
+ * copy: 4.9).  Many: the products and what feeds them, 512 x 262,144 x 4,096 in 380 us, 390-412 with the cap (24 such
+ * calls one after another 388 to 518), of which some 80 write 537 MB after each workgroup's loop; between n = 4,096 and
+ * 8,192 3.56 PFLOP/s (a library product of 16,384^3 in this format, written in 16 bits: 3.32 in all).  The matrix cores
+ * are busy for 28 to 33% of a capped call's cycles (40% of the loop's), at a clock that goes from 2.1 down to 1.65 GHz
+ * as such calls follow one another; the loop's LDS reads met none of the same bank once chunks lay as mx_spot() has
+ * them, which changed nothing, nor did more stages of half the length.
  */
 #include <math.h>
 
@@ -449,8 +450,8 @@ int launch_mx_tiles(const MxParams &p, hipStream_t stream) {
      *   300         128 x 128 198, 332; 256 x 256 210, -; 128 x 256 220, 241
      *   512         256 x 256 by quarters 229; at once 234, -; 128 x 256 314, 354; 128 x 128 286, 458
      * (128 x 256 in 6 bits: a wave has 32 rows of 128 ids; with 64 of 64 120, 178, 252, 399.  256 x 256 at once: 64
-     * rows of 128 ids; with 128 of 64 as long, and 200 x 50,257 x 1,024 24.2 for 22.5.  Two stages of 256 rows in 6
-     * bits do not fit LDS) */
+     * rows of 128 ids; with 128 of 64 as long, and 200 x 50,257 x 1,024 24.2 for 22.5.  In 6 bits two stages of 256 x
+     * 256 take 208 KB in steps of eight blocks, more than LDS has; in steps of four 112: not built) */
     if (p.rows <= 16) return launch_mx<FMT, 16, 64, 1, 4, 16, 2>(p, stream);
     if (p.rows <= 32) return launch_mx<FMT, 32, 128, 1, 4, 8, 3>(p, stream);
     if (FMT == DLK_MX_FP6) {

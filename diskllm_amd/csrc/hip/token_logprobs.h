@@ -55,7 +55,17 @@ struct LogprobParams {
  *   64 x 151,936    1: 28.7, 2: 21.7, 4: 18.0, 8: 18.2, 13: 19.7, 37: 35.8
  *   128 x 50,257    1: 16.0, 2: 15.5, 4: 16.8, 9: 21.1
  *   256 x 151,936   1: 48.9, 2: 42.7, 4: 42.5, 8: 47.6
- *   300 x 50,257    1: 20.4, 2: 22.7, 4: 29.9 */
+ *   300 x 50,257    1: 20.4, 2: 22.7, 4: 29.9
+ * without alternatives
+ *   1 x 32,000      1: 6.8, 2: 6.0, 4: 5.0, 8: 4.8
+ *   8 x 151,936     4: 9.4, 8: 7.0, 18: 6.6, 25: 6.9, 37: 8.0
+ *   16 x 151,936    8: 7.7, 12: 7.9, 16: 8.1, 24: 9.3, 37: 11.7
+ *   64 x 151,936    1: 23.9, 2: 15.4, 4: 11.4, 6: 11.1, 8: 11.6, 13: 13.5
+ *   128 x 50,257    1: 10.9, 2: 9.7, 3: 9.5, 4: 9.8, 9: 11.1
+ *   256 x 151,936   1: 37.0, 2: 27.6, 4: 28.8, 8: 30.7
+ *   300 x 50,257    1: 13.6, 2: 15.7, 4: 17.4;  x 151,936 39.2, 36.8, 37.4
+ * of 64
+ *   8 x 151,936     4: 19.5, 8: 17.1, 18: 20.6, 25: 22.3;  64 x 151,936 2: 26.3, 4: 20.9, 6: 21.9, 8: 22.3 */
 inline int logprob_slices(int64_t rows, int batches) {
     int64_t s = rows > 256 ? 1 : (384 + rows / 2) / rows;
     if (rows > 4 && s > (batches * 2 + 2) / 3) s = (batches * 2 + 2) / 3;

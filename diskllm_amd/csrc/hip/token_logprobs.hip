@@ -187,6 +187,8 @@ DLK_DEV void join_row(const LogprobParams &p, ScoreShared &sh, int rl, int32_t t
             best = max(best, ent[q]);
         }
         uint32_t bound = 0;
+        /* few entries are all ranked, without a bound first (us without / with: 64 x 151,937 of 5 alternatives, 102
+         * entries, 17.5 / 18.1; 1 x 32,000 of 20, 256, 11.3 / 10.3; 8 x 151,936 of 5, 425, 17.5 / 11.8) */
         if (E > 96) bound = score_bound(sh, (uint32_t)(best >> 32), p.n);
         else __syncthreads();
         auto gather = [&](uint64_t least) {

@@ -379,7 +379,8 @@ typedef struct {
     const float *stats;       /* [rows, 4] as dlk_token_logprobs has left them */
     const float *grad_logprobs;  /* [rows, n_given] */
     const float *grad_entropy;   /* [rows], or NULL: 0 */
-    void *grad;               /* [rows, ld_grad] of dtype: written; may be the logits themselves (ld_grad == ld) */
+    void *grad;               /* [rows, ld_grad] of dtype: written; the logits themselves (ld_grad == ld) or apart from
+                                    them */
     int64_t ld_grad;
 } dlk_logprob_grad_batch;
 
