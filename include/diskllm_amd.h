@@ -316,7 +316,8 @@ int dlk_dequantize_mx(const uint8_t *q, int64_t ldq, const uint8_t *scale, int64
 /* logits[r * ld + v] = sum over the ceil(n / 32) blocks of x's row r (x_format) and w's row v
  * (FP4) of their values' products; softcap as in dlk_logits_i8.  The products of a block are
  * exact, sums are in 32 bits: off by at most 2^-20 of the sum of the products' sizes for each
- * 512 values or part of them (four sums).  A block with scale 255 makes its row's logits NaN.
+ * 512 values or part of them (four sums); products below 2^-149 may count as 0.  A block with
+ * scale 255 makes its row's logits NaN.
  * x, w and the scales: 16-byte aligned (x in FP6: 8), strides too (the bytes of a row of
  * scales up to the next multiple of 16 are read; what stands there does not matter).  Entries
  * past vocab in a row of logits are left as they are; logits may not overlap the inputs. */

@@ -340,6 +340,24 @@ def test_far_scales(cuda):
     assert ((got == want) | ((got - want).abs() <= 2.0 ** -149)).all()
 
 
+@pytest.mark.parametrize("fmt", ["fp4", "fp6"])
+@pytest.mark.parametrize("rows", [4, 40, 100, 200, 300])
+@pytest.mark.parametrize("n", [128, 1000])
+def test_tiny_products(cuda, fmt, rows, n):
+    """Sums of equal products down to 2^-149, exact; below that no more than they are."""
+    import torch
+    from diskllm_amd import api
+    vocab, blocks = 300, (n + 31) // 32
+    w = torch.full((vocab, blocks * 16), 0x22, dtype=torch.uint8, device="cuda")                  # ones
+    x, _ = api.quantize_mx(torch.ones((rows, blocks * 32), device="cuda"), fmt)                   # 4.0
+    for total in (-126, -140, -149, -150, -153, -160, -200):
+        e = 127 + (total - 2) // 2
+        xs = torch.full((rows, (blocks + 15) // 16 * 16), e, dtype=torch.uint8, device="cuda")[:, :blocks]
+        ws = torch.full((vocab, (blocks + 15) // 16 * 16), 254 + total - 2 - e, dtype=torch.uint8, device="cuda")[:, :blocks]
+        got, want = api.logits_mx(x, xs, w, ws).double(), blocks * 32 * 2.0 ** total
+        assert (got == want).all() if total >= -149 else ((got >= 0) & (got <= want + 2.0 ** -150)).all(), total
+
+
 def test_offsets_past_32_bits(cuda):
     """A table of more than 2^32 bytes and logits of more than 2^32 bytes."""
     import torch
