@@ -618,7 +618,8 @@ def token_logprobs_grad(logits: torch.Tensor, tokens: Optional[torch.Tensor], st
                         temperature: float = 1.0, out: Optional[torch.Tensor] = None,
                         stream: Optional[int] = None) -> torch.Tensor:
     """The gradient of the logits, in their type, of token_logprobs' logprobs and entropy, given theirs
-    (dlk_token_logprobs_grad); stats as the forward call left them, out = logits: in place."""
+    (dlk_token_logprobs_grad); stats as the forward call left them, out = logits: in place.  A token or id whose logit is
+    -inf counts as one that the mask does not allow."""
     dev, dt, rows, V, ld, given, at, mk, mask_ld, mr = _scored(logits, tokens, mask, mask_row)
     st = _flat(stats, rows * 4, dev, _F32, "stats")
     _want(given == 0 or grad_logprobs is not None, "grad_logprobs: a value for each token is wanted")
