@@ -13,10 +13,10 @@
  *
  * Bounds.  Few rows: w's bytes, as there (16 x 151,936 x 4,096 in 66 us with 6-bit hidden states, 5.1 TB/s; a large
  * copy: 4.9).  Many: the products and what feeds them, 512 x 262,144 x 4,096 in 380 us, 390-412 with the cap (24 such
- * calls one after another 388 to 518), of which some 80 write 537 MB after each workgroup's loop; between n = 4,096 and
+ * calls one after another 385 to 520), of which some 80 write 537 MB after each workgroup's loop; between n = 4,096 and
  * 8,192 3.56 PFLOP/s (a library product of 16,384^3 in this format, written in 16 bits: 3.32 in all).  The matrix cores
- * are busy for 28 to 33% of a capped call's cycles (40% of the loop's), at a clock that goes from 2.1 down to 1.65 GHz
- * as such calls follow one another; the loop's LDS reads met none of the same bank once chunks lay as mx_spot() has
+ * are busy for 28 to 33% of a capped call's cycles (40% of the loop's), at a clock that goes from 2.1 down to 1.8 GHz
+ * or less as such calls follow one another; the loop's LDS reads met none of the same bank once chunks lay as mx_spot() has
  * them, which changed nothing, nor did more stages of half the length.
  */
 #include <math.h>
